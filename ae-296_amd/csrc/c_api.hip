@@ -8,6 +8,7 @@
 
 #include "../../include/mlora.h"
 #include "mlora_args.hpp"
+#include "mlora_step.hpp"
 
 namespace {
 
@@ -96,6 +97,12 @@ int check_dims(int hin, int hout)
 }  // namespace
 
 namespace mlora {
+
+int fail_text(int code, const char *fmt, va_list ap)
+{
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    return code;
+}
 
 int device_compute_units()
 {

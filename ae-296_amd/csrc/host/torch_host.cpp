@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -51,7 +52,9 @@ struct Ref {        // an owned reference
 
 PyObject *s_page_tbl, *s_rank, *s_scaling, *s_work, *s_group, *s_perm, *s_seg_start, *s_seg_len, *s_seg_adapter,
     *s_chunk_start, *s_chunk_len, *s_chunk_adapter, *s_counters, *s_row_off, *s_tok_rank, *s_tok_scale, *s_T, *s_workspace,
-    *s_n_slots, *s_max_pages, *s_page_rows, *s_n_pages, *s_max_rank, *s_tok_adapter, *s_dtype_code, *s_projections, *s_a_rows, *s_b_rows, *s_buf;
+    *s_n_slots, *s_max_pages, *s_page_rows, *s_n_pages, *s_max_rank, *s_tok_adapter, *s_dtype_code, *s_projections, *s_a_rows, *s_b_rows, *s_buf,
+    *s_packed, *s_hin, *s_hout, *s_has_zeros, *s_tok_req, *s_tok_pos, *s_pages, *s_req_prefix, *s_prefix_pages, *s_prefix_len, *s_k, *s_v,
+    *s_cos_sin, *s_interleaved, *s_batch, *s_n_q_heads, *s_n_kv_heads, *s_page_tokens;
 
 void *attr_ptr(PyObject *o, PyObject *name)          // data pointer of a tensor attribute, null for None
 {
@@ -440,6 +443,250 @@ PyObject *sgmv_multi(PyObject *const *v, Py_ssize_t nargs)
     return PyLong_FromLong(rc);
 }
 
+// ---------------------------------------------------------------- the decode step around the LoRA apply
+// A launch goes to the current device's current stream, so every tensor of the call has to be there.
+void need_here(const at::Tensor &t)
+{
+    need_device(t);
+    if (t.get_device() != c10::hip::current_device())
+        raise(PyExc_ValueError, "a tensor is on device %d, the current device is %d", (int)t.get_device(), (int)c10::hip::current_device());
+}
+
+int dtype_of(const at::Tensor &t)
+{
+    if (t.scalar_type() == at::kHalf) return MLORA_F16;
+    if (t.scalar_type() == at::kBFloat16) return MLORA_BF16;
+    raise(PyExc_TypeError, "mlora kernels take float16 or bfloat16 tensors");
+}
+
+struct Attr {       // an attribute that is a tensor, or None
+    Ref r;
+    Attr(PyObject *o, PyObject *name) : r(PyObject_GetAttr(o, name)) {}
+    bool none() const { return r.o == Py_None; }
+    const at::Tensor &t() const { return tensor(r.o); }
+};
+
+// w4_gemv(ys, xs, weights, accumulate)
+PyObject *w4_gemv(PyObject *const *v, Py_ssize_t nargs)
+{
+    if (nargs != 4) raise(PyExc_TypeError, "w4_gemv takes 4 arguments");
+    const List ys(v[0]), xs(v[1]);
+    const Ref ws(PySequence_Fast(v[2], "expected a sequence of W4Weight"));
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(ws.o);
+    if (n < 1 || n > MLORA_MAX_PROJ || ys.size() != n || xs.size() != n)
+        raise(PyExc_ValueError, "need 1..%d projections with one y, one x and one weight each", MLORA_MAX_PROJ);
+    for (Py_ssize_t i = 0; i < n; i++) { need_device(ys[i]); need_device(xs[i]); }
+    for (Py_ssize_t i = 0; i < n; i++) { need_contiguous(ys[i]); need_contiguous(xs[i]); }
+    const at::ScalarType type = xs[0].scalar_type();
+    const int dtype = dtype_of(xs[0]);
+    if (xs[0].dim() != 2) raise(PyExc_ValueError, "x must be [T, hin]");
+    const int64_t T = xs[0].size(0);
+    void *y[MLORA_MAX_PROJ];
+    const void *x[MLORA_MAX_PROJ], *packed[MLORA_MAX_PROJ];
+    int32_t hin[MLORA_MAX_PROJ], hout[MLORA_MAX_PROJ], group[MLORA_MAX_PROJ], zeros[MLORA_MAX_PROJ];
+    for (Py_ssize_t i = 0; i < n; i++) {
+        PyObject *w = PySequence_Fast_GET_ITEM(ws.o, i);
+        const Attr buf(w, s_packed);
+        const at::Tensor &b = buf.t(), &yt = ys[i], &xt = xs[i];
+        hin[i] = (int32_t)attr_int(w, s_hin);
+        hout[i] = (int32_t)attr_int(w, s_hout);
+        group[i] = (int32_t)attr_int(w, s_group);
+        const Ref has(PyObject_GetAttr(w, s_has_zeros));
+        zeros[i] = is_true(has.o);
+        if (yt.scalar_type() != type || xt.scalar_type() != type || attr_int(w, s_dtype_code) != dtype)
+            raise(PyExc_TypeError, "x, y and the weights' scales must share one 16-bit dtype");
+        if (xt.dim() != 2 || yt.dim() != 2 || xt.size(0) != T || xt.size(1) != hin[i] || yt.size(0) != T || yt.size(1) != hout[i])
+            raise(PyExc_ValueError, "projection %d: expected x [%lld, %d] and y [%lld, %d]", (int)i, (long long)T, (int)hin[i], (long long)T, (int)hout[i]);
+        if (b.scalar_type() != at::kByte || !b.is_contiguous() || b.numel() < mlora_w4_packed_bytes(hin[i], hout[i], group[i], zeros[i]))
+            raise(PyExc_ValueError, "projection %d: the packed weight is not what its sizes need", (int)i);
+        need_here(xt);
+        need_here(yt);
+        need_here(b);
+        y[i] = yt.data_ptr(); x[i] = xt.data_ptr(); packed[i] = b.data_ptr();
+    }
+    if (T > (1 << 20)) raise(PyExc_ValueError, "at most 2^20 tokens");
+    return PyLong_FromLong(launch(mlora_w4_gemv_multi, (int)n, y, x, packed, hin, hout, group, zeros, (int)T, dtype, (int)is_true(v[3]), stream()));
+}
+
+// The tables and token lists of a KVBatch.
+struct Batch {
+    const int32_t *tok_req, *tok_pos, *page_tbl, *req_prefix = nullptr, *prefix_tbl = nullptr, *prefix_len = nullptr;
+    int T, n_req, max_pages, n_prefix = 0, max_prefix_pages = 0;
+};
+
+const int32_t *int_table(const at::Tensor &t, PyObject *name, int dims)
+{
+    need_device(t);
+    if (t.scalar_type() != at::kInt) raise(PyExc_TypeError, "%U must be int32", name);
+    if (t.dim() != dims) raise(PyExc_ValueError, "%U must have %d dimension(s)", name, dims);
+    need_contiguous(t);
+    need_here(t);
+    for (int d = 0; d < dims; d++)
+        if (t.size(d) > 0x7fffffffLL) raise(PyExc_ValueError, "%U is too large", name);
+    return static_cast<const int32_t *>(t.data_ptr());
+}
+
+Batch batch_of(PyObject *o)
+{
+    Batch b;
+    const Attr req(o, s_tok_req), pos(o, s_tok_pos), pages(o, s_pages), of(o, s_req_prefix), ppages(o, s_prefix_pages), plen(o, s_prefix_len);
+    b.tok_req = int_table(req.t(), s_tok_req, 1);
+    b.tok_pos = int_table(pos.t(), s_tok_pos, 1);
+    b.page_tbl = int_table(pages.t(), s_pages, 2);
+    b.T = (int)req.t().size(0);
+    b.n_req = (int)pages.t().size(0);
+    b.max_pages = (int)pages.t().size(1);
+    if (pos.t().size(0) != b.T) raise(PyExc_ValueError, "tok_req and tok_pos must have the same length");
+    if (of.none() != plen.none()) raise(PyExc_ValueError, "req_prefix and prefix_len go together");
+    if (of.none()) {
+        if (!ppages.none()) raise(PyExc_ValueError, "prefix_pages without req_prefix");
+        return b;
+    }
+    b.req_prefix = int_table(of.t(), s_req_prefix, 1);
+    b.prefix_len = int_table(plen.t(), s_prefix_len, 1);
+    b.n_prefix = (int)plen.t().size(0);
+    if (of.t().size(0) != b.n_req) raise(PyExc_ValueError, "req_prefix must have one entry for every row of pages");
+    if (!ppages.none()) {
+        b.prefix_tbl = int_table(ppages.t(), s_prefix_pages, 2);
+        b.max_prefix_pages = (int)ppages.t().size(1);
+        if (ppages.t().size(0) != b.n_prefix) raise(PyExc_ValueError, "prefix_pages and prefix_len must have the same length");
+    }
+    return b;
+}
+
+struct Cache {
+    void *k, *v;
+    int64_t n_pages;
+    int page_tokens, n_kv_heads, head_dim, dtype;
+    at::ScalarType type;
+};
+
+Cache cache_of(PyObject *o, int64_t layer)
+{
+    const Attr ka(o, s_k), va(o, s_v);
+    const at::Tensor &k = ka.t(), &v = va.t();
+    need_here(k);
+    need_here(v);
+    if (k.dim() != 5 || v.dim() != 5 || !k.is_contiguous() || !v.is_contiguous() || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type())
+        raise(PyExc_ValueError, "the cache's k and v must be contiguous [n_layers, n_pages, n_kv_heads, page_tokens, head_dim] tensors of one type");
+    if (layer < 0 || layer >= k.size(0)) raise(PyExc_IndexError, "layer %lld outside the cache's %lld layers", (long long)layer, (long long)k.size(0));
+    const int64_t at = layer * k.stride(0) * k.element_size();
+    return {static_cast<char *>(k.data_ptr()) + at, static_cast<char *>(v.data_ptr()) + at, k.size(1), (int)k.size(3), (int)k.size(2), (int)k.size(4),
+            dtype_of(k), k.scalar_type()};
+}
+
+// Data pointer of [T, heads, head_dim] with only the tokens apart, and the elements from token to token.
+void *token_rows(const char *name, const at::Tensor &t, int64_t T, int64_t heads, const Cache &c, int64_t &stride)
+{
+    need_device(t);
+    if (t.scalar_type() != c.type) raise(PyExc_TypeError, "%s must have the cache's dtype", name);
+    if (t.dim() != 3 || t.size(0) != T || t.size(1) != heads || t.size(2) != c.head_dim)
+        raise(PyExc_ValueError, "%s must be [%lld, %lld, %d]", name, (long long)T, (long long)heads, c.head_dim);
+    if (t.stride(2) != 1 || (heads > 1 && t.stride(1) != c.head_dim)) raise(PyExc_ValueError, "the heads of a token of %s must lie one behind the other", name);
+    need_here(t);
+    stride = T > 1 ? t.stride(0) : heads * c.head_dim;
+    return t.data_ptr();
+}
+
+// kv_append(q or None, k, v, q_out or None, cache, layer, batch, rope or None, bad or None)
+PyObject *kv_append(PyObject *const *v, Py_ssize_t nargs)
+{
+    if (nargs != 9) raise(PyExc_TypeError, "kv_append takes 9 arguments");
+    const Cache c = cache_of(v[4], as_int(v[5]));
+    const Batch b = batch_of(v[6]);
+    int64_t q_stride = 0, o_stride = 0, k_stride, v_stride, q_heads = c.n_kv_heads;
+    const void *q = nullptr;
+    void *q_out = nullptr;
+    if (v[0] != Py_None) {
+        const at::Tensor &qt = tensor(v[0]);
+        q_heads = qt.dim() == 3 ? qt.size(1) : 0;
+        q = token_rows("q", qt, b.T, q_heads, c, q_stride);
+        q_out = v[3] == Py_None ? const_cast<void *>(q) : token_rows("q_out", tensor(v[3]), b.T, q_heads, c, o_stride);
+        if (v[3] == Py_None) o_stride = q_stride;
+    } else if (v[3] != Py_None) {
+        raise(PyExc_ValueError, "q_out without q");
+    }
+    const void *k = token_rows("k", tensor(v[1]), b.T, c.n_kv_heads, c, k_stride), *val = token_rows("v", tensor(v[2]), b.T, c.n_kv_heads, c, v_stride);
+    const float *cos_sin = nullptr;
+    int n_pos = 0, rot = 0, interleaved = 0;
+    if (v[7] != Py_None) {
+        const Attr table(v[7], s_cos_sin);
+        const at::Tensor &t = table.t();
+        need_here(t);
+        if (t.scalar_type() != at::kFloat || t.dim() != 2 || !t.is_contiguous()) raise(PyExc_ValueError, "the rotation's table must be contiguous float32 [n_pos, rot]");
+        const Ref inter(PyObject_GetAttr(v[7], s_interleaved));
+        cos_sin = static_cast<const float *>(t.data_ptr());
+        n_pos = (int)(t.size(0) < 0x7fffffffLL ? t.size(0) : 0x7fffffffLL);
+        rot = (int)t.size(1);
+        interleaved = is_true(inter.o);
+    }
+    int32_t *bad = nullptr;
+    if (v[8] != Py_None) {
+        const at::Tensor &t = tensor(v[8]);
+        need_here(t);
+        if (t.scalar_type() != at::kInt || t.numel() < 1) raise(PyExc_ValueError, "bad must be an int32 tensor of one value");
+        bad = static_cast<int32_t *>(t.data_ptr());
+    }
+    return PyLong_FromLong(launch(mlora_kv_append, q, q_stride, q_out, o_stride, k, k_stride, val, v_stride, c.k, c.v, c.n_pages, c.page_tokens, (int)q_heads,
+                                  c.n_kv_heads, c.head_dim, b.tok_req, b.tok_pos, b.T, b.page_tbl, b.n_req, b.max_pages, b.req_prefix, b.prefix_len,
+                                  b.n_prefix, cos_sin, n_pos, rot, interleaved, bad, c.dtype, stream()));
+}
+
+void need_prefix_pages(const Batch &b)
+{
+    if (b.n_prefix > 0 && !b.prefix_tbl) raise(PyExc_ValueError, "attention over shared prefixes needs prefix_pages");
+}
+
+void *plan_buf(const at::Tensor &t)
+{
+    need_here(t);
+    if (t.scalar_type() != at::kByte || !t.is_contiguous()) raise(PyExc_ValueError, "the plan's buf must be a contiguous uint8 buffer");
+    return t.data_ptr();
+}
+
+// attn_plan(batch, buf, page_tokens, n_q_heads, n_kv_heads)
+PyObject *attn_plan(PyObject *const *v, Py_ssize_t nargs)
+{
+    if (nargs != 5) raise(PyExc_TypeError, "attn_plan takes 5 arguments");
+    const Batch b = batch_of(v[0]);
+    need_prefix_pages(b);
+    const at::Tensor &buf = tensor(v[1]);
+    return PyLong_FromLong(launch(mlora_attn_plan, b.tok_req, b.tok_pos, b.T, b.n_req, b.max_pages, b.req_prefix, b.prefix_len, b.n_prefix,
+                                  b.max_prefix_pages, (int)as_int(v[2]), (int)as_int(v[3]), (int)as_int(v[4]), plan_buf(buf), buf.numel(), stream()));
+}
+
+// prefix_attention(q, out, cache, layer, plan, scale)
+PyObject *prefix_attention(PyObject *const *v, Py_ssize_t nargs)
+{
+    if (nargs != 6) raise(PyExc_TypeError, "prefix_attention takes 6 arguments");
+    PyObject *plan = v[4];
+    const Cache c = cache_of(v[2], as_int(v[3]));
+    const Ref batch(PyObject_GetAttr(plan, s_batch));
+    const Batch b = batch_of(batch.o);
+    need_prefix_pages(b);
+    const int64_t q_heads = attr_int(plan, s_n_q_heads);
+    if (attr_int(plan, s_n_kv_heads) != c.n_kv_heads || attr_int(plan, s_page_tokens) != c.page_tokens || attr_int(plan, s_T) != b.T)
+        raise(PyExc_ValueError, "the plan was made for another cache layout or batch size");
+    int64_t q_stride, o_stride;
+    const void *q = token_rows("q", tensor(v[0]), b.T, q_heads, c, q_stride);
+    void *out = token_rows("out", tensor(v[1]), b.T, q_heads, c, o_stride);
+    const Attr bufa(plan, s_buf);
+    const at::Tensor &buf = bufa.t();
+    const void *pb = plan_buf(buf);
+    const double scale = PyFloat_AsDouble(v[5]);
+    if (scale == -1.0 && PyErr_Occurred()) throw PyFail();
+    // this call's own, as in bgmv_ref
+    const int64_t bytes = mlora_attn_workspace_bytes(b.T, b.n_prefix, (int)q_heads, c.n_kv_heads, c.head_dim);
+    at::DataPtr room;
+    if (b.T > 0 && bytes > 0) {
+        const c10::DeviceGuard device(buf.device());
+        room = c10::GetAllocator(at::kCUDA)->allocate((size_t)bytes);
+    }
+    return PyLong_FromLong(launch(mlora_prefix_attention, out, o_stride, q, q_stride, static_cast<const void *>(c.k), static_cast<const void *>(c.v), c.n_pages, c.page_tokens, (int)q_heads, c.n_kv_heads,
+                                  c.head_dim, b.tok_req, b.tok_pos, b.T, b.page_tbl, b.n_req, b.max_pages, b.req_prefix, b.prefix_tbl, b.prefix_len, b.n_prefix,
+                                  b.max_prefix_pages, (float)scale, pb, buf.numel(), room.get(), bytes, c.dtype, stream()));
+}
+
 // ---------------------------------------------------------------- module
 template <PyObject *(*F)(PyObject *const *, Py_ssize_t)>
 PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t nargs)
@@ -456,7 +703,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 
 #define MLORA_FN(name) {#name, (PyCFunction)(void (*)())entry<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MLORA_FN(gather), MLORA_FN(bgmv), MLORA_FN(bgmv_ref), MLORA_FN(deltas_ref), MLORA_FN(order), MLORA_FN(state), MLORA_FN(prefill_plan),
-                         MLORA_FN(sgmv_multi), {nullptr, nullptr, 0, nullptr}};
+                         MLORA_FN(sgmv_multi), MLORA_FN(w4_gemv), MLORA_FN(kv_append), MLORA_FN(attn_plan), MLORA_FN(prefix_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native launch path of mlora's eager calls.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -470,7 +717,11 @@ PyMODINIT_FUNC PyInit__host()
         {&s_row_off, "row_off"}, {&s_tok_rank, "tok_rank"}, {&s_tok_scale, "tok_scale"}, {&s_T, "T"}, {&s_workspace, "workspace"},
         {&s_n_slots, "n_slots"}, {&s_max_pages, "max_pages"}, {&s_page_rows, "page_rows"}, {&s_n_pages, "n_pages"},
         {&s_max_rank, "max_rank"}, {&s_tok_adapter, "tok_adapter"}, {&s_dtype_code, "dtype_code"}, {&s_projections, "projections"},
-        {&s_a_rows, "a_rows"}, {&s_b_rows, "b_rows"}, {&s_buf, "buf"}};
+        {&s_a_rows, "a_rows"}, {&s_b_rows, "b_rows"}, {&s_buf, "buf"},
+        {&s_packed, "packed"}, {&s_hin, "hin"}, {&s_hout, "hout"}, {&s_has_zeros, "has_zeros"}, {&s_tok_req, "tok_req"},
+        {&s_tok_pos, "tok_pos"}, {&s_pages, "pages"}, {&s_req_prefix, "req_prefix"}, {&s_prefix_pages, "prefix_pages"},
+        {&s_prefix_len, "prefix_len"}, {&s_k, "k"}, {&s_v, "v"}, {&s_cos_sin, "cos_sin"}, {&s_interleaved, "interleaved"},
+        {&s_batch, "batch"}, {&s_n_q_heads, "n_q_heads"}, {&s_n_kv_heads, "n_kv_heads"}, {&s_page_tokens, "page_tokens"}};
     for (const auto &p : names)
         if (!(*p.first = PyUnicode_InternFromString(p.second))) return nullptr;
     return PyModule_Create(&module);

@@ -1,0 +1,99 @@
+// Kernel argument blocks and launchers of the decode step around the LoRA apply: 4-bit base projections, cache appends,
+// shared-prefix attention.
+#pragma once
+#include <cstdarg>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mlora {
+
+constexpr int STEP_MAX_PROJ = 8;
+
+// ---- 4-bit weights.  A packed weight is three planes: codes, scales, zero points.
+// Codes: tiles of 16 columns x 128 rows, 1024 bytes each, column tile major (a column tile's K tiles lie one behind the other).  In a
+// tile, lane l = 16 * q + c of a wavefront owns 16 bytes: dword s holds rows 32 s + 8 q + j (j < 8) of column c, row pair
+// (2i, 2i + 1) in nibbles i and i + 4 - the operand of one 16 x 16 x 32 MFMA.  Rows and columns past the weight's are zero codes.
+// Scales: [groups, columns rounded up to 16] 16-bit; zero points: the same in bytes.
+constexpr int W4_TN = 16, W4_TK = 128, W4_TILE_BYTES = W4_TN * W4_TK / 2;
+struct W4Shape {
+    int hin, hout, group;
+    int n_tiles, k_tiles, groups, cols;    // column tiles, K tiles, groups of a column, columns rounded up
+    int64_t scales_at, zeros_at, bytes;    // byte offsets of the planes (zeros_at: -1 where there are none), total
+};
+inline W4Shape w4_shape(int hin, int hout, int group, bool zeros)
+{
+    W4Shape s;
+    s.hin = hin; s.hout = hout; s.group = group;
+    s.n_tiles = (hout + W4_TN - 1) / W4_TN;
+    s.k_tiles = (hin + W4_TK - 1) / W4_TK;
+    s.groups = (hin + group - 1) / group;
+    s.cols = s.n_tiles * W4_TN;
+    s.scales_at = (int64_t)s.n_tiles * s.k_tiles * W4_TILE_BYTES;
+    const int64_t after = s.scales_at + (int64_t)s.groups * s.cols * 2;
+    s.zeros_at = zeros ? after : -1;
+    s.bytes = zeros ? after + (int64_t)s.groups * s.cols : after;
+    return s;
+}
+
+struct W4PackArgs {
+    const uint8_t *codes;
+    const uint16_t *scales;
+    const uint8_t *zeros;
+    unsigned char *packed;
+    W4Shape sh;
+};
+
+struct W4Proj {
+    void *y;
+    const void *x;
+    const unsigned char *codes;
+    const uint16_t *scales;
+    const uint8_t *zeros;      // nullptr: 8
+    int hin, hout, cols, k_tiles, n_tiles;
+    int group_shift;           // log2 of the group
+    int groups;
+};
+struct W4Args {
+    W4Proj pr[STEP_MAX_PROJ];
+    int n_proj, T, accumulate;
+};
+
+// ---- keys and values
+struct KvBatch {
+    const int32_t *tok_req, *tok_pos;
+    const int32_t *page_tbl;
+    const int32_t *req_prefix;     // nullptr: no request has a prefix
+    const int32_t *prefix_tbl, *prefix_len;
+    int T, n_req, max_pages, n_prefix, max_prefix_pages;
+};
+struct KvAppendArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t *q_out, *k_pages, *v_pages;
+    int64_t q_stride, q_out_stride, k_stride, v_stride;
+    int64_t n_pages;
+    int page_shift, n_q_heads, n_kv_heads, head_dim;
+    KvBatch b;
+    const float *cos_sin;
+    int n_pos, rot, interleaved;
+    int32_t *bad;
+};
+struct AttnArgs {
+    uint16_t *out;
+    const uint16_t *q, *k_pages, *v_pages;
+    int64_t out_stride, q_stride;
+    int64_t n_pages;
+    int page_shift, n_q_heads, n_kv_heads, head_dim, gq;   // gq: query heads per key head
+    KvBatch b;
+    float scale;
+};
+
+int launch_w4_pack(const W4PackArgs &a, hipStream_t s);
+int launch_w4_gemv(const W4Args &a, int dtype, hipStream_t s);
+int launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s);
+int launch_prefix_attention(const AttnArgs &a, int dtype, hipStream_t s);
+
+// sets the calling thread's error text and returns `code` (defined with the other entry points)
+int fail_text(int code, const char *fmt, va_list ap);
+int device_compute_units();
+
+}  // namespace mlora

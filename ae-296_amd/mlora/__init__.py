@@ -6,6 +6,7 @@ and raises if it has not been built.
 """
 from . import _ext, cpu_ops
 from ._ext import MloraError
+from .attention import AttnPlan, KVBatch, KVCache, RopeTable, kv_append, plan_attention, prefix_attention
 from .cold_start import ColdStartPrefill
 from .loader import AdapterLoader, HostAdapter, LoadTicket, layer_order
 from .lora_cpu import Lora_CPU
@@ -13,6 +14,8 @@ from .lora_gpu import Lora_GPU
 from .ops import (DecodePlan, PrefillPlan, RefDecodePlan, SideStream, side_by_side, add_lora_bgmv, add_lora_bgmv_multi, plan_decode_ref, bgmv, gemm_lora, lora_apply, lora_prefill_ref, plan_decode,
                   plan_prefill, sgmv, sgmv_multi, sgmv_workspace)
 from .pool import AdapterPool
+from .w4 import W4Weight, w4_gemv, w4_quantize
 
 __all__ = ["ColdStartPrefill", "AdapterLoader", "AdapterPool", "HostAdapter", "LoadTicket", "layer_order", "DecodePlan", "SideStream", "side_by_side", "Lora_CPU", "Lora_GPU", "MloraError", "RefDecodePlan", "add_lora_bgmv", "add_lora_bgmv_multi", "plan_decode_ref", "bgmv", "gemm_lora", "lora_apply",
-           "lora_prefill_ref", "plan_decode", "plan_prefill", "PrefillPlan", "sgmv", "sgmv_multi", "sgmv_workspace", "_ext", "cpu_ops"]
+           "lora_prefill_ref", "plan_decode", "plan_prefill", "PrefillPlan", "sgmv", "sgmv_multi", "sgmv_workspace",
+           "AttnPlan", "KVBatch", "KVCache", "RopeTable", "kv_append", "plan_attention", "prefix_attention", "W4Weight", "w4_gemv", "w4_quantize", "_ext", "cpu_ops"]

@@ -25,6 +25,7 @@ GATHER_MAX_T = 8192
 CNT_NSEG, CNT_NVALID, CNT_NCHUNK, CNT_BAD, CNT_WORDS = 0, 1, 2, 3, 8
 WORK_WORDS = 80
 SCATTER_MAX_JOBS = 16
+ATTN_MAX_T = 8192                   # MLORA_ATTN_MAX_T
 NOALLOC_SCRATCH_BYTES = 16 << 20    # MLORA_NOALLOC_SCRATCH_BYTES
 
 
@@ -78,6 +79,16 @@ SIGNATURES = {
     "mlora_gemm_lora_partial_bytes": (_i64, [_i32, _vp, _vp, _i32]),
     "mlora_gemm_lora_split": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _i32,
                                      _i32, _i32, _i64, _i32, _i32, _vp, _i64, _vp, _i64, _vp]),
+    "mlora_w4_packed_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "mlora_w4_pack": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "mlora_w4_gemv_multi": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
+    "mlora_kv_append": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i32,
+                               _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _i32, _vp]),
+    "mlora_attn_plan_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "mlora_attn_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "mlora_attn_plan": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "mlora_prefix_attention": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp,
+                                      _vp, _vp, _i32, _i32, _f32, _vp, _i64, _vp, _i64, _i32, _vp]),
     "mlora_prefill_reflayout": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
 }
 

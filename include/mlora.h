@@ -427,6 +427,83 @@ int mlora_prefill_reflayout(void *y, const void *x, const void *A_T, const void 
                             int B, int Lpad, int L, int r, int hin, int hout, int layer_idx,
                             int dtype, void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * ---- The decode step around the LoRA apply: base projections on 4-bit weights, keys and values, attention ----
+ *
+ * Base projections on 4-bit weights, for the decode tokens whose LoRA deltas mlora_bgmv_multi adds:
+ *     y_p[t][n] = (accumulate ? y_p[t][n] : 0) + sum_g s_p[g][n] * sum_{k in group g} (c_p[k][n] - z_p[g][n]) * x_p[t][k]
+ * with codes c in 0..15, a 16-bit scale for every `group` (32, 64 or 128) rows of a column and a zero point z in 0..15 (8
+ * where none are given).  hin and hout are multiples of 8; the last group of a column may be shorter.  Products and sums in
+ * fp32, rounded once.
+ *   mlora_w4_pack lays codes (uint8 [hin, hout], one code a byte, the low four bits count), scales ([groups, hout], of the type
+ *     the calls will use) and zeros (uint8 [groups, hout], or NULL) out as the kernel reads them: mlora_w4_packed_bytes(...)
+ *     bytes, 16-byte aligned, once per weight; the sources are not needed afterwards.
+ *   mlora_w4_gemv_multi takes y, x, packed, hin, hout, group and zeros (0 / 1: packed with zero points) as HOST arrays of n_proj
+ *     entries.  Any T; made for the few rows of a decode batch (the weights are read once for every 64 of them).
+ * No counterpart in the reference's LoRA path (its int4 base GEMMs: dequantize_gemm_int4.py:32,225,345).
+ */
+int64_t mlora_w4_packed_bytes(int hin, int hout, int group, int zeros);
+int mlora_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int hin, int hout, int group,
+                  void *packed, int64_t packed_bytes, void *stream);
+int mlora_w4_gemv_multi(int n_proj, void *const *y, const void *const *x, const void *const *packed,
+                        const int32_t *hin, const int32_t *hout, const int32_t *group, const int32_t *zeros,
+                        int T, int dtype, int accumulate, void *stream);
+
+/*
+ * Paged key/value cache (one slab each for keys and values per layer): [n_pages, n_kv_heads, page_tokens, head_dim] 16-bit
+ * floats, 16-byte aligned; page_tokens a power of two in 16..256, head_dim 64 or 128.
+ * A batch names, for every token t, its request tok_req[t] (int32; negative: a row without a request, which is left alone
+ * everywhere) and its position tok_pos[t] in that request's sequence.  Request r may follow a shared prefix
+ * req_prefix[r] in [0, n_prefix) (any other value, or req_prefix NULL: none) of prefix_len[...] tokens; its own keys lie on the pages
+ * page_tbl[r][0 .. max_pages), position prefix_len + i on page i / page_tokens at row i mod page_tokens, those of prefix f on
+ * prefix_tbl[f][0 .. max_prefix_pages).  Tables and lengths are device int32.
+ *
+ * mlora_kv_append: rotates q and k by their positions, writes q_out, and places k and v on the pages of their tokens:
+ *     for the pairs i < rot / 2 of a head, (u, w) = elements (i, i + rot / 2), or (2i, 2i + 1) where interleaved:
+ *     (u cos a - w sin a, u sin a + w cos a), a = the angle of (position, i) in cos_sin (fp32 [n_pos, rot]: cosines of a position,
+ *     then its sines); elements from rot on, and all of v, unchanged.  rot a multiple of 16 up to head_dim, or 0 (cos_sin NULL).
+ *   q [T, n_q_heads, head_dim], k and v [T, n_kv_heads, head_dim] with *_stride elements from token to token (multiples of 8, so
+ *   that they may be views of one fused projection output); q_out may be q itself, otherwise they must not overlap; q and
+ *   q_out may both be NULL.  Computed in fp32, rounded once.  A token whose request or position no table holds, or whose page
+ *   id is outside [0, n_pages), is left out as a whole and counted in *bad (device int32, or NULL).  (request, position)
+ *   pairs must differ: of two equal ones either may be kept.
+ * Replaces rotary_emb_fwd and destindex_copy_kv of the reference's layer (rotary_emb.py:8, destindex_copy_kv.py:8).
+ */
+int mlora_kv_append(const void *q, int64_t q_stride, void *q_out, int64_t q_out_stride, const void *k, int64_t k_stride,
+                    const void *v, int64_t v_stride, void *k_pages, void *v_pages, int64_t n_pages, int page_tokens,
+                    int n_q_heads, int n_kv_heads, int head_dim, const int32_t *tok_req, const int32_t *tok_pos, int T,
+                    const int32_t *page_tbl, int n_req, int max_pages, const int32_t *req_prefix, const int32_t *prefix_len,
+                    int n_prefix, const float *cos_sin, int n_pos, int rot, int interleaved, int32_t *bad, int dtype,
+                    void *stream);
+
+/*
+ * Attention of a batch's tokens over that cache, the keys of a shared prefix read once for all the tokens behind it:
+ *     out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j,  j over positions 0 .. tok_pos[t] of t's request,
+ * query head h reading key head h / (n_q_heads / n_kv_heads).  Scores, softmax statistics and sums in fp32; the softmax weights are
+ * rounded to the 16-bit type for their product with v; the result is rounded once.  Keys on page ids outside [0, n_pages), or on pages
+ * behind a table's end, count as absent; a row that sees no key at all is zeros; what lies on a page behind the last position
+ * is never used, whatever it holds.  Made for one new token per request; several tokens of one request are computed rightly,
+ * their own keys read once for each.
+ *   mlora_attn_plan divides the step's work: once per step, for every layer, into `plan` (mlora_attn_plan_bytes bytes).
+ *   mlora_prefix_attention runs one layer against it; q and out as in mlora_kv_append (they must not overlap); workspace:
+ *   mlora_attn_workspace_bytes bytes of fp32 partial results.  Calls that share a workspace, or write a plan that another
+ *   reads, must be ordered on one stream.  The tables must be the ones the plan was made from.
+ * T <= MLORA_ATTN_MAX_T, n_prefix <= MLORA_ATTN_MAX_PREFIX.
+ */
+#define MLORA_ATTN_MAX_T 8192
+#define MLORA_ATTN_MAX_PREFIX 8192
+int64_t mlora_attn_plan_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads);
+int64_t mlora_attn_workspace_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads, int head_dim);
+int mlora_attn_plan(const int32_t *tok_req, const int32_t *tok_pos, int T, int n_req, int max_pages, const int32_t *req_prefix,
+                    const int32_t *prefix_len, int n_prefix, int max_prefix_pages, int page_tokens, int n_q_heads, int n_kv_heads,
+                    void *plan, int64_t plan_bytes, void *stream);
+int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t q_stride, const void *k_pages,
+                           const void *v_pages, int64_t n_pages, int page_tokens, int n_q_heads, int n_kv_heads, int head_dim,
+                           const int32_t *tok_req, const int32_t *tok_pos, int T, const int32_t *page_tbl, int n_req, int max_pages,
+                           const int32_t *req_prefix, const int32_t *prefix_tbl, const int32_t *prefix_len, int n_prefix,
+                           int max_prefix_pages, float scale, const void *plan, int64_t plan_bytes, void *workspace,
+                           int64_t workspace_bytes, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
