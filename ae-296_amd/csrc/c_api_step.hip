@@ -79,6 +79,13 @@ int check_batch(mlora::KvBatch &b, const int32_t *tok_req, const int32_t *tok_po
     return MLORA_OK;
 }
 
+int check_attn_sizes(int T, int n_prefix, int n_q_heads, int n_kv_heads)
+{
+    if (T < 0 || T > MLORA_ATTN_MAX_T) return fail(MLORA_ERANGE, "T must be in 0..%d (got %d)", MLORA_ATTN_MAX_T, T);
+    if (n_prefix < 0 || n_prefix > MLORA_ATTN_MAX_PREFIX) return fail(MLORA_ERANGE, "n_prefix must be in 0..%d (got %d)", MLORA_ATTN_MAX_PREFIX, n_prefix);
+    return check_cache(1, 16, n_q_heads, n_kv_heads, 64);
+}
+
 }  // namespace
 
 extern "C" {
@@ -170,12 +177,17 @@ int mlora_kv_append(const void *q, int64_t q_stride, void *q_out, int64_t q_out_
     return MLORA_OK;
 }
 
-// The plan of the simple form holds nothing yet.
-int64_t mlora_attn_plan_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads) { (void)T; (void)n_prefix; (void)n_q_heads; (void)n_kv_heads; return 16; }
+int64_t mlora_attn_plan_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads)
+{
+    const int rc = check_attn_sizes(T, n_prefix, n_q_heads, n_kv_heads);
+    return rc ? rc : mlora::attn_plan_bytes(T, n_prefix, n_q_heads, n_kv_heads);
+}
+
 int64_t mlora_attn_workspace_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads, int head_dim)
 {
-    (void)T; (void)n_prefix; (void)n_q_heads; (void)n_kv_heads; (void)head_dim;
-    return 16;
+    int rc = check_attn_sizes(T, n_prefix, n_q_heads, n_kv_heads);
+    if (rc || (rc = check_cache(1, 16, n_q_heads, n_kv_heads, head_dim))) return rc;
+    return mlora::attn_workspace_bytes(T, n_prefix, n_q_heads, n_kv_heads, head_dim);
 }
 
 int mlora_attn_plan(const int32_t *tok_req, const int32_t *tok_pos, int T, int n_req, int max_pages, const int32_t *req_prefix,
@@ -191,8 +203,13 @@ int mlora_attn_plan(const int32_t *tok_req, const int32_t *tok_pos, int T, int n
     if (n_prefix > 0 && (rc = check_table("max_prefix_pages", max_prefix_pages, page_tokens))) return rc;
     if (!tok_req || !tok_pos || !plan) return fail(MLORA_EINVAL, "tok_req, tok_pos and plan must not be NULL");
     if (!aligned16(plan)) return fail(MLORA_EALIGN, "plan must be 16-byte aligned");
-    if (plan_bytes < mlora_attn_plan_bytes(T, n_prefix, n_q_heads, n_kv_heads)) return fail(MLORA_ENOSPACE, "plan has %lld bytes, too few", (long long)plan_bytes);
-    (void)stream;
+    if (plan_bytes < mlora::attn_plan_bytes(T, n_prefix, n_q_heads, n_kv_heads)) return fail(MLORA_ENOSPACE, "plan has %lld bytes, too few", (long long)plan_bytes);
+    mlora::KvBatch b;
+    memset(&b, 0, sizeof(b));
+    b.tok_req = tok_req; b.tok_pos = tok_pos; b.req_prefix = n_prefix > 0 ? req_prefix : nullptr; b.prefix_len = prefix_len;
+    b.T = T; b.n_req = n_req; b.max_pages = max_pages; b.n_prefix = n_prefix; b.max_prefix_pages = max_prefix_pages;
+    rc = mlora::launch_attn_plan(b, log2_exact(page_tokens), n_q_heads, n_kv_heads, plan, static_cast<hipStream_t>(stream));
+    if (rc) return fail(MLORA_ELAUNCH, "plan launch failed: %s", hipGetErrorString((hipError_t)rc));
     return MLORA_OK;
 }
 
@@ -208,14 +225,15 @@ int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t
     int rc = check_cache(n_pages, page_tokens, n_q_heads, n_kv_heads, head_dim);
     if (rc) return rc;
     if (T == 0) return MLORA_OK;
+    if ((rc = check_prefix(req_prefix, prefix_len, n_prefix))) return rc;
     if (n_prefix > 0 && !prefix_tbl) return fail(MLORA_EINVAL, "prefix_tbl is needed with n_prefix > 0");
     if (n_prefix > 0 && (rc = check_table("max_prefix_pages", max_prefix_pages, page_tokens))) return rc;
     if (!out || !q || !k_pages || !v_pages || !plan) return fail(MLORA_EINVAL, "out, q, k_pages, v_pages and plan must not be NULL");
     if (!aligned16(out) || !aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(plan) || !aligned16(workspace))
         return fail(MLORA_EALIGN, "device pointers must be 16-byte aligned");
     if ((rc = check_stride("q", q_stride, n_q_heads, head_dim)) || (rc = check_stride("out", out_stride, n_q_heads, head_dim))) return rc;
-    if (plan_bytes < mlora_attn_plan_bytes(T, n_prefix, n_q_heads, n_kv_heads)) return fail(MLORA_ENOSPACE, "plan has %lld bytes, too few", (long long)plan_bytes);
-    const int64_t need = mlora_attn_workspace_bytes(T, n_prefix, n_q_heads, n_kv_heads, head_dim);
+    if (plan_bytes < mlora::attn_plan_bytes(T, n_prefix, n_q_heads, n_kv_heads)) return fail(MLORA_ENOSPACE, "plan has %lld bytes, too few", (long long)plan_bytes);
+    const int64_t need = mlora::attn_workspace_bytes(T, n_prefix, n_q_heads, n_kv_heads, head_dim);
     if (workspace_bytes < need || !workspace) return fail(MLORA_ENOSPACE, "workspace has %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
     mlora::AttnArgs a;
     memset(&a, 0, sizeof(a));
@@ -226,7 +244,7 @@ int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t
     a.out_stride = out_stride; a.q_stride = q_stride; a.n_pages = n_pages; a.page_shift = log2_exact(page_tokens);
     a.n_q_heads = n_q_heads; a.n_kv_heads = n_kv_heads; a.head_dim = head_dim; a.gq = n_q_heads / n_kv_heads;
     a.scale = scale;
-    rc = mlora::launch_prefix_attention(a, dtype, static_cast<hipStream_t>(stream));
+    rc = mlora::launch_prefix_attention(a, dtype, plan, workspace, static_cast<hipStream_t>(stream));
     if (rc) return fail(MLORA_ELAUNCH, "attention launch failed: %s", hipGetErrorString((hipError_t)rc));
     return MLORA_OK;
 }

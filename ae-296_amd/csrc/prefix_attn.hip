@@ -2,6 +2,11 @@
 //     out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j,   j over positions 0 .. tok_pos[t] of t's request
 // with the keys of a shared prefix on the prefix's pages and the others on the request's own.
 //
+// Three kernels.  The plan (once per step) cuts the work into items: up to 32 query rows x a range of keys of one list.  The rows of
+// an item are the query heads that read one key head, of one token over its own keys, or of all tokens behind a prefix over
+// the prefix's, so those are read once for 32 rows.  The attention kernel runs an item per workgroup and key head, the join adds up the
+// parts of rows that were cut, with their maxima and sums.
+//
 // One pass over the keys with the running maximum m and sum l of the softmax.  A wavefront multiplies 32 keys at a time with 16 query
 // rows on v_mfma_f32_16x16x32: first S^T = K q^T, whose result leaves every lane with eight scores of ONE query row (column lane % 16; keys
 // 4 g + i and 16 + 4 g + i, g = lane / 16), then out^T += V^T P^T.  The second product sums over keys, and its operands may hold the keys in
@@ -26,6 +31,7 @@ __device__ __forceinline__ float4_t pa_mfma(const uint4 &a, const uint4 &b, floa
 }
 
 constexpr int PA_WAVES = 4;
+constexpr int PA_ROWS = 32;                    // query rows of an item at most
 constexpr int PA_KEYS = 32;                    // keys of a block
 constexpr float PA_LOG2E = 1.44269504088896341f;
 
@@ -33,11 +39,208 @@ constexpr float PA_LOG2E = 1.44269504088896341f;
 // at one column spread over all banks.
 template <int D> __device__ __forceinline__ int pa_swizzle(int r, int c) { return D == 128 ? c ^ ((r & 7) << 1) : c ^ (((r >> 1) & 3) << 1); }
 
-// A run of keys on pages of one list.
-struct KeyRun {
-    const int32_t *pages;      // the list's row of its table
-    int n_listed;              // entries of it
-    int first, last;           // keys [first, last), first a multiple of 16
+// ------------------------------------------------------------------ plan
+// Item (int32 words): [0] query rows (<= PA_ROWS), [1] the token (own keys) or the first entry of the group's token list, [2] 1: a group,
+// [3] first row of the group's, row r being head r % gq of list entry r / gq, [4] row of the table, [5] 1: the prefix table,
+// [6], [7] keys [first, last), [8] slot of list entry 0 for this key range, -1: the rows have no other part and go to `out`.
+// Join record of a token: [0] first slot of its own parts, [1] how many, [2] first slot of its prefix parts, [3] how many, [4] slots from one
+// to the next.  A slot holds the gq rows of every key head.
+constexpr int PA_ITEM = 12, PA_JOIN = 8;
+constexpr int PL_THREADS = 1024;
+constexpr int PL_PREFIXES = 4096;     // prefixes at most
+
+struct PlanView {
+    int32_t *n_items;       // [4]
+    int32_t *list;          // [T] tokens of the groups
+    int32_t *join;          // [T][PA_JOIN]
+    int32_t *items;         // [cap][PA_ITEM]
+};
+
+// Key heads times items that fill the device: two workgroups for each place that a compute unit has for one.
+__host__ __device__ inline int pa_target(int n_kv_heads) { const int t = 1024 / n_kv_heads; return t < 1 ? 1 : t; }
+
+// With C keys a range where C >= (sum of own keys + sum over groups of keys x row tiles) / target, a list is cut into at most
+// keys / C + 1 ranges, which bounds the items and the slots by sizes the host knows.
+inline int64_t pa_items_cap(int T, int n_prefix, int gq, int n_kv_heads)
+{
+    const int64_t groups = T < n_prefix ? T : n_prefix, tiles = (int64_t)T * gq / PA_ROWS + groups, own_tiles = (gq + PA_ROWS - 1) / PA_ROWS;
+    return T * own_tiles + (n_prefix ? tiles : 0) + pa_target(n_kv_heads) * own_tiles + 1;
+}
+inline int64_t pa_slots_cap(int T, int n_prefix, int gq, int n_kv_heads)
+{
+    const int64_t target = pa_target(n_kv_heads), per_tile = (PA_ROWS + gq - 1) / gq;
+    return (int64_t)T * (n_prefix ? 2 : 1) + target * (n_prefix ? per_tile : 1) + 1;
+}
+
+__host__ __device__ inline PlanView pa_plan_view(void *plan, int T)
+{
+    int32_t *p = static_cast<int32_t *>(plan);
+    return {p, p + 4, p + 4 + (T + 3) / 4 * 4, p + 4 + (T + 3) / 4 * 4 + (size_t)T * PA_JOIN};
+}
+
+struct PlanArgs {
+    KvBatch b;
+    void *plan;
+    int page_shift, gq, target;
+    long long items_cap, slots_cap;
+};
+
+// What a token reads.  An own list, or the part of its prefix that it sees where it stands inside of it (then it is no member of
+// the group); keys behind the table's end are absent.
+struct TokenRun { int prefix; int own; int table, row; };       // prefix: the group, -1 none
+__device__ __forceinline__ TokenRun pa_token(const KvBatch &b, int page_shift, int t)
+{
+    TokenRun r = {-1, 0, 0, 0};
+    const int req = b.tok_req[t], pos = b.tok_pos[t];
+    if (req < 0 || req >= b.n_req) return r;
+    r.row = req;
+    long long base = 0;
+    if (b.req_prefix) {
+        const int f = b.req_prefix[req];
+        if (f >= 0 && f < b.n_prefix) {
+            base = max(b.prefix_len[f], 0);
+            const long long there = min(base, (long long)b.max_prefix_pages << page_shift), seen = min((long long)pos + 1, there);
+            if (seen == there) { if (there > 0) r.prefix = f; }
+            else { r.own = (int)max(seen, 0LL); r.table = 1; r.row = f; return r; }
+        }
+    }
+    r.own = (int)max(min((long long)pos + 1 - base, (long long)b.max_pages << page_shift), 0LL);
+    return r;
+}
+
+// Exclusive sum of v over the workgroup's threads; *total: the sum.  `scratch`: a value per wavefront.
+__device__ __forceinline__ int pl_scan(int v, int *scratch, int *total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int upto = (int)wave_scan((uint32_t)v);
+    __syncthreads();
+    if (lane == 63) scratch[wave] = upto;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < PL_THREADS / 64; w++) { const int x = scratch[w]; before += w < wave ? x : 0; all += x; }
+    *total = all;
+    return before + upto - v;
+}
+
+__device__ __forceinline__ int pl_find(const int *first, int n, int i)       // last entry e with first[e] <= i
+{
+    int lo = 0, hi = n;
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (first[mid] <= i) lo = mid; else hi = mid; }
+    return lo;
+}
+
+// One workgroup.  Tokens enter their group's list in any order (LDS atomics): a row's arithmetic does not depend on its place in a tile.
+__global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
+{
+    __shared__ int s_count[PL_PREFIXES], s_list[PL_PREFIXES], s_slot[PL_PREFIXES], s_item[PL_PREFIXES], s_scan[PL_THREADS / 64];
+    __shared__ int s_first[PL_THREADS], s_own[PL_THREADS], s_row[PL_THREADS], s_part[PL_THREADS];
+    __shared__ unsigned long long s_work;
+    const int T = p.b.T, F = p.b.req_prefix ? p.b.n_prefix : 0;
+    const PlanView v = pa_plan_view(p.plan, T);
+    for (int f = threadIdx.x; f < F; f += PL_THREADS) s_count[f] = 0;
+    if (threadIdx.x == 0) s_work = 0;
+    __syncthreads();
+    // how much there is
+    unsigned long long work = 0;
+    for (int t = threadIdx.x; t < T; t += PL_THREADS) {
+        const TokenRun r = pa_token(p.b, p.page_shift, t);
+        work += (unsigned)r.own;
+        if (r.prefix >= 0) atomicAdd(&s_count[r.prefix], 1);
+    }
+    __syncthreads();
+    auto prefix_keys = [&](int f) { return (int)min((long long)p.b.prefix_len[f], (long long)p.b.max_prefix_pages << p.page_shift); };
+    auto tiles_of = [&](int f) { return (int)(((long long)s_count[f] * p.gq + PA_ROWS - 1) / PA_ROWS); };
+    for (int f = threadIdx.x; f < F; f += PL_THREADS)
+        if (s_count[f]) work += (unsigned long long)prefix_keys(f) * tiles_of(f);
+    for (int o = 32; o; o >>= 1) work += __shfl_xor(work, o);
+    if ((threadIdx.x & 63) == 0 && work) atomicAdd(&s_work, work);
+    __syncthreads();
+    // keys of a range, a multiple of what the wavefronts take at a time
+    const long long step = PA_WAVES * PA_KEYS;
+    const long long C = (((long long)s_work + p.target - 1) / p.target + step - 1) / step * step;
+    auto range_of = [&](int keys, int cuts) { return ((keys + (long long)cuts - 1) / cuts + step - 1) / step * step; };
+    auto cuts_of = [&](int keys) { return keys > 0 ? (int)((keys + C - 1) / C) : 0; };
+    // groups: their lists, slots and items
+    int n_list = 0, n_slot = 0, n_item = 0;
+    for (int f0 = 0; f0 < F; f0 += PL_THREADS) {
+        const int f = f0 + threadIdx.x;
+        const int members = f < F ? s_count[f] : 0, cuts = members ? cuts_of(prefix_keys(f)) : 0;
+        int a, b, c;
+        const int la = n_list + pl_scan(members, s_scan, &a);
+        const int sl = n_slot + pl_scan(members * cuts, s_scan, &b);
+        const int it = n_item + pl_scan(members ? tiles_of(f) * cuts : 0, s_scan, &c);
+        if (f < F) { s_list[f] = la; s_slot[f] = sl; s_item[f] = it; }
+        n_list += a; n_slot += b; n_item += c;
+    }
+    __syncthreads();
+    const int group_items = n_item;
+    for (int i = threadIdx.x; i < group_items && i < p.items_cap; i += PL_THREADS) {
+        const int f = pl_find(s_item, F, i);
+        const int keys = prefix_keys(f), cuts = cuts_of(keys), tiles = tiles_of(f), at = i - s_item[f];
+        const int cut = at / tiles, tile = at - cut * tiles;       // the tiles of a range lie side by side: they share its keys in L2
+        const long long per = range_of(keys, cuts);
+        int32_t *e = v.items + (size_t)i * PA_ITEM;
+        e[0] = (int)min((long long)PA_ROWS, (long long)s_count[f] * p.gq - (long long)tile * PA_ROWS);
+        e[1] = s_list[f]; e[2] = 1; e[3] = tile * PA_ROWS; e[4] = f; e[5] = 1;
+        e[6] = (int)min(cut * per, (long long)keys); e[7] = (int)min((cut + 1) * per, (long long)keys);
+        e[8] = s_slot[f] + cut * s_count[f];
+    }
+    __syncthreads();
+    // the members, and every token's own parts
+    int *s_take = s_item;
+    for (int f = threadIdx.x; f < F; f += PL_THREADS) s_take[f] = 0;
+    __syncthreads();
+    const int own_tiles = (p.gq + PA_ROWS - 1) / PA_ROWS;
+    for (int t0 = 0; t0 < T; t0 += PL_THREADS) {
+        const int t = t0 + threadIdx.x;
+        TokenRun r = {-1, 0, 0, 0};
+        int place = 0, prefix_cuts = 0;
+        if (t < T) {
+            r = pa_token(p.b, p.page_shift, t);
+            if (r.prefix >= 0) {
+                place = atomicAdd(&s_take[r.prefix], 1);
+                if (s_list[r.prefix] + place < T) v.list[s_list[r.prefix] + place] = t;
+                prefix_cuts = cuts_of(prefix_keys(r.prefix));
+            }
+        }
+        const int cuts = cuts_of(r.own), kept = cuts + prefix_cuts > 1 ? cuts : 0;
+        int a, b;
+        const int sl = n_slot + pl_scan(kept, s_scan, &a);
+        const int it = n_item + pl_scan(cuts * own_tiles, s_scan, &b);
+        s_first[threadIdx.x] = it; s_own[threadIdx.x] = r.own; s_row[threadIdx.x] = 2 * r.row + r.table; s_part[threadIdx.x] = kept ? sl : -1;
+        if (t < T) {
+            int32_t *j = v.join + (size_t)t * PA_JOIN;
+            j[0] = sl; j[1] = cuts; j[3] = prefix_cuts;
+            j[2] = r.prefix >= 0 ? s_slot[r.prefix] + place : 0;
+            j[4] = r.prefix >= 0 ? s_count[r.prefix] : 0;
+        }
+        __syncthreads();
+        for (int i = n_item + threadIdx.x; i < n_item + b && i < p.items_cap; i += PL_THREADS) {
+            const int w = pl_find(s_first, PL_THREADS, i), keys = s_own[w], cuts_w = cuts_of(keys), at = i - s_first[w];
+            const int cut = at / own_tiles, tile = at - cut * own_tiles;
+            const long long per = range_of(keys, cuts_w);
+            int32_t *e = v.items + (size_t)i * PA_ITEM;
+            e[0] = min(PA_ROWS, p.gq - tile * PA_ROWS); e[1] = t0 + w; e[2] = 0; e[3] = tile * PA_ROWS; e[4] = s_row[w] >> 1; e[5] = s_row[w] & 1;
+            e[6] = (int)min(cut * per, (long long)keys); e[7] = (int)min((cut + 1) * per, (long long)keys);
+            e[8] = s_part[w] < 0 ? -1 : s_part[w] + cut;
+        }
+        n_slot += a; n_item += b;
+    }
+    if (threadIdx.x == 0) v.n_items[0] = (int)min((long long)n_item, p.items_cap);
+}
+
+// ------------------------------------------------------------------ attention
+struct AttnKernelArgs {
+    AttnArgs a;
+    void *plan;
+    float *parts;          // [slots][n_kv_heads][gq][D] sums, then [slots][n_kv_heads][gq][2] maximum and weight
+    long long items_cap, slots_cap;
+};
+
+// K and V of one block of 32 keys, on their way.
+template <int D> struct KeyBlock {
+    uint4 k[2][D / 32], v[D / 16];
+    bool there[2];
 };
 
 // What a wavefront holds of 16 query rows.
@@ -47,72 +250,110 @@ template <int D> struct RowState {
     float4_t acc[D / 16];      // out^T: columns 16 i + 4 g .. + 3 of row lane % 16
 };
 
+// One wavefront's way through keys [first, last) of a list.  It holds 64 page ids at a time, one a lane.
 template <int DT, int D>
-__device__ __forceinline__ void pa_blocks(const AttnArgs &p, int head, const KeyRun &run, int b0, int stride, float scale2, RowState<D> &st,
-                                          unsigned char *vlds)
-{
-    constexpr int KS = D / 32, DTILES = D / 16, VL = D / 16, CH = D / 8;       // K steps, column tiles, 16-byte loads of V a lane, chunks of a row
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int psize = 1 << p.page_shift;
-    const size_t page_elems = (size_t)p.n_kv_heads << p.page_shift;            // rows of a page
-    for (int key0 = run.first + b0 * PA_KEYS; key0 < run.last; key0 += stride * PA_KEYS) {
-        size_t row0[2];
-        bool there[2];
+struct Walk {
+    static constexpr int KS = D / 32, DTILES = D / 16, VL = D / 16, CH = D / 8;    // K steps, column tiles, 16-byte loads of V a lane, chunks of a row
+    const AttnArgs &p;
+    const int32_t *pages;
+    unsigned char *vlds;
+    float scale2;
+    int n_listed, first, last, head;
+    int window, ids;                   // 64 pages from page `window` on; -1: none yet
+
+    __device__ __forceinline__ int page_of(int nth)
+    {
+        if (window < 0 || nth < window || nth >= window + 64) {
+            window = nth;
+            const int at = nth + (threadIdx.x & 63);
+            ids = at < n_listed ? pages[at] : -1;
+        }
+        const int page = __builtin_amdgcn_readlane(ids, nth - window);
+        return page < p.n_pages ? page : -1;
+    }
+
+    // Issue the loads of the block at key0 (a block past the end is loaded from page 0 and masked).
+    __device__ __forceinline__ void load(KeyBlock<D> &b, int key0)
+    {
+        // what differs between lanes is one 32-bit offset for K and one for V: the rest of an address is the same for the wavefront
+        const int lane = threadIdx.x & 63;
+        const unsigned klane = (lane & 15) * D + (lane >> 4) * 8, vlane = (lane / CH) * D + (lane % CH) * 8;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int at = key0 + 16 * h, nth = at >> p.page_shift;
-            const int page = at < run.last && nth < run.n_listed ? run.pages[nth] : -1;
-            there[h] = page >= 0 && page < p.n_pages;
-            row0[h] = (there[h] ? page : 0) * page_elems + ((size_t)head << p.page_shift) + (at & (psize - 1));
+            const int at = key0 + 16 * h;
+            const int page = at < last ? page_of(at >> p.page_shift) : -1;
+            b.there[h] = page >= 0;
+            const size_t row0 = (((size_t)(page >= 0 ? page : 0) * p.n_kv_heads + head) << p.page_shift) + (at & ((1 << p.page_shift) - 1));
+            const uint16_t *k = p.k_pages + row0 * D, *v = p.v_pages + row0 * D;
+#pragma unroll
+            for (int s = 0; s < KS; s++) b.k[h][s] = ldg16(k + klane + s * 32);
+#pragma unroll
+            for (int u = 0; u < VL / 2; u++) b.v[h * (VL / 2) + u] = ldg16(v + vlane + u * (64 / CH) * D);
         }
-        uint4 kf[2][KS], vf[VL];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int s = 0; s < KS; s++) kf[h][s] = ldg16(p.k_pages + (row0[h] + c) * D + s * 32 + g * 8);
-#pragma unroll
-        for (int u = 0; u < VL; u++) {
-            const int r = u * (64 / CH) + lane / CH;
-            vf[u] = ldg16(p.v_pages + (row0[u >= VL / 2] + (r & 15)) * D + (lane % CH) * 8);
+    }
+
+    // Scores of the block at key0, and V's way to LDS: after this the block's registers are free.
+    template <int NR>
+    __device__ __forceinline__ void scores(KeyBlock<D> &b, int key0, const RowState<D> (&st)[NR], float4_t (&s)[NR][2])
+    {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        const bool whole = b.there[0] && b.there[1] && key0 + PA_KEYS <= last;
+        if (!whole) {
             // what lies behind the last key, or on no page at all, must not meet a weight of zero: it may be infinite
-            if (key0 + r >= run.last || !there[u >= VL / 2]) vf[u] = zero16();
-        }
-        float4_t s[2];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            s[h] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < KS; k++) s[h] = pa_mfma<DT>(kf[h][k], st.q[k], s[h]);
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                s[h][i] = there[h] && key0 + 16 * h + 4 * g + i < run.last ? s[h][i] * scale2 : -INFINITY;
-                top = fmaxf(top, s[h][i]);
+            for (int u = 0; u < VL; u++) {
+                const uint32_t keep = key0 + u * (64 / CH) + lane / CH < last && b.there[u >= VL / 2] ? ~0u : 0u;
+                b.v[u] = make_uint4(b.v[u].x & keep, b.v[u].y & keep, b.v[u].z & keep, b.v[u].w & keep);
             }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float m = fmaxf(st.m, top), ref = m == -INFINITY ? 0.f : m, keep = __builtin_amdgcn_exp2f(st.m - ref);
-        st.m = m;
-        st.l *= keep;
-#pragma unroll
-        for (int d = 0; d < DTILES; d++) st.acc[d] *= keep;
-        float w[8];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) { w[4 * h + i] = __builtin_amdgcn_exp2f(s[h][i] - ref); st.l += w[4 * h + i]; }
-        const uint4 wf = pack8<DT>(w);
+        }
 #pragma unroll
         for (int u = 0; u < VL; u++) {
             const int r = u * (64 / CH) + lane / CH;
-            stg16(vlds + r * (D * 2) + pa_swizzle<D>(r, lane % CH) * 16, vf[u]);
+            stg16(vlds + r * (D * 2) + pa_swizzle<D>(r, lane % CH) * 16, b.v[u]);
+        }
+#pragma unroll
+        for (int n = 0; n < NR; n++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                s[n][h] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KS; k++) s[n][h] = pa_mfma<DT>(b.k[h][k], st[n].q[k], s[n][h]);
+                s[n][h] *= scale2;
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[n][h][i] = b.there[h] && key0 + 16 * h + 4 * g + i < last ? s[n][h][i] : -INFINITY;
+                }
+            }
+    }
+
+    // Softmax weights of the block, and the sums over its keys.
+    template <int NR>
+    __device__ __forceinline__ void sums(RowState<D> (&st)[NR], const float4_t (&s)[NR][2])
+    {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+        uint4 wf[NR];
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])), fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float m = fmaxf(st[n].m, top), ref = m == -INFINITY ? 0.f : m;
+            if (__ballot(m > st[n].m)) {           // a higher maximum in some row: what was summed so far shrinks
+                const float keep = __builtin_amdgcn_exp2f(st[n].m - ref);
+                st[n].l *= keep;
+#pragma unroll
+                for (int d = 0; d < DTILES; d++) st[n].acc[d] *= keep;
+                st[n].m = m;
+            }
+            float w[8];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) { w[4 * h + i] = __builtin_amdgcn_exp2f(s[n][h][i] - ref); st[n].l += w[4 * h + i]; }
+            wf[n] = pack8<DT>(w);
         }
         __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int d = 0; d < DTILES; d++) {
+        auto column = [&](int d) {                 // V^T of 16 columns
             uint2 half[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -120,88 +361,240 @@ __device__ __forceinline__ void pa_blocks(const AttnArgs &p, int head, const Key
                 half[h] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                     (pa_lds_short4 *)(vlds + r * (D * 2) + pa_swizzle<D>(r, 2 * d + (c % 4) / 2) * 16 + (c & 1) * 8)));
             }
-            st.acc[d] = pa_mfma<DT>(make_uint4(half[0].x, half[0].y, half[1].x, half[1].y), wf, st.acc[d]);
+            return make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
+        };
+        // two columns ahead and no more, or the registers run out
+        constexpr int AHEAD = 2;
+        uint4 vt[AHEAD];
+#pragma unroll
+        for (int d = 0; d < AHEAD; d++) vt[d] = column(d);
+#pragma unroll
+        for (int d = 0; d < DTILES; d++) {
+            const uint4 now = vt[d % AHEAD];
+            if (d + AHEAD < DTILES) vt[d % AHEAD] = column(d + AHEAD);
+#pragma unroll
+            for (int n = 0; n < NR; n++) st[n].acc[d] = pa_mfma<DT>(now, wf[n], st[n].acc[d]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_wave_barrier();
     }
+
+    template <int NR>
+    __device__ __forceinline__ void all(RowState<D> (&st)[NR])
+    {
+        int key0 = first;
+        if (key0 >= last) return;
+        float4_t s[NR][2];
+        KeyBlock<D> b;
+        load(b, key0);
+        // the next block comes during the softmax and the second product, into the same registers
+#pragma unroll 1
+        while (key0 + PA_KEYS < last) {
+            scores<NR>(b, key0, st, s);
+            key0 += PA_KEYS;
+            load(b, key0);
+            sums<NR>(st, s);
+        }
+        scores<NR>(b, key0, st, s);
+        sums<NR>(st, s);
+    }
+};
+
+constexpr int pa_pitch(int D) { return D + 4; }            // floats of a row in the LDS exchange: a float4 of 16 rows meets all banks
+
+// One item for one key head: NR tiles of 16 query rows, the keys shared by the four wavefronts and joined in LDS.
+template <int DT, int D, int NR>
+__device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const int32_t *e, const PlanView &pv, int head, unsigned char *lds, float (*s_m)[16], float (*s_l)[16])
+{
+    constexpr int PITCH = pa_pitch(D), E = D / 16;
+    const AttnArgs &p = ka.a;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int rows = e[0], from = e[1], grouped = e[2], row0 = e[3], slot = e[8];
+    auto token_of = [&](int idx) { return grouped ? pv.list[from + idx] : from; };
+    RowState<D> st[NR];
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        const int r = row0 + min(n * 16 + c, rows - 1), idx = r / p.gq;
+        const uint16_t *q = p.q + token_of(idx) * p.q_stride + ((size_t)head * p.gq + (r - idx * p.gq)) * D;
+#pragma unroll
+        for (int k = 0; k < D / 32; k++) st[n].q[k] = ldg16(q + k * 32 + g * 8);
+        st[n].m = -INFINITY;
+        st[n].l = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) st[n].acc[d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    const int first = e[6], last = e[7], share = (last - first + PA_WAVES * PA_KEYS - 1) / (PA_WAVES * PA_KEYS) * PA_KEYS;
+    const int mine = first + wave * share;
+    const int listed = e[5] ? p.b.max_prefix_pages : p.b.max_pages;
+    Walk<DT, D> walk{p, (e[5] ? p.b.prefix_tbl : p.b.page_tbl) + (size_t)e[4] * listed, lds + wave * (PA_KEYS * D * 2), p.scale * PA_LOG2E,
+                     listed, mine, min(mine + share, last), head, -1, -1};
+    walk.template all<NR>(st);
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        float l = st[n].l;
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        __syncthreads();                       // the wavefronts are through with V, or with the exchange before this one
+        if (g == 0) { s_m[wave][c] = st[n].m; s_l[wave][c] = l; }
+        __syncthreads();
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PA_WAVES; w++) m = fmaxf(m, s_m[w][c]);
+        const float f = st[n].m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[n].m - m);
+        float *part = reinterpret_cast<float *>(lds) + (wave * 16 + c) * PITCH;
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) *reinterpret_cast<float4_t *>(part + d * 16 + g * 4) = st[n].acc[d] * f;
+        __syncthreads();
+        const int r = threadIdx.x >> 4, col = (threadIdx.x & 15) * E;
+        if (n * 16 + r >= rows) continue;
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < PA_WAVES; w++) m = fmaxf(m, s_m[w][r]);
+#pragma unroll
+        for (int w = 0; w < PA_WAVES; w++) l += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - m);
+        float v[E];
+#pragma unroll
+        for (int k = 0; k < E; k += 4) {
+            float4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < PA_WAVES; w++) sum += *reinterpret_cast<const float4_t *>(reinterpret_cast<const float *>(lds) + (w * 16 + r) * PITCH + col + k);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[k + i] = sum[i];
+        }
+        const int row = row0 + n * 16 + r, idx = row / p.gq, sub = row - idx * p.gq;
+        if (slot < 0) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            uint16_t *out = p.out + token_of(idx) * p.out_stride + ((size_t)head * p.gq + sub) * D + col;
+#pragma unroll
+            for (int k = 0; k < E; k += 4) *reinterpret_cast<uint2 *>(out + k) = make_uint2(pack2<DT>(v[k] * inv, v[k + 1] * inv), pack2<DT>(v[k + 2] * inv, v[k + 3] * inv));
+        } else if (slot + idx < ka.slots_cap) {
+            const size_t at = ((size_t)(slot + idx) * p.n_kv_heads + head) * p.gq + sub;
+#pragma unroll
+            for (int k = 0; k < E; k += 4) *reinterpret_cast<float4_t *>(ka.parts + at * D + col + k) = float4_t{v[k], v[k + 1], v[k + 2], v[k + 3]};
+            if (col == 0) *reinterpret_cast<float2 *>(ka.parts + (size_t)ka.slots_cap * p.n_q_heads * D + at * 2) = make_float2(m, l);
+        }
+    }
 }
 
-// One workgroup: up to 16 query heads of one token that read one key head; its wavefronts share the keys.
 template <int DT, int D>
-__global__ __launch_bounds__(64 * PA_WAVES) void prefix_attention_kernel(const AttnArgs p)
+__global__ __launch_bounds__(64 * PA_WAVES, 2) void prefix_attention_kernel(const AttnKernelArgs ka)
 {
-    constexpr int PITCH = D + 4;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[PA_WAVES * 16 * PITCH * 4];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[PA_WAVES * 16 * pa_pitch(D) * 4];
     __shared__ float s_m[PA_WAVES][16], s_l[PA_WAVES][16];
-    const int t = blockIdx.x, head = blockIdx.y, first_row = blockIdx.z * 16;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int req = p.b.tok_req[t], pos = p.b.tok_pos[t];
-    if (req < 0) return;
-    int f = -1, base = 0;
-    if (p.b.req_prefix && req < p.b.n_req) {
-        f = p.b.req_prefix[req];
-        if (f < 0 || f >= p.b.n_prefix) f = -1;
-        else base = max(p.b.prefix_len[f], 0);
-    }
-    const int rows = min(16, p.gq - first_row);
-    RowState<D> st;
-    const uint16_t *q = p.q + t * p.q_stride + ((size_t)head * p.gq + first_row + (c < rows ? c : 0)) * D;
-#pragma unroll
-    for (int k = 0; k < D / 32; k++) st.q[k] = ldg16(q + k * 32 + g * 8);
-    st.m = -INFINITY;
-    st.l = 0.f;
-#pragma unroll
-    for (int d = 0; d < D / 16; d++) st.acc[d] = float4_t{0.f, 0.f, 0.f, 0.f};
-    const float scale2 = p.scale * PA_LOG2E;
-    unsigned char *vlds = lds + wave * (PA_KEYS * D * 2);
-    if (f >= 0) {
-        const long long last = min(min((long long)base, (long long)pos + 1), (long long)p.b.max_prefix_pages << p.page_shift);
-        const KeyRun run = {p.b.prefix_tbl + (size_t)f * p.b.max_prefix_pages, p.b.max_prefix_pages, 0, (int)last};
-        pa_blocks<DT, D>(p, head, run, wave, PA_WAVES, scale2, st, vlds);
-    }
-    if (req < p.b.n_req) {
-        const long long last = min((long long)pos + 1 - base, (long long)p.b.max_pages << p.page_shift);
-        const KeyRun run = {p.b.page_tbl + (size_t)req * p.b.max_pages, p.b.max_pages, 0, (int)last};
-        pa_blocks<DT, D>(p, head, run, wave, PA_WAVES, scale2, st, vlds);
-    }
-    float l = st.l;
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (g == 0) { s_m[wave][c] = st.m; s_l[wave][c] = l; }
-    __syncthreads();
-    float m = -INFINITY;
-    for (int w = 0; w < PA_WAVES; w++) m = fmaxf(m, s_m[w][c]);
-    const float mine = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
-    float *part = reinterpret_cast<float *>(lds) + wave * 16 * PITCH + c * PITCH;
-#pragma unroll
-    for (int d = 0; d < D / 16; d++) *reinterpret_cast<float4_t *>(part + d * 16 + g * 4) = st.acc[d] * mine;
-    __syncthreads();
-    const int r = threadIdx.x >> 4;
-    if (r >= rows) return;
-    m = -INFINITY;
-    for (int w = 0; w < PA_WAVES; w++) m = fmaxf(m, s_m[w][r]);
-    l = 0.f;
-    for (int w = 0; w < PA_WAVES; w++) l += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - m);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t *out = p.out + t * p.out_stride + ((size_t)head * p.gq + first_row + r) * D;
-    for (int d = (threadIdx.x & 15) * 2; d < D; d += 32) {
-        float v[2] = {0.f, 0.f};
-        for (int w = 0; w < PA_WAVES; w++)
-            for (int e = 0; e < 2; e++) v[e] += reinterpret_cast<const float *>(lds)[(w * 16 + r) * PITCH + d + e];
-        *reinterpret_cast<uint32_t *>(out + d) = pack2<DT>(v[0] * inv, v[1] * inv);
-    }
+    const AttnArgs &p = ka.a;
+    const PlanView pv = pa_plan_view(ka.plan, p.b.T);
+    // key heads fastest: with a multiple of eight of them a head stays on one XCD, and with it what the row tiles of a prefix share
+    const unsigned item = blockIdx.x / (unsigned)p.n_kv_heads, head = blockIdx.x - item * (unsigned)p.n_kv_heads;
+    if ((int)item >= min((long long)pv.n_items[0], ka.items_cap)) return;
+    const int32_t *e = pv.items + (size_t)item * PA_ITEM;
+    if (e[0] <= 16) pa_item<DT, D, 1>(ka, e, pv, head, lds, s_m, s_l);
+    else pa_item<DT, D, 2>(ka, e, pv, head, lds, s_m, s_l);
 }
 
-int launch_prefix_attention(const AttnArgs &a, int dtype, hipStream_t s)
+// ------------------------------------------------------------------ join
+// A workgroup: PA_JOIN_ROWS query rows of one token, 16 threads and G groups of them a row, the groups share the parts.
+template <int DT, int D, int G>
+__global__ __launch_bounds__(256) void pa_join_kernel(const AttnKernelArgs ka)
 {
-    const dim3 grid((unsigned)a.b.T, (unsigned)a.n_kv_heads, (unsigned)((a.gq + 15) / 16));
-    if (dtype == DT_F16) {
-        if (a.head_dim == 64) hipLaunchKernelGGL((prefix_attention_kernel<DT_F16, 64>), grid, dim3(64 * PA_WAVES), 0, s, a);
-        else hipLaunchKernelGGL((prefix_attention_kernel<DT_F16, 128>), grid, dim3(64 * PA_WAVES), 0, s, a);
-    } else {
-        if (a.head_dim == 64) hipLaunchKernelGGL((prefix_attention_kernel<DT_BF16, 64>), grid, dim3(64 * PA_WAVES), 0, s, a);
-        else hipLaunchKernelGGL((prefix_attention_kernel<DT_BF16, 128>), grid, dim3(64 * PA_WAVES), 0, s, a);
+    constexpr int ROWS = 16 / G, E = D / 16;
+    __shared__ float s_v[G > 1 ? 16 : 1][G > 1 ? D : 1], s_m[16], s_l[16];
+    const AttnArgs &p = ka.a;
+    const int t = blockIdx.x;
+    if (p.b.tok_req[t] < 0) return;
+    const PlanView pv = pa_plan_view(ka.plan, p.b.T);
+    const int32_t *j = pv.join + (size_t)t * PA_JOIN;
+    const int own = j[1], shared = j[3];
+    if (own == 1 && shared == 0) return;                         // written by its only item
+    const int slice = threadIdx.x >> 4, col = (threadIdx.x & 15) * E, part0 = slice % G;
+    const int row = blockIdx.y * ROWS + slice / G;               // query head
+    float m = -INFINITY, l = 0.f, v[E] = {};
+    if (row < p.n_q_heads) {
+        const float *ml = ka.parts + (size_t)ka.slots_cap * p.n_q_heads * D;
+        for (int i = part0; i < own + shared; i += G) {
+            const long long slot = i < own ? (long long)j[0] + i : j[2] + (long long)(i - own) * j[4];
+            if (slot < 0 || slot >= ka.slots_cap) continue;
+            const size_t at = (size_t)slot * p.n_q_heads + row;
+            const float2 x = *reinterpret_cast<const float2 *>(ml + at * 2);
+            if (x.x == -INFINITY) continue;
+            const float top = fmaxf(m, x.x), a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), b = __builtin_amdgcn_exp2f(x.x - top);
+            m = top;
+            l = l * a + x.y * b;
+#pragma unroll
+            for (int k = 0; k < E; k += 4) {
+                const float4_t y = *reinterpret_cast<const float4_t *>(ka.parts + at * D + col + k);
+#pragma unroll
+                for (int q = 0; q < 4; q++) v[k + q] = v[k + q] * a + y[q] * b;
+            }
+        }
     }
+    if constexpr (G > 1) {
+        if (col == 0) { s_m[slice] = m; s_l[slice] = l; }
+#pragma unroll
+        for (int k = 0; k < E; k++) s_v[slice][col + k] = v[k];
+        __syncthreads();
+        if (part0) return;
+        float top = m;
+        for (int q = 1; q < G; q++) top = fmaxf(top, s_m[slice + q]);
+        float all = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; k++) v[k] = 0.f;
+        for (int q = 0; q < G; q++) {
+            const float f = s_m[slice + q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[slice + q] - top);
+            all += s_l[slice + q] * f;
+#pragma unroll
+            for (int k = 0; k < E; k++) v[k] += s_v[slice + q][col + k] * f;
+        }
+        l = all;
+    }
+    if (row >= p.n_q_heads) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t *out = p.out + t * p.out_stride + (size_t)row * D + col;
+#pragma unroll
+    for (int k = 0; k < E; k += 4) *reinterpret_cast<uint2 *>(out + k) = make_uint2(pack2<DT>(v[k] * inv, v[k + 1] * inv), pack2<DT>(v[k + 2] * inv, v[k + 3] * inv));
+}
+
+// ------------------------------------------------------------------ launchers
+int64_t attn_plan_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads)
+{
+    const int64_t list = (T + 3) / 4 * 4, items = pa_items_cap(T, n_prefix, n_q_heads / n_kv_heads, n_kv_heads);
+    return 4 * (4 + list + (int64_t)T * PA_JOIN + items * PA_ITEM);
+}
+
+int64_t attn_workspace_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads, int head_dim)
+{
+    return pa_slots_cap(T, n_prefix, n_q_heads / n_kv_heads, n_kv_heads) * n_q_heads * (head_dim + 2) * 4;
+}
+
+int launch_attn_plan(const KvBatch &b, int page_shift, int n_q_heads, int n_kv_heads, void *plan, hipStream_t s)
+{
+    PlanArgs a;
+    a.b = b; a.plan = plan; a.page_shift = page_shift; a.gq = n_q_heads / n_kv_heads; a.target = pa_target(n_kv_heads);
+    a.items_cap = pa_items_cap(b.T, b.n_prefix, a.gq, n_kv_heads);
+    hipLaunchKernelGGL(pa_plan_kernel, dim3(1), dim3(PL_THREADS), 0, s, a);
+    return (int)hipGetLastError();
+}
+
+template <int DT, int D>
+static void attention_of(const AttnKernelArgs &a, hipStream_t s)
+{
+    hipLaunchKernelGGL((prefix_attention_kernel<DT, D>), dim3((unsigned)(a.items_cap * a.a.n_kv_heads)), dim3(64 * PA_WAVES), 0, s, a);
+    // few rows have many parts each: then sixteen slices of a workgroup share a row's
+    const dim3 wide((unsigned)a.a.b.T, (unsigned)a.a.n_q_heads), narrow((unsigned)a.a.b.T, (unsigned)((a.a.n_q_heads + 3) / 4));
+    if ((long long)a.a.b.T * a.a.n_q_heads <= 1024) hipLaunchKernelGGL((pa_join_kernel<DT, D, 16>), wide, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((pa_join_kernel<DT, D, 4>), narrow, dim3(256), 0, s, a);
+}
+
+int launch_prefix_attention(const AttnArgs &a, int dtype, const void *plan, void *workspace, hipStream_t s)
+{
+    AttnKernelArgs k;
+    k.a = a;
+    k.plan = const_cast<void *>(plan);
+    k.parts = static_cast<float *>(workspace);
+    k.items_cap = pa_items_cap(a.b.T, a.b.n_prefix, a.gq, a.n_kv_heads);
+    k.slots_cap = pa_slots_cap(a.b.T, a.b.n_prefix, a.gq, a.n_kv_heads);
+    if (dtype == DT_F16) { if (a.head_dim == 64) attention_of<DT_F16, 64>(k, s); else attention_of<DT_F16, 128>(k, s); }
+    else { if (a.head_dim == 64) attention_of<DT_BF16, 64>(k, s); else attention_of<DT_BF16, 128>(k, s); }
     return (int)hipGetLastError();
 }
 

@@ -491,7 +491,7 @@ int mlora_kv_append(const void *q, int64_t q_stride, void *q_out, int64_t q_out_
  * T <= MLORA_ATTN_MAX_T, n_prefix <= MLORA_ATTN_MAX_PREFIX.
  */
 #define MLORA_ATTN_MAX_T 8192
-#define MLORA_ATTN_MAX_PREFIX 8192
+#define MLORA_ATTN_MAX_PREFIX 4096
 int64_t mlora_attn_plan_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads);
 int64_t mlora_attn_workspace_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads, int head_dim);
 int mlora_attn_plan(const int32_t *tok_req, const int32_t *tok_pos, int T, int n_req, int max_pages, const int32_t *req_prefix,

@@ -253,3 +253,38 @@ def test_no_tokens():
     batch = mlora.KVBatch(e, e, torch.zeros((1, 1), dtype=torch.int32, device="cuda"))
     plan = mlora.plan_attention(batch, cache, 4)
     assert mlora.prefix_attention(torch.empty((0, 4, 64), dtype=F16, device="cuda"), cache, 0, plan).shape == (0, 4, 64)
+
+
+def test_refusals():
+    s = Scene([(0, 20), (-1, 30)], [40], 4, 2, 64, 16, F16, seed=18, layers=2)
+    plan = mlora.plan_attention(s.batch, s.cache, 4)
+    q = s.dev_q
+    with pytest.raises(IndexError):
+        mlora.prefix_attention(q, s.cache, 2, plan)
+    with pytest.raises(ValueError, match="q must be"):
+        mlora.prefix_attention(q[:1], s.cache, 0, plan)
+    with pytest.raises(TypeError, match="dtype"):
+        mlora.prefix_attention(q.float(), s.cache, 0, plan)
+    with pytest.raises(ValueError, match="behind the other"):
+        mlora.prefix_attention(torch.zeros((2, 64, 4), dtype=F16, device="cuda").transpose(1, 2), s.cache, 0, plan)
+    with pytest.raises(mlora.MloraError, match="stride"):
+        mlora.prefix_attention(q[:1].expand(2, 4, 64), s.cache, 0, plan)
+    with pytest.raises(ValueError, match="another cache layout"):
+        mlora.prefix_attention(q, mlora.KVCache(1, 4, 4, 64), 0, plan)
+    with pytest.raises(ValueError, match="another cache layout"):
+        mlora.prefix_attention(q, mlora.KVCache(1, 4, 2, 64, page_tokens=32), 0, plan)
+    many = Scene([(0, 5)] * 400, [40], 4, 2, 64, 16, F16, seed=18)
+    with pytest.raises(mlora.MloraError) as e:
+        mlora.plan_attention(many.batch, many.cache, 4, out=plan)
+    assert e.value.code == mlora._ext.MLORA_ENOSPACE
+    s.compare(mlora.prefix_attention(q, s.cache, 0, plan))          # the plan is still the one it was
+    for field, value, error in (("tok_pos", s.batch.tok_pos.long(), TypeError), ("tok_pos", s.batch.tok_pos[:1], ValueError),
+                                ("pages", s.batch.pages[0], ValueError), ("pages", s.batch.pages.t(), ValueError),
+                                ("req_prefix", s.batch.req_prefix[:1], ValueError), ("prefix_len", None, ValueError),
+                                ("prefix_pages", None, ValueError), ("prefix_pages", s.batch.prefix_pages.repeat(2, 1), ValueError),
+                                ("tok_req", s.batch.tok_req.cpu(), ValueError)):
+        old = getattr(s.batch, field)
+        setattr(s.batch, field, value)
+        with pytest.raises(error):
+            mlora.plan_attention(s.batch, s.cache, 4)
+        setattr(s.batch, field, old)
