@@ -130,12 +130,9 @@ int mlora_w4_gemv_multi(int n_proj, void *const *y, const void *const *x, const 
         if (!aligned16(y[p]) || !aligned16(x[p]) || !aligned16(packed[p])) return fail(MLORA_EALIGN, "projection %d: device pointers must be 16-byte aligned", p);
         const mlora::W4Shape sh = mlora::w4_shape(hin[p], hout[p], group[p], zeros[p] != 0);
         mlora::W4Proj &w = a.pr[p];
-        const unsigned char *base = static_cast<const unsigned char *>(packed[p]);
-        w.y = y[p]; w.x = x[p]; w.codes = base;
-        w.scales = reinterpret_cast<const uint16_t *>(base + sh.scales_at);
-        w.zeros = zeros[p] ? base + sh.zeros_at : nullptr;
-        w.hin = sh.hin; w.hout = sh.hout; w.cols = sh.cols; w.k_tiles = sh.k_tiles; w.n_tiles = sh.n_tiles;
-        w.group_shift = log2_exact(sh.group); w.groups = sh.groups;
+        w.y = y[p]; w.x = x[p]; w.packed = static_cast<const unsigned char *>(packed[p]);
+        w.groups_at = sh.groups_at; w.hin = sh.hin; w.hout = sh.hout; w.k_tiles = sh.k_tiles; w.n_tiles = sh.n_tiles;
+        w.per_tile = sh.per_tile; w.zeros = zeros[p] != 0;
     }
     if (T == 0) return MLORA_OK;
     const int rc = mlora::launch_w4_gemv(a, dtype, static_cast<hipStream_t>(stream));

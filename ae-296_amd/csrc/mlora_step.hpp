@@ -9,16 +9,17 @@ namespace mlora {
 
 constexpr int STEP_MAX_PROJ = 8;
 
-// ---- 4-bit weights.  A packed weight is three planes: codes, scales, zero points.
+// ---- 4-bit weights.  A packed weight is two planes: codes, and the groups' scales and zero points.
 // Codes: tiles of 16 columns x 128 rows, 1024 bytes each, column tile major (a column tile's K tiles lie one behind the other).  In a
 // tile, lane l = 16 * q + c of a wavefront owns 16 bytes: dword s holds rows 32 s + 8 q + j (j < 8) of column c, row pair
 // (2i, 2i + 1) in nibbles i and i + 4 - the operand of one 16 x 16 x 32 MFMA.  Rows and columns past the weight's are zero codes.
-// Scales: [groups, columns rounded up to 16] 16-bit; zero points: the same in bytes.
+// Groups, tile by tile: [groups of a K tile (1, 2 or 4)][16 columns] of the 16-bit scale, or where there are zero points of a dword
+// whose upper half is 16 + the zero point; zeros past the weight's.
 constexpr int W4_TN = 16, W4_TK = 128, W4_TILE_BYTES = W4_TN * W4_TK / 2;
 struct W4Shape {
     int hin, hout, group;
-    int n_tiles, k_tiles, groups, cols;    // column tiles, K tiles, groups of a column, columns rounded up
-    int64_t scales_at, zeros_at, bytes;    // byte offsets of the planes (zeros_at: -1 where there are none), total
+    int n_tiles, k_tiles, groups, per_tile;    // column tiles, K tiles, groups of a column, groups of a K tile
+    int64_t groups_at, bytes;                  // byte offset of the second plane, total
 };
 inline W4Shape w4_shape(int hin, int hout, int group, bool zeros)
 {
@@ -27,11 +28,10 @@ inline W4Shape w4_shape(int hin, int hout, int group, bool zeros)
     s.n_tiles = (hout + W4_TN - 1) / W4_TN;
     s.k_tiles = (hin + W4_TK - 1) / W4_TK;
     s.groups = (hin + group - 1) / group;
-    s.cols = s.n_tiles * W4_TN;
-    s.scales_at = (int64_t)s.n_tiles * s.k_tiles * W4_TILE_BYTES;
-    const int64_t after = s.scales_at + (int64_t)s.groups * s.cols * 2;
-    s.zeros_at = zeros ? after : -1;
-    s.bytes = zeros ? after + (int64_t)s.groups * s.cols : after;
+    s.per_tile = W4_TK / group;
+    const int64_t tiles = (int64_t)s.n_tiles * s.k_tiles;
+    s.groups_at = tiles * W4_TILE_BYTES;
+    s.bytes = s.groups_at + tiles * s.per_tile * W4_TN * (zeros ? 4 : 2);
     return s;
 }
 
@@ -46,16 +46,17 @@ struct W4PackArgs {
 struct W4Proj {
     void *y;
     const void *x;
-    const unsigned char *codes;
-    const uint16_t *scales;
-    const uint8_t *zeros;      // nullptr: 8
-    int hin, hout, cols, k_tiles, n_tiles;
-    int group_shift;           // log2 of the group
-    int groups;
+    const unsigned char *packed;
+    int64_t groups_at;
+    int hin, hout, k_tiles, n_tiles;
+    int per_tile;              // groups of a K tile
+    int zeros;                 // 0: 8 everywhere
+    unsigned end;              // column blocks of the projections up to this one (set by the launcher)
 };
 struct W4Args {
     W4Proj pr[STEP_MAX_PROJ];
     int n_proj, T, accumulate;
+    unsigned row_blocks;       // set by the launcher
 };
 
 // ---- keys and values

@@ -40,8 +40,8 @@ def test_gemv_arguments(kw, code):
 def test_pack_arguments():
     lib = _ext.lib()
     need = lib.mlora_w4_packed_bytes(72, 24, 64, 1)
-    assert need == 2 * 1 * 1024 + 2 * 32 * 2 + 2 * 32          # two column tiles of one K tile; two groups of 32 columns
-    assert lib.mlora_w4_packed_bytes(72, 24, 64, 0) == need - 64
+    assert need == 2 * 1 * 1024 + 2 * 2 * 16 * 4               # two column tiles of one K tile; two groups of 16 columns each
+    assert lib.mlora_w4_packed_bytes(72, 24, 64, 0) == need - 2 * 2 * 16 * 2
     assert lib.mlora_w4_packed_bytes(72, 24, 48, 0) == ERANGE and lib.mlora_w4_packed_bytes(71, 24, 64, 0) == EALIGN
     pack = lambda c=one, s=one, z=one, p=one, n=need: lib.mlora_w4_pack(c, s, z, 72, 24, 64, p, n, None)     # noqa: E731
     assert pack(n=need - 1) == ENOSPACE and pack(p=off) == EALIGN
