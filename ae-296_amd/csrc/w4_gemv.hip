@@ -83,49 +83,182 @@ template <int NT> struct W4Tile {
     uint32_t group[NT];
 };
 
-// A workgroup: NT column tiles x MT token tiles, its eight wavefronts share the K tiles (every eighth each, so that together they read
-// a column tile's codes in one stretch) and are joined in LDS.  A wavefront asks for its next K tile's codes, groups and - where that
-// is few registers - x before it multiplies the present one.  A lane loads the scale and zero point of one column and K step; the
-// result's layout wants those of four columns, which come from their lanes through the LDS crossbar.
-template <int DT, int MT, int NT>
-__global__ __launch_bounds__(64 * W4_WAVES, MT * NT <= 4 ? 4 : 2) void w4_gemv_kernel(const W4Args p)
+// The column block, token block and projection of a workgroup.  Eight neighbouring ids go to the eight XCDs: the token blocks of one
+// column block follow each other on one of them.
+struct W4Place { int proj; unsigned col_block, row_block; };
+__device__ __forceinline__ W4Place w4_place(const W4Args &p)
 {
-    constexpr bool XPRE = MT == 1 && NT < 4;
-    __shared__ float part[W4_WAVES][MT * 16][17];
-    // eight neighbouring ids go to the eight XCDs: the token blocks of one column block follow each other on one of them
-    const unsigned id = blockIdx.x, blk = (id >> 3) / p.row_blocks, rb = (id >> 3) - blk * p.row_blocks;
-    unsigned cb = blk * 8 + (id & 7);
-    int proj = 0;
-    while (proj + 1 < p.n_proj && cb >= p.pr[proj].end) proj++;
-    const W4Proj &w = p.pr[proj];
-    if (cb >= w.end) return;
-    cb -= proj ? p.pr[proj - 1].end : 0;
-    const int nt0 = (int)cb * NT, t0 = (int)rb * (MT * 16);
+    const unsigned id = blockIdx.x, blk = (id >> 3) / p.row_blocks;
+    W4Place at = {0, blk * 8 + (id & 7), (id >> 3) - blk * p.row_blocks};
+    while (at.proj < p.n_proj && at.col_block >= p.pr[at.proj].end) at.proj++;
+    if (at.proj && at.proj < p.n_proj) at.col_block -= p.pr[at.proj - 1].end;
+    return at;                                                    // proj == n_proj: no such block
+}
+
+// Up to 16 tokens.  A workgroup: NT column tiles, its eight wavefronts share the K tiles (every eighth each, so that together they read
+// a column tile's codes in one stretch) and are joined in LDS.  A wavefront asks for its next K tile's codes, groups and x before it
+// multiplies the present one.  A lane loads the scale and zero point of one column and K step; the result's layout wants those of
+// four columns, which it gets through LDS.  Bound by the way in and out at one projection (4096 -> 4096, one token: 4.7 us for 8.4 MB; the
+// launch alone takes half) and by vector instructions beyond (5120 -> 27648, 70.8 MB: 20.8 us, 3.4 TB/s).
+template <int DT, int NT, int STEPS>
+__global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args p)
+{
+    constexpr int PER_TILE = 4 / STEPS;
+    __shared__ float part[W4_WAVES][16][17];
+    __shared__ __attribute__((aligned(16))) uint32_t words[W4_WAVES][NT][64];
+    const W4Place place = w4_place(p);
+    if (place.proj == p.n_proj) return;
+    const W4Proj &w = p.pr[place.proj];
+    const int nt0 = (int)place.col_block * NT, t0 = (int)place.row_block * 16;
+    const unsigned char *codes = w.packed, *groups = w.packed + w.groups_at;
+    const int hin = w.hin, k_tiles = w.k_tiles, n_last = w.n_tiles - 1;
+    const bool zeros = w.zeros != 0;
+    const uint32_t middle = zeros ? 0u : 24u << 16;               // 16 + 8 where no zero points are stored; joined where it is used: a load is
+                                                                  // waited for by the first instruction that touches what it brings
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-    const unsigned char *x0row = static_cast<const unsigned char *>(w.x) + (size_t)t0 * w.hin * 2;
-    uint32_t xrow[MT];                                            // bytes from it: 64 rows of 2^24 columns at most
-#pragma unroll
-    for (int m = 0; m < MT; m++) xrow[m] = ((uint32_t)min(m * 16 + c, p.T - 1 - t0) * (uint32_t)w.hin + q * 8) * 2;
+    const unsigned char *x_block = static_cast<const unsigned char *>(w.x) + (size_t)t0 * hin * 2;
+    const uint32_t x_row = ((uint32_t)min(c, p.T - 1 - t0) * (uint32_t)hin + q * 8) * 2;
     const uint32_t one = DT == DT_F16 ? 0x3c003c00u : 0x3f803f80u;
     const uint4 ones = make_uint4(one, one, one, one);
-    const int steps = 4 / w.per_tile;                             // K steps of 32 rows in a group
-    const unsigned glane = (q / steps) * W4_TN + c;
+    const unsigned group_lane = (q / STEPS) * W4_TN + c;
 
-    auto load = [&](W4Tile<NT> &b, int kt) {
+    auto fetch = [&](W4Tile<NT> &b, uint4 (&x)[4], int kt) {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const int nt = min(nt0 + n, w.n_tiles - 1);          // a block past the last column tile repeats it and stores nothing
-            const size_t tile = (size_t)nt * w.k_tiles + kt;
-            b.code[n] = ldg16_stream(w.packed + tile * W4_TILE_BYTES + lane * 16);
-            const unsigned char *plane = w.packed + w.groups_at;
-            const size_t at = tile * (w.per_tile * W4_TN) + glane;
-            b.group[n] = w.zeros ? reinterpret_cast<const uint32_t *>(plane)[at] : reinterpret_cast<const uint16_t *>(plane)[at] | 24u << 16;
+            const size_t tile = (size_t)min(nt0 + n, n_last) * k_tiles + kt;   // past the last column tile: that one, and nothing is stored
+            const size_t at = tile * (PER_TILE * W4_TN) + group_lane;
+            b.code[n] = ldg16_stream(codes + tile * W4_TILE_BYTES + lane * 16);
+            b.group[n] = zeros ? reinterpret_cast<const uint32_t *>(groups)[at] : reinterpret_cast<const uint16_t *>(groups)[at];
+        }
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const int k = kt * W4_TK + s * 32;
+            x[s] = k + q * 8 < hin ? ldg16(x_block + (x_row + (uint32_t)k * 2)) : zero16();
         }
     };
-    auto xload = [&](uint4 (&x)[MT], int kt, int s) {
-        const int k = kt * W4_TK + s * 32;
+
+    float4_t out[NT];
 #pragma unroll
-        for (int m = 0; m < MT; m++) x[m] = k + q * 8 < w.hin ? ldg16(x0row + (xrow[m] + (uint32_t)k * 2)) : zero16();
+    for (int n = 0; n < NT; n++) out[n] = float4_t{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const W4Tile<NT> &b, const uint4 (&x)[4]) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) words[wave][n][lane] = b.group[n];
+        __builtin_amdgcn_wave_barrier();
+        float4_t acc[NT], sum;
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const bool begins = s % STEPS == 0;                   // a group begins here: its sums start from nothing
+            const float4_t none = {0.f, 0.f, 0.f, 0.f};
+            sum = mfma16<DT>(ones, x[s], begins ? none : sum);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+                acc[n] = mfma16<DT>(widen<DT>(s == 0 ? b.code[n].x : s == 1 ? b.code[n].y : s == 2 ? b.code[n].z : b.code[n].w), x[s], begins ? none : acc[n]);
+            if ((s + 1) % STEPS == 0) {                           // and ends here
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const uint4 g = *reinterpret_cast<const uint4 *>(&words[wave][n][s / STEPS * STEPS * 16 + q * 4]);
+                    const uint32_t u[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) out[n][i] += lo_f32<DT>(u[i]) * (acc[n][i] - (float)((u[i] | middle) >> 16) * sum[i]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);                    // or the steps' operands are all made at once and the registers run out
+        }
+    };
+    if (wave < k_tiles) {
+        W4Tile<NT> b0, b1;
+        uint4 x0[4], x1[4];
+        int kt = wave;
+        fetch(b0, x0, kt);
+#pragma unroll 1
+        for (;;) {
+            kt += W4_WAVES;
+            if (kt < k_tiles) fetch(b1, x1, kt);
+            multiply(b0, x0);
+            if (kt >= k_tiles) break;
+            kt += W4_WAVES;
+            if (kt < k_tiles) fetch(b0, x0, kt);
+            multiply(b1, x1);
+            if (kt >= k_tiles) break;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        if (n) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++) part[wave][c][q * 4 + i] = out[n][i];
+        __syncthreads();
+        if (threadIdx.x >= 128) continue;
+        const int r = threadIdx.x >> 3, col = (threadIdx.x & 7) * 2, at = (nt0 + n) * W4_TN + col;
+        if (t0 + r >= p.T || at >= w.hout) continue;
+        float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < W4_WAVES; k++) { v0 += part[k][r][col]; v1 += part[k][r][col + 1]; }
+        uint32_t *y = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(w.y) + (size_t)(t0 + r) * w.hout + at);
+        if (p.accumulate) { v0 += lo_f32<DT>(*y); v1 += hi_f32<DT>(*y); }
+        *y = pack2<DT>(v0, v1);
+    }
+}
+
+// ------------------------------------------------------------------ product, more tokens
+// From 17 tokens on a wavefront of the kernel above would read more bytes of x than of codes.  Here WN wavefronts side by side (NT column
+// tiles each) share the x of a K tile through LDS, and the 8 / WN such parts of a workgroup take K tiles by turns.  x comes by loads
+// that fill LDS directly, whole rows of 256 bytes; 16-byte chunk `ch` of row r lies at chunk ch ^ (r % 16), so that the operand reads (one
+// chunk of sixteen rows) meet all banks.
+//
+// A K tile takes a wavefront less time than a load from HBM: codes are asked for three tiles ahead, x two.  The loads to LDS are
+// inline assembly, because the compiler would end them before any read of LDS; not knowing of them it waits for codes somewhat
+// earlier than it has to, one reason for the third tile.
+template <int DT, int MT, int NT, int WN, int STEPS>
+__global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args p)
+{
+    constexpr int WK = W4_WAVES / WN, BUFS = 4, AHEAD = 2;
+    constexpr int XTILE = MT * 16 * W4_TK * 2, XLOADS = MT * 4 / WN;     // bytes of x of a K tile, loads of a wavefront for it
+    static_assert(XLOADS >= 1, "a wavefront's loads to LDS");
+    constexpr int EXCHANGE = (W4_WAVES - WN) * MT * 16 * 17 * 4, RINGS = WK * BUFS * XTILE;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[EXCHANGE > RINGS ? EXCHANGE : RINGS];
+    const W4Place place = w4_place(p);
+    if (place.proj == p.n_proj) return;
+    const W4Proj &w = p.pr[place.proj];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    const int wn = wave & (WN - 1), wk = wave / WN;
+    const int nt0 = (int)place.col_block * (WN * NT) + wn * NT, t0 = (int)place.row_block * (MT * 16);
+    const unsigned char *codes = w.packed, *groups = w.packed + w.groups_at;
+    const int hin = w.hin, k_tiles = w.k_tiles, n_last = w.n_tiles - 1;
+    const bool zeros = w.zeros != 0;
+    const uint32_t middle = zeros ? 0u : 24u << 16;               // 16 + 8 where no zero points are stored; joined where it is used: a load is
+                                                                  // waited for by the first instruction that touches what it brings
+    const uint32_t one = DT == DT_F16 ? 0x3c003c00u : 0x3f803f80u;
+    const uint4 ones = make_uint4(one, one, one, one);
+    constexpr int PER_TILE = 4 / STEPS;
+    const unsigned glane = (q / STEPS) * W4_TN + c;
+
+    auto load = [&](W4Tile<NT> &b, int at_kt) {
+        const int kt = min(at_kt, k_tiles - 1);                 // past the end: loaded again and not used
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const size_t tile = (size_t)min(nt0 + n, n_last) * k_tiles + kt;        // past the last column tile: that one, and nothing is stored
+            const size_t at = tile * (PER_TILE * W4_TN) + glane;
+            b.group[n] = zeros ? reinterpret_cast<const uint32_t *>(groups)[at] : reinterpret_cast<const uint16_t *>(groups)[at];
+            b.code[n] = ldg16_stream(codes + tile * W4_TILE_BYTES + lane * 16);
+        }
+    };
+    // this wavefront's share of its part's x tile: four rows a load
+    const unsigned char *x0 = static_cast<const unsigned char *>(w.x) + (size_t)t0 * hin * 2;
+    unsigned char *tiles = lds + wk * (BUFS * XTILE);
+    const uint32_t tiles_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)tiles;
+    __shared__ __attribute__((aligned(16))) uint32_t all_words[W4_WAVES][NT * 64];
+    uint32_t *words = all_words[wave];
+    const unsigned char *mine = reinterpret_cast<const unsigned char *>(words + q * 4);
+    auto xload = [&](int at_kt, int buf) {
+        const int kt = min(at_kt, k_tiles - 1);
+#pragma unroll
+        for (int m = 0; m < XLOADS; m++) {
+            const int r = (wn * XLOADS + m) * 4 + q;
+            const int k = min(kt * W4_TK + (c ^ (r & 15)) * 8, hin - 8);          // columns past the last: taken for zeros where they are used
+            const unsigned char *src = x0 + ((uint32_t)min(r, p.T - 1 - t0) * (uint32_t)hin + k) * 2;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(tiles_at + buf * XTILE + (wn * XLOADS + m) * 1024), "v"(src) : "memory");
+        }
     };
 
     float4_t out[MT][NT];
@@ -133,127 +266,198 @@ __global__ __launch_bounds__(64 * W4_WAVES, MT * NT <= 4 ? 4 : 2) void w4_gemv_k
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int n = 0; n < NT; n++) out[m][n] = float4_t{0.f, 0.f, 0.f, 0.f};
-    // one K tile against x[0..3] (XPRE) or x[0], x[1] by turns, the next step's x on its way
-    auto multiply = [&](const W4Tile<NT> &b, int kt, uint4 (&x)[XPRE ? 4 : 2][MT], int next) {
+    // tile kt from buffer `buf`
+    auto multiply = [&](const W4Tile<NT> &b, W4Tile<NT> &ahead, int kt, int buf) {
+        load(ahead, kt + 3 * WK);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < NT; n++) words[n * 64 + lane] = b.group[n];
+        __builtin_amdgcn_wave_barrier();
         float4_t acc[MT][NT], sum[MT];
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            sum[m] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int n = 0; n < NT; n++) acc[m][n] = float4_t{0.f, 0.f, 0.f, 0.f};
-        }
-#pragma unroll
         for (int s = 0; s < 4; s++) {
-            uint4 (&now)[MT] = x[XPRE ? s : s & 1];
-            if constexpr (!XPRE) {
-                if (s < 3) xload(x[(s + 1) & 1], kt, s + 1);
-                else if (next < w.k_tiles) xload(x[0], next, 0);
+            const bool begins = s % STEPS == 0, ends = (s + 1) % STEPS == 0;      // of a group
+            const float4_t none = {0.f, 0.f, 0.f, 0.f};
+            uint4 x[MT];
+#pragma unroll
+            for (int m = 0; m < MT; m++) x[m] = *reinterpret_cast<const uint4 *>(tiles + buf * XTILE + (m * 16 + c) * 256 + ((s * 4 + q) ^ c) * 16);
+            const int k = kt * W4_TK + s * 32;
+            if (k + 32 > hin) {
+                const uint32_t keep = k + q * 8 < hin ? ~0u : 0u;
+#pragma unroll
+                for (int m = 0; m < MT; m++) x[m] = make_uint4(x[m].x & keep, x[m].y & keep, x[m].z & keep, x[m].w & keep);
+            }
+            uint4 group[NT];
+            if (ends) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) group[n] = *reinterpret_cast<const uint4 *>(mine + (n * 64 + s / STEPS * STEPS * 16) * 4);
             }
 #pragma unroll
-            for (int m = 0; m < MT; m++) sum[m] = mfma16<DT>(ones, now[m], sum[m]);
+            for (int m = 0; m < MT; m++) sum[m] = mfma16<DT>(ones, x[m], begins ? none : sum[m]);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const uint4 a = widen<DT>(s == 0 ? b.code[n].x : s == 1 ? b.code[n].y : s == 2 ? b.code[n].z : b.code[n].w);
 #pragma unroll
-                for (int m = 0; m < MT; m++) acc[m][n] = mfma16<DT>(a, now[m], acc[m][n]);
+                for (int m = 0; m < MT; m++) acc[m][n] = mfma16<DT>(a, x[m], begins ? none : acc[m][n]);
             }
-            if (((s + 1) & (steps - 1)) == 0) {                   // the group ends here
-                const int src = (s & ~(steps - 1)) * 16 + q * 4;
+            if (ends) {
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
+                    const uint32_t u[4] = {group[n].x, group[n].y, group[n].z, group[n].w};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const uint32_t u = (uint32_t)__builtin_amdgcn_ds_bpermute((src + i) * 4, (int)b.group[n]);
-                        const float f = lo_f32<DT>(u & 0xffffu), z = (float)(u >> 16);
+                        const float f = lo_f32<DT>(u[i]), z = (float)((u[i] | middle) >> 16);
 #pragma unroll
                         for (int m = 0; m < MT; m++) out[m][n][i] += f * (acc[m][n][i] - z * sum[m][i]);
                     }
                 }
-#pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    sum[m] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int n = 0; n < NT; n++) acc[m][n] = float4_t{0.f, 0.f, 0.f, 0.f};
-                }
             }
-            __builtin_amdgcn_sched_barrier(0);                    // or the steps' operands are all made at once and the registers run out
+            __builtin_amdgcn_sched_barrier(0);
+            if (s == 0) xload(kt + AHEAD * WK, (buf + AHEAD) % BUFS);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        // the next tile's x, asked for a tile ago: behind it came this tile's loads of codes, groups and x
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * NT + XLOADS) : "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
     };
-    int kt = wave;
-    if (kt < w.k_tiles) {
-        W4Tile<NT> b0, b1;
-        uint4 x0[XPRE ? 4 : 2][MT], x1[XPRE ? 4 : 1][MT];
-        auto fetch = [&](W4Tile<NT> &b, uint4 (*x)[MT], int at) {
-            load(b, at);
-            if constexpr (XPRE) {
-#pragma unroll
-                for (int s = 0; s < 4; s++) xload(x[s], at, s);
-            }
-        };
-        fetch(b0, x0, kt);
-        if constexpr (!XPRE) xload(x0[0], kt, 0);
+    W4Tile<NT> b0, b1, b2, b3;
+    // all parts pass the same barriers: where one has no last tile it multiplies by zeros (k is past the last column)
+    load(b0, wk);
+    __builtin_amdgcn_sched_barrier(0);
+    xload(wk, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    load(b1, wk + WK);
+    __builtin_amdgcn_sched_barrier(0);
+    xload(wk + WK, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    load(b2, wk + 2 * WK);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(4 * NT + XLOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
-        for (;;) {
-            int next = kt + W4_WAVES;
-            if (next < w.k_tiles) fetch(b1, x1, next);
-            multiply(b0, kt, x0, next);
-            if (next >= w.k_tiles) break;
-            kt = next;
-            next = kt + W4_WAVES;
-            if (next < w.k_tiles) fetch(b0, x0, next);
-            if constexpr (XPRE) multiply(b1, kt, x1, next); else multiply(b1, kt, x0, next);
-            if (next >= w.k_tiles) break;
-            kt = next;
-        }
+    for (int kt = wk, left = (k_tiles + WK - 1) / WK;;) {
+        multiply(b0, b3, kt, 0);
+        kt += WK;
+        if (--left == 0) break;
+        multiply(b1, b0, kt, 1);
+        kt += WK;
+        if (--left == 0) break;
+        multiply(b2, b1, kt, 2);
+        kt += WK;
+        if (--left == 0) break;
+        multiply(b3, b2, kt, 3);
+        kt += WK;
+        if (--left == 0) break;
     }
+    __builtin_amdgcn_s_waitcnt(0);                                // loads to the ring may still be on their way
+    // the parts' sums, one column tile of each wavefront at a time
+    float (*part)[MT * 16][17] = reinterpret_cast<float (*)[MT * 16][17]>(lds);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        if (n) __syncthreads();
+        if constexpr (WK > 1) {
+            __syncthreads();
+            if (wk) {
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+                for (int m = 0; m < MT; m++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) part[wave][m * 16 + c][q * 4 + i] = out[m][n][i];
-        __syncthreads();
-        for (int e = threadIdx.x; e < MT * 128; e += 64 * W4_WAVES) {
-            const int r = e >> 3, col = (e & 7) * 2, at = (nt0 + n) * W4_TN + col;
-            if (t0 + r >= p.T || at >= w.hout) continue;
-            float v0 = 0.f, v1 = 0.f;
+                    for (int i = 0; i < 4; i++) part[wave - WN][m * 16 + c][q * 4 + i] = out[m][n][i];
+            }
+            __syncthreads();
+            if (wk) continue;
 #pragma unroll
-            for (int k = 0; k < W4_WAVES; k++) { v0 += part[k][r][col]; v1 += part[k][r][col + 1]; }
-            uint32_t *y = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(w.y) + (size_t)(t0 + r) * w.hout + at);
-            if (p.accumulate) { v0 += lo_f32<DT>(*y); v1 += hi_f32<DT>(*y); }
-            *y = pack2<DT>(v0, v1);
+            for (int k = 1; k < WK; k++)
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) out[m][n][i] += part[(k - 1) * WN + wn][m * 16 + c][q * 4 + i];
+        }
+        const int col = (nt0 + n) * W4_TN + q * 4;
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const int r = t0 + m * 16 + c;
+            if (r >= p.T || col >= w.hout) continue;
+            uint2 *y = reinterpret_cast<uint2 *>(static_cast<uint16_t *>(w.y) + (size_t)r * w.hout + col);
+            float4_t v = out[m][n];
+            if (p.accumulate) {
+                const uint2 old = *y;
+                v += float4_t{lo_f32<DT>(old.x), hi_f32<DT>(old.x), lo_f32<DT>(old.y), hi_f32<DT>(old.y)};
+            }
+            *y = make_uint2(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
         }
     }
 }
 
-template <int DT, int MT, int NT>
-static void gemv_of(W4Args a, hipStream_t s)
+// ------------------------------------------------------------------ launches
+// Numbers the column blocks of `cols` column tiles, and gives the workgroups of `rows` tokens each.
+static unsigned w4_blocks(W4Args &a, int cols, int rows)
 {
     unsigned end = 0;
     for (int p = 0; p < a.n_proj; p++) {
-        end += (unsigned)((a.pr[p].n_tiles + NT - 1) / NT);
+        end += (unsigned)((a.pr[p].n_tiles + cols - 1) / cols);
         a.pr[p].end = end;
     }
-    a.row_blocks = (unsigned)((a.T + MT * 16 - 1) / (MT * 16));
-    hipLaunchKernelGGL((w4_gemv_kernel<DT, MT, NT>), dim3((end + 7) / 8 * 8 * a.row_blocks), dim3(64 * W4_WAVES), 0, s, a);
+    a.row_blocks = (unsigned)((a.T + rows - 1) / rows);
+    return end * a.row_blocks;
+}
+
+static dim3 w4_grid(const W4Args &a) { return dim3((a.pr[a.n_proj - 1].end + 7) / 8 * 8 * a.row_blocks); }
+
+template <int DT, int NT, int STEPS>
+static void gemv_of(W4Args &a, hipStream_t s)
+{
+    w4_blocks(a, NT, 16);
+    hipLaunchKernelGGL((w4_gemv_kernel<DT, NT, STEPS>), w4_grid(a), dim3(64 * W4_WAVES), 0, s, a);
+}
+
+template <int DT, int MT, int NT, int WN, int STEPS>
+static void wide_of(W4Args &a, hipStream_t s)
+{
+    w4_blocks(a, WN * NT, MT * 16);
+    hipLaunchKernelGGL((w4_wide_kernel<DT, MT, NT, WN, STEPS>), w4_grid(a), dim3(64 * W4_WAVES), 0, s, a);
+}
+
+// The projections of one group size.  Up to 16 tokens: two column tiles a workgroup once one each makes more workgroups than compute units
+// (16 tokens, 4096 -> 22016, group 128: 17.6 us against 26.2 with one and 18.0 with four; 4096 -> 4096: 8.0 against 6.7).
+// Beyond: the smallest workgroup whose number still runs in one round, since a round costs the walk over K (us, group 128, for
+// the forms in the order below; 4096 -> 4096, 32 tokens: 10.5 15.3 19.8 33.6 49.1; 4096 -> 22016, 32 tokens: 29.0 22.6 39.3 34.9 49.7,
+// 64: 55.6 34.1 39.4 35.1 51.0, 125: 95.9 58.3 57.9 67.6 51.8; 5120 -> 27648, 125: 145 86.8 92.8 83.9 64.0).  Two workgroups of the second
+// form fit a compute unit.  The last form's accumulators fit the registers with one group a K tile only.
+template <int DT, int STEPS>
+static void gemv_by_size(W4Args a, hipStream_t s)
+{
+    const unsigned cus = (unsigned)device_compute_units();
+    if (a.T <= 16) {
+        if (w4_blocks(a, 1, 16) > cus) gemv_of<DT, 2, STEPS>(a, s); else gemv_of<DT, 1, STEPS>(a, s);
+        return;
+    }
+    if (w4_blocks(a, 2, 32) <= cus) return wide_of<DT, 2, 1, 2, STEPS>(a, s);
+    if (w4_blocks(a, 4, 32) <= 2 * cus) return wide_of<DT, 2, 1, 4, STEPS>(a, s);
+    if (w4_blocks(a, 4, 64) <= cus) return wide_of<DT, 4, 1, 4, STEPS>(a, s);
+    if (w4_blocks(a, 8, 64) <= cus) return wide_of<DT, 4, 1, 8, STEPS>(a, s);
+    if constexpr (STEPS == 4) wide_of<DT, 4, 2, 8, STEPS>(a, s);
+    else wide_of<DT, 4, 1, 4, STEPS>(a, s);
 }
 
 template <int DT>
-static void gemv_by_size(const W4Args &a, hipStream_t s)
+static void gemv_by_group(const W4Args &all, hipStream_t s)
 {
-    int tiles = 0;
-    for (int p = 0; p < a.n_proj; p++) tiles += a.pr[p].n_tiles;
-    const int cus = device_compute_units();
-    const int nt = tiles >= 4 * cus ? 4 : tiles >= 2 * cus ? 2 : 1;
-    if (a.T <= 16) { if (nt == 4) gemv_of<DT, 1, 4>(a, s); else if (nt == 2) gemv_of<DT, 1, 2>(a, s); else gemv_of<DT, 1, 1>(a, s); }
-    else if (a.T <= 32) { if (nt == 4) gemv_of<DT, 2, 4>(a, s); else if (nt == 2) gemv_of<DT, 2, 2>(a, s); else gemv_of<DT, 2, 1>(a, s); }
-    else { if (nt == 4) gemv_of<DT, 4, 4>(a, s); else if (nt == 2) gemv_of<DT, 4, 2>(a, s); else gemv_of<DT, 4, 1>(a, s); }
+    for (int per_tile = 1; per_tile <= 4; per_tile *= 2) {        // a call's projections usually have one group size
+        W4Args a = all;
+        a.n_proj = 0;
+        for (int p = 0; p < all.n_proj; p++)
+            if (all.pr[p].per_tile == per_tile) a.pr[a.n_proj++] = all.pr[p];
+        if (a.n_proj == 0) continue;
+        if (per_tile == 1) gemv_by_size<DT, 4>(a, s);
+        else if (per_tile == 2) gemv_by_size<DT, 2>(a, s);
+        else gemv_by_size<DT, 1>(a, s);
+    }
 }
 
 int launch_w4_gemv(const W4Args &a, int dtype, hipStream_t s)
 {
-    if (dtype == DT_F16) gemv_by_size<DT_F16>(a, s); else gemv_by_size<DT_BF16>(a, s);
+    if (dtype == DT_F16) gemv_by_group<DT_F16>(a, s); else gemv_by_group<DT_BF16>(a, s);
     return (int)hipGetLastError();
 }
 
