@@ -2,10 +2,11 @@
 //     out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j,   j over positions 0 .. tok_pos[t] of t's request
 // with the keys of a shared prefix on the prefix's pages and the others on the request's own.
 //
-// Three kernels.  The plan (once per step) cuts the work into items: up to 32 query rows x a range of keys of one list.  The rows of
-// an item are the query heads that read one key head, of one token over its own keys, or of all tokens behind a prefix over
-// the prefix's, so those are read once for 32 rows.  The attention kernel runs an item per workgroup and key head, the join adds up the
-// parts of rows that were cut, with their maxima and sums.
+// Three kernels.  The plan (once per step) cuts the work into items: some query rows x a range of keys of one list.  The rows of an item
+// are the query heads that read one key head, of one token over its own keys, or of the tokens behind a prefix over the
+// prefix's.  The attention kernel runs an item per workgroup and key head: up to 32 rows with the keys shared by its wavefronts, which is
+// what reading keys once takes, or up to 128 with the rows shared, each wavefront 32 of them, and the keys brought to LDS for all.  The join
+// adds up the parts of rows that were cut, with their maxima and sums.
 //
 // One pass over the keys with the running maximum m and sum l of the softmax.  A wavefront multiplies 32 keys at a time with 16 query
 // rows on v_mfma_f32_16x16x32: first S^T = K q^T, whose result leaves every lane with eight scores of ONE query row (column lane % 16; keys
@@ -31,7 +32,8 @@ __device__ __forceinline__ float4_t pa_mfma(const uint4 &a, const uint4 &b, floa
 }
 
 constexpr int PA_WAVES = 4;
-constexpr int PA_ROWS = 32;                    // query rows of an item at most
+constexpr int PA_ROWS = 32;                    // query rows of an item whose wavefronts share the keys, at most
+constexpr int PA_WIDE = 128;                   // of one whose wavefronts share the rows
 constexpr int PA_KEYS = 32;                    // keys of a block
 constexpr float PA_LOG2E = 1.44269504088896341f;
 
@@ -40,7 +42,7 @@ constexpr float PA_LOG2E = 1.44269504088896341f;
 template <int D> __device__ __forceinline__ int pa_swizzle(int r, int c) { return D == 128 ? c ^ ((r & 7) << 1) : c ^ (((r >> 1) & 3) << 1); }
 
 // ------------------------------------------------------------------ plan
-// Item (int32 words): [0] query rows (<= PA_ROWS), [1] the token (own keys) or the first entry of the group's token list, [2] 1: a group,
+// Item (int32 words): [0] query rows (at most PA_ROWS, or PA_WIDE of a group), [1] the token (own keys) or the first entry of the group's token list, [2] 1: a group,
 // [3] first row of the group's, row r being head r % gq of list entry r / gq, [4] row of the table, [5] 1: the prefix table,
 // [6], [7] keys [first, last), [8] slot of list entry 0 for this key range, -1: the rows have no other part and go to `out`.
 // Join record of a token: [0] first slot of its own parts, [1] how many, [2] first slot of its prefix parts, [3] how many, [4] slots from one
@@ -68,7 +70,7 @@ inline int64_t pa_items_cap(int T, int n_prefix, int gq, int n_kv_heads)
 }
 inline int64_t pa_slots_cap(int T, int n_prefix, int gq, int n_kv_heads)
 {
-    const int64_t target = pa_target(n_kv_heads), per_tile = (PA_ROWS + gq - 1) / gq;
+    const int64_t target = pa_target(n_kv_heads), per_tile = (PA_WIDE + gq - 1) / gq;
     return (int64_t)T * (n_prefix ? 2 : 1) + target * (n_prefix ? per_tile : 1) + 1;
 }
 
@@ -142,14 +144,18 @@ __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
     __syncthreads();
     // how much there is
     unsigned long long work = 0;
+    TokenRun first = {-1, 0, 0, 0};            // of token threadIdx.x: looked up once
     for (int t = threadIdx.x; t < T; t += PL_THREADS) {
         const TokenRun r = pa_token(p.b, p.page_shift, t);
+        if (t == (int)threadIdx.x) first = r;
         work += (unsigned)r.own;
         if (r.prefix >= 0) atomicAdd(&s_count[r.prefix], 1);
     }
     __syncthreads();
     auto prefix_keys = [&](int f) { return (int)min((long long)p.b.prefix_len[f], (long long)p.b.max_prefix_pages << p.page_shift); };
-    auto tiles_of = [&](int f) { return (int)(((long long)s_count[f] * p.gq + PA_ROWS - 1) / PA_ROWS); };
+    // 65 rows and more in wide tiles: the prefix comes from L2 once for 128 rows instead of once for 32
+    auto rows_of = [&](int f) { return (long long)s_count[f] * p.gq > 2 * PA_ROWS ? PA_WIDE : PA_ROWS; };
+    auto tiles_of = [&](int f) { return (int)(((long long)s_count[f] * p.gq + rows_of(f) - 1) / rows_of(f)); };
     for (int f = threadIdx.x; f < F; f += PL_THREADS)
         if (s_count[f]) work += (unsigned long long)prefix_keys(f) * tiles_of(f);
     for (int o = 32; o; o >>= 1) work += __shfl_xor(work, o);
@@ -157,7 +163,7 @@ __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
     __syncthreads();
     // keys of a range, a multiple of what the wavefronts take at a time
     const long long step = PA_WAVES * PA_KEYS;
-    const long long C = (((long long)s_work + p.target - 1) / p.target + step - 1) / step * step;
+    const long long C = max((((long long)s_work + p.target - 1) / p.target + step - 1) / step, 1LL) * step;
     auto range_of = [&](int keys, int cuts) { return ((keys + (long long)cuts - 1) / cuts + step - 1) / step * step; };
     auto cuts_of = [&](int keys) { return keys > 0 ? (int)((keys + C - 1) / C) : 0; };
     // groups: their lists, slots and items
@@ -180,8 +186,9 @@ __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
         const int cut = at / tiles, tile = at - cut * tiles;       // the tiles of a range lie side by side: they share its keys in L2
         const long long per = range_of(keys, cuts);
         int32_t *e = v.items + (size_t)i * PA_ITEM;
-        e[0] = (int)min((long long)PA_ROWS, (long long)s_count[f] * p.gq - (long long)tile * PA_ROWS);
-        e[1] = s_list[f]; e[2] = 1; e[3] = tile * PA_ROWS; e[4] = f; e[5] = 1;
+        const int rows = rows_of(f);
+        e[0] = (int)min((long long)rows, (long long)s_count[f] * p.gq - (long long)tile * rows);
+        e[1] = s_list[f]; e[2] = 1; e[3] = tile * rows; e[4] = f; e[5] = 1;
         e[6] = (int)min(cut * per, (long long)keys); e[7] = (int)min((cut + 1) * per, (long long)keys);
         e[8] = s_slot[f] + cut * s_count[f];
     }
@@ -196,7 +203,7 @@ __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
         TokenRun r = {-1, 0, 0, 0};
         int place = 0, prefix_cuts = 0;
         if (t < T) {
-            r = pa_token(p.b, p.page_shift, t);
+            r = t0 ? pa_token(p.b, p.page_shift, t) : first;
             if (r.prefix >= 0) {
                 place = atomicAdd(&s_take[r.prefix], 1);
                 if (s_list[r.prefix] + place < T) v.list[s_list[r.prefix] + place] = t;
@@ -272,9 +279,11 @@ struct Walk {
         return page < p.n_pages ? page : -1;
     }
 
-    // Issue the loads of the block at key0 (a block past the end is loaded from page 0 and masked).
+    // Issue the loads of the block at key0 (keys past the last are loaded from page 0 and masked).  STREAM: keys that nobody else reads.
+    template <bool STREAM>
     __device__ __forceinline__ void load(KeyBlock<D> &b, int key0)
     {
+        auto get = [](const uint16_t *src) { return STREAM ? ldg16_stream(src) : ldg16(src); };
         // what differs between lanes is one 32-bit offset for K and one for V: the rest of an address is the same for the wavefront
         const int lane = threadIdx.x & 63;
         const unsigned klane = (lane & 15) * D + (lane >> 4) * 8, vlane = (lane / CH) * D + (lane % CH) * 8;
@@ -286,9 +295,9 @@ struct Walk {
             const size_t row0 = (((size_t)(page >= 0 ? page : 0) * p.n_kv_heads + head) << p.page_shift) + (at & ((1 << p.page_shift) - 1));
             const uint16_t *k = p.k_pages + row0 * D, *v = p.v_pages + row0 * D;
 #pragma unroll
-            for (int s = 0; s < KS; s++) b.k[h][s] = ldg16(k + klane + s * 32);
+            for (int s = 0; s < KS; s++) b.k[h][s] = get(k + klane + s * 32);
 #pragma unroll
-            for (int u = 0; u < VL / 2; u++) b.v[h * (VL / 2) + u] = ldg16(v + vlane + u * (64 / CH) * D);
+            for (int u = 0; u < VL / 2; u++) b.v[h * (VL / 2) + u] = get(v + vlane + u * (64 / CH) * D);
         }
     }
 
@@ -379,20 +388,20 @@ struct Walk {
         __builtin_amdgcn_wave_barrier();
     }
 
-    template <int NR>
+    template <int NR, bool STREAM>
     __device__ __forceinline__ void all(RowState<D> (&st)[NR])
     {
         int key0 = first;
         if (key0 >= last) return;
         float4_t s[NR][2];
         KeyBlock<D> b;
-        load(b, key0);
+        load<STREAM>(b, key0);
         // the next block comes during the softmax and the second product, into the same registers
 #pragma unroll 1
         while (key0 + PA_KEYS < last) {
             scores<NR>(b, key0, st, s);
             key0 += PA_KEYS;
-            load(b, key0);
+            load<STREAM>(b, key0);
             sums<NR>(st, s);
         }
         scores<NR>(b, key0, st, s);
@@ -403,7 +412,7 @@ struct Walk {
 constexpr int pa_pitch(int D) { return D + 4; }            // floats of a row in the LDS exchange: a float4 of 16 rows meets all banks
 
 // One item for one key head: NR tiles of 16 query rows, the keys shared by the four wavefronts and joined in LDS.
-template <int DT, int D, int NR>
+template <int DT, int D, int NR, bool STREAM>
 __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const int32_t *e, const PlanView &pv, int head, unsigned char *lds, float (*s_m)[16], float (*s_l)[16])
 {
     constexpr int PITCH = pa_pitch(D), E = D / 16;
@@ -428,7 +437,7 @@ __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const int32_t 
     const int listed = e[5] ? p.b.max_prefix_pages : p.b.max_pages;
     Walk<DT, D> walk{p, (e[5] ? p.b.prefix_tbl : p.b.page_tbl) + (size_t)e[4] * listed, lds + wave * (PA_KEYS * D * 2), p.scale * PA_LOG2E,
                      listed, mine, min(mine + share, last), head, -1, -1};
-    walk.template all<NR>(st);
+    walk.template all<NR, STREAM>(st);
 #pragma unroll
     for (int n = 0; n < NR; n++) {
         float l = st[n].l;
@@ -477,10 +486,133 @@ __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const int32_t 
     }
 }
 
+// LDS chunk of K at which chunk ch of key row r lies: an operand read takes one chunk of sixteen rows.
+template <int D> __device__ __forceinline__ int pa_kswizzle(int r, int ch) { return D == 128 ? ch ^ (r & 15) : ch ^ ((r >> 1) & 7); }
+
+constexpr int PA_TILE = 64;                                // keys in LDS at a time
+
+// One wide item for one key head: 32 rows a wavefront, every key tile brought to LDS once for all of them, the next one on its way meanwhile.
+template <int DT, int D>
+__device__ __forceinline__ void pa_wide(const AttnKernelArgs &ka, const int32_t *e, const PlanView &pv, int head, unsigned char *lds)
+{
+    constexpr int NR = 2, KS = D / 32, CH = D / 8, PER = PA_TILE * CH / (64 * PA_WAVES), BYTES = PA_TILE * D * 2;
+    const AttnArgs &p = ka.a;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int rows = e[0], from = e[1], row0 = e[3], slot = e[8], last = e[7];
+    RowState<D> st[NR];
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        const int r = row0 + min(wave * 32 + n * 16 + c, rows - 1), idx = r / p.gq;
+        const uint16_t *q = p.q + pv.list[from + idx] * p.q_stride + ((size_t)head * p.gq + (r - idx * p.gq)) * D;
+#pragma unroll
+        for (int k = 0; k < KS; k++) st[n].q[k] = ldg16(q + k * 32 + g * 8);
+        st[n].m = -INFINITY;
+        st[n].l = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) st[n].acc[d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    const int listed = p.b.max_prefix_pages;
+    Walk<DT, D> walk{p, p.b.prefix_tbl + (size_t)e[4] * listed, nullptr, p.scale * PA_LOG2E, listed, e[6], last, head, -1, -1};
+    uint4 kr[PER], vr[PER];
+    auto load = [&](int key0) {                            // this thread's chunks: 64 / CH rows of a load in one half of sixteen
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int r0 = (i * PA_WAVES + wave) * (64 / CH), at = key0 + (r0 & ~15);
+            const int page = at < last ? walk.page_of(at >> p.page_shift) : -1;
+            const size_t row = (((size_t)max(page, 0) * p.n_kv_heads + head) << p.page_shift) + (at & ((1 << p.page_shift) - 1)) + (r0 & 15);
+            const unsigned mine = (lane / CH) * D + (lane % CH) * 8;
+            kr[i] = ldg16(p.k_pages + row * D + mine);
+            vr[i] = ldg16(p.v_pages + row * D + mine);
+        }
+    };
+    bool there[4];                                         // which sixteens of the tile at hand have a page
+    auto look = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) there[i] = key0 + 16 * i < last && walk.page_of((key0 + 16 * i) >> p.page_shift) >= 0;
+    };
+    auto store = [&](unsigned char *buf, int key0) {
+        const bool whole = there[0] && there[1] && there[2] && there[3] && key0 + PA_TILE <= last;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int r0 = (i * PA_WAVES + wave) * (64 / CH), r = r0 + lane / CH, ch = lane % CH;
+            if (!whole) {                                  // absent keys must not meet a weight of zero: they may be infinite
+                const bool here = r0 < 16 ? there[0] : r0 < 32 ? there[1] : r0 < 48 ? there[2] : there[3];
+                const uint32_t keep = here && key0 + r < last ? ~0u : 0u;
+                vr[i] = make_uint4(vr[i].x & keep, vr[i].y & keep, vr[i].z & keep, vr[i].w & keep);
+            }
+            stg16(buf + r * (D * 2) + pa_kswizzle<D>(r, ch) * 16, kr[i]);
+            stg16(buf + BYTES + r * (D * 2) + pa_swizzle<D>(r, ch) * 16, vr[i]);
+        }
+    };
+    int key0 = e[6];
+    load(key0);
+    look(key0);
+    store(lds, key0);
+    __syncthreads();
+#pragma unroll 1
+    for (int buf = 0; key0 < last; key0 += PA_TILE, buf ^= 1) {
+        const bool more = key0 + PA_TILE < last;
+        if (more) load(key0 + PA_TILE);
+        unsigned char *tile = lds + buf * 2 * BYTES;
+        if (wave * 32 < rows) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const int k0 = key0 + half * 32;
+                if (k0 >= last) break;
+                float4_t s[NR][2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint4 kf[KS];
+                    const int r = half * 32 + h * 16 + c;
+#pragma unroll
+                    for (int k = 0; k < KS; k++) kf[k] = *reinterpret_cast<const uint4 *>(tile + r * (D * 2) + pa_kswizzle<D>(r, k * 4 + g) * 16);
+#pragma unroll
+                    for (int n = 0; n < NR; n++) {
+                        s[n][h] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int k = 0; k < KS; k++) s[n][h] = pa_mfma<DT>(kf[k], st[n].q[k], s[n][h]);
+                        s[n][h] *= walk.scale2;
+                    }
+                }
+                if (!(there[2 * half] && there[2 * half + 1] && k0 + 32 <= last)) {
+#pragma unroll
+                    for (int n = 0; n < NR; n++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) s[n][h][i] = there[2 * half + h] && k0 + 16 * h + 4 * g + i < last ? s[n][h][i] : -INFINITY;
+                }
+                walk.vlds = tile + BYTES + half * 32 * (D * 2);
+                walk.template sums<NR>(st, s);
+            }
+        }
+        if (more) {
+            look(key0 + PA_TILE);
+            store(lds + (buf ^ 1) * 2 * BYTES, key0 + PA_TILE);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        float l = st[n].l;
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        const int r = wave * 32 + n * 16 + c;
+        if (r >= rows) continue;
+        const int row = row0 + r, idx = row / p.gq, sub = row - idx * p.gq;
+        if (slot < 0 || slot + idx >= ka.slots_cap) continue;      // a group's rows always have a slot
+        const size_t at = ((size_t)(slot + idx) * p.n_kv_heads + head) * p.gq + sub;
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) *reinterpret_cast<float4_t *>(ka.parts + at * D + d * 16 + g * 4) = st[n].acc[d];
+        if (g == 0) *reinterpret_cast<float2 *>(ka.parts + (size_t)ka.slots_cap * p.n_q_heads * D + at * 2) = make_float2(st[n].m, l);
+    }
+}
+
 template <int DT, int D>
 __global__ __launch_bounds__(64 * PA_WAVES, 2) void prefix_attention_kernel(const AttnKernelArgs ka)
 {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[PA_WAVES * 16 * pa_pitch(D) * 4];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * 2 * PA_TILE * D * 2];
+    static_assert(PA_WAVES * 16 * pa_pitch(D) * 4 <= 2 * 2 * PA_TILE * D * 2, "the wavefronts' V blocks, and the exchange of their sums, fit too");
     __shared__ float s_m[PA_WAVES][16], s_l[PA_WAVES][16];
     const AttnArgs &p = ka.a;
     const PlanView pv = pa_plan_view(ka.plan, p.b.T);
@@ -488,8 +620,10 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void prefix_attention_kernel(cons
     const unsigned item = blockIdx.x / (unsigned)p.n_kv_heads, head = blockIdx.x - item * (unsigned)p.n_kv_heads;
     if ((int)item >= min((long long)pv.n_items[0], ka.items_cap)) return;
     const int32_t *e = pv.items + (size_t)item * PA_ITEM;
-    if (e[0] <= 16) pa_item<DT, D, 1>(ka, e, pv, head, lds, s_m, s_l);
-    else pa_item<DT, D, 2>(ka, e, pv, head, lds, s_m, s_l);
+    if (e[0] > PA_ROWS) pa_wide<DT, D>(ka, e, pv, head, lds);
+    else if (e[0] > 16) pa_item<DT, D, 2, false>(ka, e, pv, head, lds, s_m, s_l);
+    else if (e[2]) pa_item<DT, D, 1, false>(ka, e, pv, head, lds, s_m, s_l);
+    else pa_item<DT, D, 1, true>(ka, e, pv, head, lds, s_m, s_l);
 }
 
 // ------------------------------------------------------------------ join

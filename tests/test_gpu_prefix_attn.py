@@ -288,3 +288,16 @@ def test_refusals():
         with pytest.raises(error):
             mlora.plan_attention(s.batch, s.cache, 4)
         setattr(s.batch, field, old)
+
+
+@pytest.mark.parametrize("dtype, D, P", [(F16, 128, 16), (BF16, 64, 16), (BF16, 128, 64), (F16, 64, 256)])
+@pytest.mark.parametrize("n_req, prefix", [(17, 63), (17, 64), (33, 65), (40, 129), (64, 1000), (65, 1)])
+def test_groups_of_many_rows(n_req, prefix, dtype, D, P):
+    """From 65 rows on the wavefronts of a workgroup share the rows: full and odd tiles of rows and of keys, absent pages among them."""
+    say(f"attention rows {4 * n_req} prefix {prefix} {dtype} D={D} P={P}")
+    rng = np.random.default_rng(n_req + prefix)
+    s = Scene([(0, int(rng.integers(1, 20))) for _ in range(n_req)], [prefix], 4, 1, D, P, dtype, seed=n_req + prefix)
+    if prefix > 2 * P:
+        s.prefix_lists[0][1] = -1
+        s.batch.prefix_pages[0, 1] = -1
+    run(s)
