@@ -36,6 +36,9 @@ constexpr int PA_ROWS = 32;                    // query rows of an item whose wa
 constexpr int PA_WIDE = 128;                   // of one whose wavefronts share the rows
 constexpr int PA_KEYS = 32;                    // keys of a block
 constexpr float PA_LOG2E = 1.44269504088896341f;
+// The sums of a row are kept relative to a maximum that follows the true one at a distance of up to 2^8: weights up to 256 keep the
+// 16-bit types' precision as well as weights up to 1, and most blocks then leave the sums as they are.
+constexpr float PA_SLACK = 8.f;
 
 // LDS chunk (16 bytes) at which chunk c of key row r of a wavefront's V block lies: the 16 rows a transposing read touches
 // at one column spread over all banks.
@@ -58,8 +61,9 @@ struct PlanView {
     int32_t *items;         // [cap][PA_ITEM]
 };
 
-// Key heads times items that fill the device: two workgroups for each place that a compute unit has for one.
-__host__ __device__ inline int pa_target(int n_kv_heads) { const int t = 1024 / n_kv_heads; return t < 1 ? 1 : t; }
+// Ranges of keys that fill the device: two workgroups a compute unit.  Twice as many cost more in parts than they level out (128 requests
+// over one prefix of 8191 keys: 82 us a layer against 90).
+__host__ __device__ inline int pa_target(int n_kv_heads) { const int t = 512 / n_kv_heads; return t < 1 ? 1 : t; }
 
 // With C keys a range where C >= (sum of own keys + sum over groups of keys x row tiles) / target, a list is cut into at most
 // keys / C + 1 ranges, which bounds the items and the slots by sizes the host knows.
@@ -165,12 +169,14 @@ __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
     const long long step = PA_WAVES * PA_KEYS;
     const long long C = max((((long long)s_work + p.target - 1) / p.target + step - 1) / step, 1LL) * step;
     auto range_of = [&](int keys, int cuts) { return ((keys + (long long)cuts - 1) / cuts + step - 1) / step * step; };
+    // a wide tile leaves as much behind as it reads in 130 keys: its ranges are 256 at least
+    auto group_cuts_of = [&](int f) { const int keys = prefix_keys(f); const long long c = rows_of(f) == PA_WIDE ? max(C, 256LL) : C; return (int)((keys + c - 1) / c); };
     auto cuts_of = [&](int keys) { return keys > 0 ? (int)((keys + C - 1) / C) : 0; };
     // groups: their lists, slots and items
     int n_list = 0, n_slot = 0, n_item = 0;
     for (int f0 = 0; f0 < F; f0 += PL_THREADS) {
         const int f = f0 + threadIdx.x;
-        const int members = f < F ? s_count[f] : 0, cuts = members ? cuts_of(prefix_keys(f)) : 0;
+        const int members = f < F ? s_count[f] : 0, cuts = members ? group_cuts_of(f) : 0;
         int a, b, c;
         const int la = n_list + pl_scan(members, s_scan, &a);
         const int sl = n_slot + pl_scan(members * cuts, s_scan, &b);
@@ -182,7 +188,7 @@ __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
     const int group_items = n_item;
     for (int i = threadIdx.x; i < group_items && i < p.items_cap; i += PL_THREADS) {
         const int f = pl_find(s_item, F, i);
-        const int keys = prefix_keys(f), cuts = cuts_of(keys), tiles = tiles_of(f), at = i - s_item[f];
+        const int keys = prefix_keys(f), cuts = group_cuts_of(f), tiles = tiles_of(f), at = i - s_item[f];
         const int cut = at / tiles, tile = at - cut * tiles;       // the tiles of a range lie side by side: they share its keys in L2
         const long long per = range_of(keys, cuts);
         int32_t *e = v.items + (size_t)i * PA_ITEM;
@@ -207,7 +213,7 @@ __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
             if (r.prefix >= 0) {
                 place = atomicAdd(&s_take[r.prefix], 1);
                 if (s_list[r.prefix] + place < T) v.list[s_list[r.prefix] + place] = t;
-                prefix_cuts = cuts_of(prefix_keys(r.prefix));
+                prefix_cuts = group_cuts_of(r.prefix);
             }
         }
         const int cuts = cuts_of(r.own), kept = cuts + prefix_cuts > 1 ? cuts : 0;
@@ -247,13 +253,13 @@ struct AttnKernelArgs {
 // K and V of one block of 32 keys, on their way.
 template <int D> struct KeyBlock {
     uint4 k[2][D / 32], v[D / 16];
-    bool there[2];
+    int have;                  // bit h: the h-th sixteen of keys has a page
 };
 
 // What a wavefront holds of 16 query rows.
 template <int D> struct RowState {
     uint4 q[D / 32];
-    float m, l;                // of row lane % 16: the maximum, in powers of two, over all lanes; the sum of this lane's keys
+    float m, l;                // of row lane % 16: what its weights are relative to, in powers of two, for all lanes; the sum of this lane's keys
     float4_t acc[D / 16];      // out^T: columns 16 i + 4 g .. + 3 of row lane % 16
 };
 
@@ -268,15 +274,31 @@ struct Walk {
     int n_listed, first, last, head;
     int window, ids;                   // 64 pages from page `window` on; -1: none yet
 
-    __device__ __forceinline__ int page_of(int nth)
+    // Pages of the sixteens of keys from key0 on, -1 for those that are absent; bit i of the result: the i-th has one.
+    template <int N>
+    __device__ __forceinline__ int find(int key0, int (&page)[N])
     {
-        if (window < 0 || nth < window || nth >= window + 64) {
-            window = nth;
-            const int at = nth + (threadIdx.x & 63);
+        const int from = key0 >> p.page_shift, to = (key0 + 16 * (N - 1)) >> p.page_shift;
+        if (window < 0 || from < window || to >= window + 64) {
+            window = from;
+            const int at = from + (threadIdx.x & 63);
             ids = at < n_listed ? pages[at] : -1;
+            ids = ids < p.n_pages ? ids : -1;
+            // waited for here: behind the branch every look at the ids would wait for whatever was loaded last
+            asm volatile("" : "+v"(ids));
         }
-        const int page = __builtin_amdgcn_readlane(ids, nth - window);
-        return page < p.n_pages ? page : -1;
+        int have = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            page[i] = __builtin_amdgcn_readlane(ids, ((key0 + 16 * i) >> p.page_shift) - window);
+            have |= key0 + 16 * i < last && page[i] >= 0 ? 1 << i : 0;
+        }
+        return have;
+    }
+
+    __device__ __forceinline__ size_t row_of(int page, int key) const      // of a slab of [rows, D]
+    {
+        return (((size_t)page * p.n_kv_heads + head) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
     }
 
     // Issue the loads of the block at key0 (keys past the last are loaded from page 0 and masked).  STREAM: keys that nobody else reads.
@@ -287,12 +309,11 @@ struct Walk {
         // what differs between lanes is one 32-bit offset for K and one for V: the rest of an address is the same for the wavefront
         const int lane = threadIdx.x & 63;
         const unsigned klane = (lane & 15) * D + (lane >> 4) * 8, vlane = (lane / CH) * D + (lane % CH) * 8;
+        int page[2];
+        b.have = find<2>(key0, page);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int at = key0 + 16 * h;
-            const int page = at < last ? page_of(at >> p.page_shift) : -1;
-            b.there[h] = page >= 0;
-            const size_t row0 = (((size_t)(page >= 0 ? page : 0) * p.n_kv_heads + head) << p.page_shift) + (at & ((1 << p.page_shift) - 1));
+            const size_t row0 = row_of(b.have >> h & 1 ? page[h] : 0, key0 + 16 * h);
             const uint16_t *k = p.k_pages + row0 * D, *v = p.v_pages + row0 * D;
 #pragma unroll
             for (int s = 0; s < KS; s++) b.k[h][s] = get(k + klane + s * 32);
@@ -306,12 +327,12 @@ struct Walk {
     __device__ __forceinline__ void scores(KeyBlock<D> &b, int key0, const RowState<D> (&st)[NR], float4_t (&s)[NR][2])
     {
         const int lane = threadIdx.x & 63, g = lane >> 4;
-        const bool whole = b.there[0] && b.there[1] && key0 + PA_KEYS <= last;
+        const bool whole = b.have == 3 && key0 + PA_KEYS <= last;
         if (!whole) {
             // what lies behind the last key, or on no page at all, must not meet a weight of zero: it may be infinite
 #pragma unroll
             for (int u = 0; u < VL; u++) {
-                const uint32_t keep = key0 + u * (64 / CH) + lane / CH < last && b.there[u >= VL / 2] ? ~0u : 0u;
+                const uint32_t keep = key0 + u * (64 / CH) + lane / CH < last && (b.have >> (u >= VL / 2) & 1) ? ~0u : 0u;
                 b.v[u] = make_uint4(b.v[u].x & keep, b.v[u].y & keep, b.v[u].z & keep, b.v[u].w & keep);
             }
         }
@@ -327,10 +348,9 @@ struct Walk {
                 s[n][h] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < KS; k++) s[n][h] = pa_mfma<DT>(b.k[h][k], st[n].q[k], s[n][h]);
-                s[n][h] *= scale2;
                 if (!whole) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) s[n][h][i] = b.there[h] && key0 + 16 * h + 4 * g + i < last ? s[n][h][i] : -INFINITY;
+                    for (int i = 0; i < 4; i++) s[n][h][i] = (b.have >> h & 1) && key0 + 16 * h + 4 * g + i < last ? s[n][h][i] : -INFINITY;
                 }
             }
     }
@@ -346,19 +366,20 @@ struct Walk {
             float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])), fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float m = fmaxf(st[n].m, top), ref = m == -INFINITY ? 0.f : m;
-            if (__ballot(m > st[n].m)) {           // a higher maximum in some row: what was summed so far shrinks
-                const float keep = __builtin_amdgcn_exp2f(st[n].m - ref);
+            top *= scale2;
+            if (__ballot(top > st[n].m + PA_SLACK)) {      // a maximum has grown too far in some row: what was summed so far shrinks
+                const float m = fmaxf(st[n].m, top), keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[n].m - m);
                 st[n].l *= keep;
 #pragma unroll
                 for (int d = 0; d < DTILES; d++) st[n].acc[d] *= keep;
                 st[n].m = m;
             }
+            const float ref = st[n].m == -INFINITY ? 0.f : st[n].m;
             float w[8];
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) { w[4 * h + i] = __builtin_amdgcn_exp2f(s[n][h][i] - ref); st[n].l += w[4 * h + i]; }
+                for (int i = 0; i < 4; i++) { w[4 * h + i] = __builtin_amdgcn_exp2f(fmaf(s[n][h][i], scale2, -ref)); st[n].l += w[4 * h + i]; }
             wf[n] = pack8<DT>(w);
         }
         __builtin_amdgcn_wave_barrier();
@@ -411,6 +432,16 @@ struct Walk {
 
 constexpr int pa_pitch(int D) { return D + 4; }            // floats of a row in the LDS exchange: a float4 of 16 rows meets all banks
 
+// Scale and q as the walk takes them: the scale in powers of two, positive (a maximum of scores is one of scaled scores then, and a masked
+// score stays minus infinity), its sign in q.
+__device__ __forceinline__ float pa_scale2(float scale) { return fmaxf(fabsf(scale) * PA_LOG2E, 1e-30f); }
+__device__ __forceinline__ uint4 pa_load_q(const uint16_t *q, float scale)
+{
+    const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
+    const uint4 v = ldg16(q);
+    return make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+}
+
 // One item for one key head: NR tiles of 16 query rows, the keys shared by the four wavefronts and joined in LDS.
 template <int DT, int D, int NR, bool STREAM>
 __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const int32_t *e, const PlanView &pv, int head, unsigned char *lds, float (*s_m)[16], float (*s_l)[16])
@@ -426,7 +457,7 @@ __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const int32_t 
         const int r = row0 + min(n * 16 + c, rows - 1), idx = r / p.gq;
         const uint16_t *q = p.q + token_of(idx) * p.q_stride + ((size_t)head * p.gq + (r - idx * p.gq)) * D;
 #pragma unroll
-        for (int k = 0; k < D / 32; k++) st[n].q[k] = ldg16(q + k * 32 + g * 8);
+        for (int k = 0; k < D / 32; k++) st[n].q[k] = pa_load_q(q + k * 32 + g * 8, p.scale);
         st[n].m = -INFINITY;
         st[n].l = 0.f;
 #pragma unroll
@@ -435,7 +466,7 @@ __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const int32_t 
     const int first = e[6], last = e[7], share = (last - first + PA_WAVES * PA_KEYS - 1) / (PA_WAVES * PA_KEYS) * PA_KEYS;
     const int mine = first + wave * share;
     const int listed = e[5] ? p.b.max_prefix_pages : p.b.max_pages;
-    Walk<DT, D> walk{p, (e[5] ? p.b.prefix_tbl : p.b.page_tbl) + (size_t)e[4] * listed, lds + wave * (PA_KEYS * D * 2), p.scale * PA_LOG2E,
+    Walk<DT, D> walk{p, (e[5] ? p.b.prefix_tbl : p.b.page_tbl) + (size_t)e[4] * listed, lds + wave * (PA_KEYS * D * 2), pa_scale2(p.scale),
                      listed, mine, min(mine + share, last), head, -1, -1};
     walk.template all<NR, STREAM>(st);
 #pragma unroll
@@ -505,39 +536,37 @@ __device__ __forceinline__ void pa_wide(const AttnKernelArgs &ka, const int32_t 
         const int r = row0 + min(wave * 32 + n * 16 + c, rows - 1), idx = r / p.gq;
         const uint16_t *q = p.q + pv.list[from + idx] * p.q_stride + ((size_t)head * p.gq + (r - idx * p.gq)) * D;
 #pragma unroll
-        for (int k = 0; k < KS; k++) st[n].q[k] = ldg16(q + k * 32 + g * 8);
+        for (int k = 0; k < KS; k++) st[n].q[k] = pa_load_q(q + k * 32 + g * 8, p.scale);
         st[n].m = -INFINITY;
         st[n].l = 0.f;
 #pragma unroll
         for (int d = 0; d < D / 16; d++) st[n].acc[d] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
     const int listed = p.b.max_prefix_pages;
-    Walk<DT, D> walk{p, p.b.prefix_tbl + (size_t)e[4] * listed, nullptr, p.scale * PA_LOG2E, listed, e[6], last, head, -1, -1};
+    Walk<DT, D> walk{p, p.b.prefix_tbl + (size_t)e[4] * listed, nullptr, pa_scale2(p.scale), listed, e[6], last, head, -1, -1};
     uint4 kr[PER], vr[PER];
-    auto load = [&](int key0) {                            // this thread's chunks: 64 / CH rows of a load in one half of sixteen
+    const unsigned mine = (lane / CH) * D + (lane % CH) * 8;
+    int have, have_next;                                   // sixteens of the tile at hand, and of the one on its way, that have a page
+    auto load = [&](int key0) {                            // this thread's chunks: 64 / CH rows of a load, all in one sixteen
+        int page[4];
+        have_next = walk.template find<4>(key0, page);
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            const int r0 = (i * PA_WAVES + wave) * (64 / CH), at = key0 + (r0 & ~15);
-            const int page = at < last ? walk.page_of(at >> p.page_shift) : -1;
-            const size_t row = (((size_t)max(page, 0) * p.n_kv_heads + head) << p.page_shift) + (at & ((1 << p.page_shift) - 1)) + (r0 & 15);
-            const unsigned mine = (lane / CH) * D + (lane % CH) * 8;
+            const int r0 = (i * PA_WAVES + wave) * (64 / CH), six = r0 / 16;
+            const int pg = six == 0 ? page[0] : six == 1 ? page[1] : six == 2 ? page[2] : page[3];
+            const size_t row = walk.row_of(have_next >> six & 1 ? pg : 0, key0 + six * 16) + (r0 & 15);
             kr[i] = ldg16(p.k_pages + row * D + mine);
             vr[i] = ldg16(p.v_pages + row * D + mine);
         }
     };
-    bool there[4];                                         // which sixteens of the tile at hand have a page
-    auto look = [&](int key0) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) there[i] = key0 + 16 * i < last && walk.page_of((key0 + 16 * i) >> p.page_shift) >= 0;
-    };
     auto store = [&](unsigned char *buf, int key0) {
-        const bool whole = there[0] && there[1] && there[2] && there[3] && key0 + PA_TILE <= last;
+        have = have_next;
+        const bool whole = have == 15 && key0 + PA_TILE <= last;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int r0 = (i * PA_WAVES + wave) * (64 / CH), r = r0 + lane / CH, ch = lane % CH;
             if (!whole) {                                  // absent keys must not meet a weight of zero: they may be infinite
-                const bool here = r0 < 16 ? there[0] : r0 < 32 ? there[1] : r0 < 48 ? there[2] : there[3];
-                const uint32_t keep = here && key0 + r < last ? ~0u : 0u;
+                const uint32_t keep = (have >> (r0 / 16) & 1) && key0 + r < last ? ~0u : 0u;
                 vr[i] = make_uint4(vr[i].x & keep, vr[i].y & keep, vr[i].z & keep, vr[i].w & keep);
             }
             stg16(buf + r * (D * 2) + pa_kswizzle<D>(r, ch) * 16, kr[i]);
@@ -546,7 +575,6 @@ __device__ __forceinline__ void pa_wide(const AttnKernelArgs &ka, const int32_t 
     };
     int key0 = e[6];
     load(key0);
-    look(key0);
     store(lds, key0);
     __syncthreads();
 #pragma unroll 1
@@ -571,25 +599,21 @@ __device__ __forceinline__ void pa_wide(const AttnKernelArgs &ka, const int32_t 
                         s[n][h] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int k = 0; k < KS; k++) s[n][h] = pa_mfma<DT>(kf[k], st[n].q[k], s[n][h]);
-                        s[n][h] *= walk.scale2;
                     }
                 }
-                if (!(there[2 * half] && there[2 * half + 1] && k0 + 32 <= last)) {
+                if ((have >> 2 * half & 3) != 3 || k0 + 32 > last) {
 #pragma unroll
                     for (int n = 0; n < NR; n++)
 #pragma unroll
                         for (int h = 0; h < 2; h++)
 #pragma unroll
-                            for (int i = 0; i < 4; i++) s[n][h][i] = there[2 * half + h] && k0 + 16 * h + 4 * g + i < last ? s[n][h][i] : -INFINITY;
+                            for (int i = 0; i < 4; i++) s[n][h][i] = (have >> (2 * half + h) & 1) && k0 + 16 * h + 4 * g + i < last ? s[n][h][i] : -INFINITY;
                 }
                 walk.vlds = tile + BYTES + half * 32 * (D * 2);
                 walk.template sums<NR>(st, s);
             }
         }
-        if (more) {
-            look(key0 + PA_TILE);
-            store(lds + (buf ^ 1) * 2 * BYTES, key0 + PA_TILE);
-        }
+        if (more) store(lds + (buf ^ 1) * 2 * BYTES, key0 + PA_TILE);
         __syncthreads();
     }
 #pragma unroll
