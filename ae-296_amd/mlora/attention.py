@@ -119,14 +119,15 @@ class AttnPlan:
     buf: torch.Tensor
 
 
-def plan_attention(batch: KVBatch, cache: KVCache, n_q_heads: int, out: Optional[AttnPlan] = None) -> AttnPlan:
+def plan_attention(batch: KVBatch, cache: KVCache, n_q_heads: int, out: Optional[AttnPlan] = None, room: int = 0) -> AttnPlan:
     """Divide the step's attention work once; the plan serves every layer's ``prefix_attention``.  Pass `out` to reuse a plan's
-    buffer (no allocation; safe under graph capture; a batch larger than the one it was made for is refused)."""
+    buffer (no allocation; safe under graph capture; a batch larger than the one it was made for is refused); `room`: prefixes that
+    a new buffer is sized for where that is more than the batch has."""
     if n_q_heads < 1 or n_q_heads % cache.n_kv_heads:
         raise ValueError(f"n_q_heads must be a multiple of the cache's {cache.n_kv_heads} key heads")
     n_prefix = 0 if batch.prefix_len is None else batch.prefix_len.numel()
     if out is None:
-        need = _ext.lib().mlora_attn_plan_bytes(batch.T, n_prefix, n_q_heads, cache.n_kv_heads)
+        need = _ext.lib().mlora_attn_plan_bytes(batch.T, max(n_prefix, room), n_q_heads, cache.n_kv_heads)
         if need < 0:
             _ext.check(need)
         buf = torch.empty(need, dtype=torch.uint8, device=batch.tok_req.device)

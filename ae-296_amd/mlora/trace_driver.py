@@ -17,7 +17,8 @@ What is mirrored from the reference:
 
 What is synthetic: output lengths (the reference takes them from a dataset that is not part of it,
 ``client_maf.py:33-34,50``) are drawn from a seeded geometric distribution; the virtual duration of a scheduler
-step is a parameter.
+step is a parameter.  With a ``TraceContext`` the runner also keeps keys and values: every adapter has a task prompt of a fixed
+length (synthetic keys and values) that all its requests share, and every request the tokens it has decoded since.
 """
 from __future__ import annotations
 
@@ -59,6 +60,7 @@ class TraceStep:
     lora_ids: np.ndarray
     admitted: List[int] = field(default_factory=list)       # request numbers admitted in this step
     finished: int = 0
+    requests: Optional[np.ndarray] = None                   # request number of every running request, as lora_ids
 
 
 def simulate(event_times: Sequence[float], lora_ids: Sequence[int], out_lens: Sequence[int], step_s: float = 0.03,
@@ -86,9 +88,10 @@ def simulate(event_times: Sequence[float], lora_ids: Sequence[int], out_lens: Se
             done = [rq for rq in admitted if running[rq] <= 0]
             for rq in done:
                 del running[rq]
-            steps.append(TraceStep(len(steps), t, "prefill", np.array([lora_ids[rq] for rq in running], np.int32), admitted, len(done)))
+            steps.append(TraceStep(len(steps), t, "prefill", np.array([lora_ids[rq] for rq in running], np.int32), admitted, len(done),
+                                   np.array(list(running), np.int32)))
         else:
-            ids = np.array([lora_ids[rq] for rq in running], np.int32)
+            ids, numbers = np.array([lora_ids[rq] for rq in running], np.int32), np.array(list(running), np.int32)
             done = []
             for rq in running:
                 running[rq] -= 1
@@ -96,7 +99,7 @@ def simulate(event_times: Sequence[float], lora_ids: Sequence[int], out_lens: Se
                     done.append(rq)
             for rq in done:
                 del running[rq]
-            steps.append(TraceStep(len(steps), t, "decode", ids, [], len(done)))
+            steps.append(TraceStep(len(steps), t, "decode", ids, [], len(done), numbers))
         t += step_s
     return steps
 
@@ -140,14 +143,62 @@ class AdapterResidency:
         return np.array([self.slot_of[int(a)] for a in lora_ids], np.int32)
 
 
+class TraceContext:
+    """Keys and values of a trace's running requests: pages of a cache, one prompt of `prompt` tokens per adapter (written on its
+    first use and kept), and per request the pages of the tokens decoded so far, given back when it no longer runs."""
+
+    def __init__(self, cache, prompt: int, seed: int = 0):
+        self.cache, self.prompt, self.seed = cache, prompt, seed
+        self.prompts: "OrderedDict[int, List[int]]" = OrderedDict()        # adapter -> pages; its place is its prefix id
+        self.pages: Dict[int, List[int]] = {}                              # request -> pages
+        self.length: Dict[int, int] = {}                                   # request -> tokens of its own
+
+    def _prompt_of(self, adapter: int) -> int:
+        import torch
+        if adapter not in self.prompts:
+            c = self.cache
+            pages = c.allocate(-(-self.prompt // c.page_tokens))
+            g = torch.Generator().manual_seed(self.seed * 1000003 + adapter)
+            for p in pages:
+                for t in (c.k, c.v):
+                    t[:, p].copy_(torch.randn(t[:, p].shape, generator=g))
+            self.prompts[adapter] = pages
+        return list(self.prompts).index(adapter)
+
+    def advance(self, requests: Sequence[int], lora_ids: Sequence[int]) -> dict:
+        """One more token for every request listed; those no longer listed give their pages back.  The batch as host lists."""
+        P = self.cache.page_tokens
+        gone = set(self.pages) - {int(r) for r in requests}
+        for r in gone:
+            self.cache.release(self.pages.pop(r))
+            del self.length[r]
+        prompt_pages = -(-self.prompt // P)
+        need = prompt_pages * len({int(a) for a in lora_ids} - set(self.prompts)) + sum(self.length.get(int(r), 0) % P == 0 for r in requests)
+        if need > self.cache.free_pages:              # before anything changes
+            raise MemoryError(f"the step needs {need} more pages of keys, {self.cache.free_pages} are free")
+        of = [self._prompt_of(int(a)) for a in lora_ids]
+        for r in map(int, requests):
+            mine = self.pages.setdefault(r, [])
+            self.length[r] = self.length.get(r, 0) + 1
+            if self.length[r] > len(mine) * P:
+                mine.extend(self.cache.allocate(1))
+        lists = [self.pages[int(r)] for r in requests]
+        width = max(map(len, lists))
+        return dict(tok_req=list(range(len(lists))), tok_pos=[self.prompt + self.length[int(r)] - 1 for r in requests],
+                    pages=[p + [-1] * (width - len(p)) for p in lists], req_prefix=of,
+                    prefix_pages=list(self.prompts.values()), prefix_len=[self.prompt] * len(self.prompts))
+
+
 class TraceRunner:
     """Runs the decode steps of a simulated trace on the GPU: adapters are staged in pinned host memory on first
     use (weights drawn from a generator seeded by the adapter id), swapped into a paged pool of `n_slots` slots
     through ``AdapterLoader`` when a step needs them, and every decode step is one gather plus one BGMV call per
-    layer over q, k, v (the projections the reference applies LoRA to)."""
+    layer over q, k, v (the projections the reference applies LoRA to).  With a `head_dim` it also keeps keys and values of the
+    requests ``decode_step`` names (`n_cache_pages` pages of 16 tokens, prompts of `prompt` tokens) and runs each layer's append
+    and attention behind its projections."""
 
     def __init__(self, n_layers: int, hidden: int, rank: int, n_slots: int, device="cuda", dtype=None, seed: int = 0,
-                 scaling: float = 2.0, max_batch: int = 256):
+                 scaling: float = 2.0, max_batch: int = 256, head_dim: int = 0, prompt: int = 0, n_cache_pages: int = 0):
         import torch
 
         from . import AdapterLoader, AdapterPool
@@ -173,6 +224,15 @@ class TraceRunner:
                        torch.empty(max_batch, dtype=torch.int32, device=self.device), torch.cuda.Event()) for _ in range(8)]
         self._ring_at = 0
         self._plans: Dict[int, object] = {}
+        self.context = self.step = None
+        if head_dim:
+            from . import KVCache, RopeTable, TokenStep
+            if prompt < 1:
+                raise ValueError("prompt must be positive")
+            self.context = TraceContext(KVCache(n_layers, n_cache_pages, hidden // head_dim, head_dim, dtype=self.dtype, device=self.device), prompt, seed)
+            self.step = TokenStep(self.pool, self.context.cache, None, hidden // head_dim,
+                                  RopeTable(prompt + 16 * n_cache_pages, head_dim, device=self.device))
+        self.attended: List[object] = []
         self.tickets: List[object] = []
 
     def adapter_weights(self, adapter: int):
@@ -195,8 +255,10 @@ class TraceRunner:
             self.tickets.clear()
         return len(todo)
 
-    def decode_step(self, lora_ids: np.ndarray, accumulate: bool = True):
-        """One decode step for a batch whose requests use `lora_ids`; returns (tok_adapter slots, y tensors)."""
+    def decode_step(self, lora_ids: np.ndarray, accumulate: bool = True, requests: Optional[Sequence[int]] = None):
+        """One decode step for a batch whose requests use `lora_ids`; returns (tok_adapter slots, y tensors).  With `requests`, their
+        numbers, a runner that keeps keys and values appends one token to each and attends: q, k and v are the adapters' deltas
+        alone then, and `attended` holds the layers' outputs."""
         from . import ops
         torch = self.torch
         T = len(lora_ids)
@@ -212,6 +274,15 @@ class TraceRunner:
         host[:T].copy_(torch.from_numpy(slots))
         tok = devbuf[:T]
         tok.copy_(host[:T], non_blocking=True)
+        if requests is not None:
+            if self.context is None:
+                raise ValueError("a runner without head_dim keeps no keys and values")
+            from . import KVBatch
+            held = {k: torch.tensor(v, dtype=torch.int32, device=self.device) for k, v in self.context.advance(requests, lora_ids).items()}
+            self.step.begin(KVBatch(**held), tok)
+            self.attended = [self.step.layer(l, self.x[l][:T]).clone() for l in range(self.n_layers)]
+            ev.record()
+            return slots, self.y
         plan = self._plans.get(T)
         plan = ops.plan_decode(tok, self.pool, out=plan) if plan is not None else ops.plan_decode(tok, self.pool)
         self._plans[T] = plan

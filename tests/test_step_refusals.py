@@ -202,3 +202,43 @@ def test_host_tensors_are_refused():
         mlora.w4_gemv([y], [y], [object()])
     with pytest.raises(ValueError, match="1..8"):
         mlora.w4_gemv([], [], [])
+
+
+# ---------------------------------------------------------------- the step, and the trace's bookkeeping
+def test_token_step_arguments():
+    pool = mlora.AdapterPool(2, {"q": (64, 256), "k": (64, 128), "v": (64, 128)}, 2, 4, max_rank=16, device="cpu")
+    c = cache()
+    mlora.TokenStep(pool, c, None, 4)
+    with pytest.raises(ValueError, match="q must be"):
+        mlora.TokenStep(pool, c, None, 2)
+    with pytest.raises(ValueError, match="names"):
+        mlora.TokenStep(pool, c, None, 4, names=("q", "k"))
+    with pytest.raises(ValueError, match="one dtype"):
+        mlora.TokenStep(pool, cache(dtype=torch.bfloat16), None, 4)
+    with pytest.raises(ValueError, match="one dtype"):
+        mlora.TokenStep(pool, cache(n_layers=1), None, 4)
+    with pytest.raises(ValueError, match="every layer"):
+        mlora.TokenStep(pool, c, [{}], 4)
+    step = mlora.TokenStep(pool, c, None, 4)
+    with pytest.raises(RuntimeError, match="begin"):
+        step.layer(0, torch.zeros((1, 64), dtype=torch.float16))
+    with pytest.raises(ValueError, match="every token"):
+        step.begin(mlora.KVBatch(torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros((2, 1), dtype=torch.int32)),
+                   torch.zeros(3, dtype=torch.int32))
+
+
+def test_trace_context_pages():
+    from mlora.trace_driver import TraceContext, simulate
+    c = TraceContext(mlora.KVCache(1, 12, 1, 64, device="cpu"), 17)
+    b = c.advance([5, 9], [2, 2])
+    assert b["req_prefix"] == [0, 0] and b["prefix_len"] == [17] and b["tok_pos"] == [17, 17] and len(c.prompts[2]) == 2
+    for _ in range(16):
+        b = c.advance([5, 9], [2, 2])
+    assert b["tok_pos"] == [33, 33] and len(b["pages"][0]) == 2 and c.cache.free_pages == 12 - 2 - 4
+    b = c.advance([9, 7], [2, 4])                     # 5 is gone, 7 came with another adapter
+    assert b["req_prefix"] == [0, 1] and b["tok_pos"] == [34, 17] and b["pages"][1][1] == -1 and c.cache.free_pages == 12 - 4 - 2 - 1
+    with pytest.raises(MemoryError):
+        c.advance(range(20, 40), [2] * 20)
+    steps = simulate([0.0, 0.0, 0.1], [1, 2, 3], [4, 2, 3])
+    for s in steps:
+        assert len(s.requests) == len(s.lora_ids) and [[1, 2, 3][r] for r in s.requests] == s.lora_ids.tolist()
