@@ -59,7 +59,8 @@ def rope_exact(x, pos, rot, interleaved, base=10000.0):
 def attention_exact(q, keys, values, scale, dtype):
     """One query row over its visible keys (64-bit arrays): (result, bound).  The bound counts: the fp32 sum of a score's D products and its
     scaling (they move an exponent), the exponential (2 steps), the rounding of a weight to 16 bits (HALF of it, or half of the
-    smallest step), the fp32 sums over n keys in numerator and denominator, and the joining of parts."""
+    smallest step) in both sums - sum r(p) v / sum r(p) is off by (sum |r(p) - p| |v| + |out| sum |r(p) - p|) / sum r(p), where |out| is at
+    most sum p |v| / sum p -, the fp32 sums over n keys in numerator and denominator, and the joining of parts."""
     D = q.shape[0]
     n = keys.shape[0]
     if n == 0:
@@ -69,9 +70,9 @@ def attention_exact(q, keys, values, scale, dtype):
     l = p.sum()
     out = p @ values / l
     exponent = ((D + 2) * U32 * np.abs(keys) @ np.abs(q) * abs(scale)).max() + 6 * U32 * np.abs(s).max()
-    rel = 2 * np.expm1(exponent) + 2 * 2.0 ** -22 + HALF[dtype] + 2 * (n + 80) * U32
+    rel = 2 * np.expm1(exponent) + 2 * 2.0 ** -22 + 2 * HALF[dtype] / (1 - HALF[dtype]) + 2 * (n + 80) * U32
     spread = p @ np.abs(values) / l
-    return out, rel * spread + n * TINY[dtype] * np.abs(values).max(0) / l + HALF[dtype] * np.abs(out) + TINY[dtype]
+    return out, rel * spread + 2 * n * TINY[dtype] * np.abs(values).max(0) / l + HALF[dtype] * np.abs(out) + TINY[dtype]
 
 
 def check(got, want, bound, what=""):
