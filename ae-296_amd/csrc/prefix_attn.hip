@@ -36,9 +36,6 @@ constexpr int PA_ROWS = 32;                    // query rows of an item whose wa
 constexpr int PA_WIDE = 128;                   // of one whose wavefronts share the rows
 constexpr int PA_KEYS = 32;                    // keys of a block
 constexpr float PA_LOG2E = 1.44269504088896341f;
-// The sums of a row are kept relative to a maximum that follows the true one at a distance of up to 2^8: weights up to 256 keep the
-// 16-bit types' precision as well as weights up to 1, and most blocks then leave the sums as they are.
-constexpr float PA_SLACK = 8.f;
 
 // LDS chunk (16 bytes) at which chunk c of key row r of a wavefront's V block lies: the 16 rows a transposing read touches
 // at one column spread over all banks.
@@ -259,7 +256,7 @@ template <int D> struct KeyBlock {
 // What a wavefront holds of 16 query rows.
 template <int D> struct RowState {
     uint4 q[D / 32];
-    float m, l;                // of row lane % 16: what its weights are relative to, in powers of two, for all lanes; the sum of this lane's keys
+    float m, l;                // of row lane % 16: the maximum, in powers of two, over all lanes; the sum of this lane's keys
     float4_t acc[D / 16];      // out^T: columns 16 i + 4 g .. + 3 of row lane % 16
 };
 
@@ -367,7 +364,10 @@ struct Walk {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             top *= scale2;
-            if (__ballot(top > st[n].m + PA_SLACK)) {      // a maximum has grown too far in some row: what was summed so far shrinks
+            // A higher maximum in some row: what was summed so far shrinks.  Letting the sums stand until a maximum has grown by 2^8 takes 3 to
+            // 5 % off the prefix items and nothing off the others, and costs the exact weight of 1 of a row's largest key (0.0022 of the
+            // result's norm off the 64-bit result in bf16 instead of 0.0019).
+            if (__ballot(top > st[n].m)) {
                 const float m = fmaxf(st[n].m, top), keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[n].m - m);
                 st[n].l *= keep;
 #pragma unroll
@@ -381,8 +381,7 @@ struct Walk {
 #pragma unroll
                 for (int i = 0; i < 4; i++) w[4 * h + i] = __builtin_amdgcn_exp2f(fmaf(s[n][h][i], scale2, -ref));
             wf[n] = pack8<DT>(w);
-            // the sum takes the weights as rounded: a rounding that is in both sums moves their quotient less (128 requests over one prefix in
-            // bf16: 0.0022 of the result's norm off the 64-bit result with the sum of the unrounded ones)
+            // the sum takes the weights as rounded: a rounding that is in both sums moves their quotient less, and four instructions do it
             const uint32_t one = DT == DT_F16 ? 0x3c003c00u : 0x3f803f80u;
             st[n].l = dot8<DT>(wf[n], make_uint4(one, one, one, one), st[n].l);
         }
