@@ -447,7 +447,7 @@ __device__ __forceinline__ uint4 pa_load_q(const uint16_t *q, float scale)
 
 // One item for one key head: NR tiles of 16 query rows, the keys shared by the four wavefronts and joined in LDS.
 template <int DT, int D, int NR, bool STREAM>
-__device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const int32_t *e, const PlanView &pv, int head, unsigned char *lds, float (*s_m)[16], float (*s_l)[16])
+__device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const_i32_ptr e, const PlanView &pv, int head, unsigned char *lds, float (*s_m)[16], float (*s_l)[16])
 {
     constexpr int PITCH = pa_pitch(D), E = D / 16;
     const AttnArgs &p = ka.a;
@@ -527,7 +527,7 @@ constexpr int PA_TILE = 64;                                // keys in LDS at a t
 
 // One wide item for one key head: 32 rows a wavefront, every key tile brought to LDS once for all of them, the next one on its way meanwhile.
 template <int DT, int D>
-__device__ __forceinline__ void pa_wide(const AttnKernelArgs &ka, const int32_t *e, const PlanView &pv, int head, unsigned char *lds)
+__device__ __forceinline__ void pa_wide(const AttnKernelArgs &ka, const_i32_ptr e, const PlanView &pv, int head, unsigned char *lds)
 {
     constexpr int NR = 2, KS = D / 32, CH = D / 8, PER = PA_TILE * CH / (64 * PA_WAVES), BYTES = PA_TILE * D * 2;
     const AttnArgs &p = ka.a;
@@ -645,8 +645,9 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void prefix_attention_kernel(cons
     const PlanView pv = pa_plan_view(ka.plan, p.b.T);
     // key heads fastest: with a multiple of eight of them a head stays on one XCD, and with it what the row tiles of a prefix share
     const unsigned item = blockIdx.x / (unsigned)p.n_kv_heads, head = blockIdx.x - item * (unsigned)p.n_kv_heads;
-    if ((int)item >= min((long long)pv.n_items[0], ka.items_cap)) return;
-    const int32_t *e = pv.items + (size_t)item * PA_ITEM;
+    if ((int)item >= min((long long)as_const(pv.n_items)[0], ka.items_cap)) return;
+    // the plan is read as constant memory: what an item says is the same for the workgroup, and belongs in scalar registers
+    const const_i32_ptr e = as_const(pv.items + (size_t)item * PA_ITEM);
     if (e[0] > PA_ROWS) pa_wide<DT, D>(ka, e, pv, head, lds);
     else if (e[0] > 16) pa_item<DT, D, 2, false>(ka, e, pv, head, lds, s_m, s_l);
     else if (e[2]) pa_item<DT, D, 1, false>(ka, e, pv, head, lds, s_m, s_l);
@@ -664,7 +665,7 @@ __global__ __launch_bounds__(256) void pa_join_kernel(const AttnKernelArgs ka)
     const int t = blockIdx.x;
     if (p.b.tok_req[t] < 0) return;
     const PlanView pv = pa_plan_view(ka.plan, p.b.T);
-    const int32_t *j = pv.join + (size_t)t * PA_JOIN;
+    const const_i32_ptr j = as_const(pv.join + (size_t)t * PA_JOIN);
     const int own = j[1], shared = j[3];
     if (own == 1 && shared == 0) return;                         // written by its only item
     const int slice = threadIdx.x >> 4, col = (threadIdx.x & 15) * E, part0 = slice % G;
