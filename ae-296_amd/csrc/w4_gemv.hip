@@ -62,17 +62,27 @@ __device__ __forceinline__ float4_t mfma16(const uint4 &a, const uint4 &b, float
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf168_t, a), __builtin_bit_cast(bf168_t, b), c, 0, 0, 0);
 }
 
-// eight codes of a dword as 16 + c
+// Eight codes of a dword as 16 + c.  fp16: 16.0 is 0x4c00 with a unit of the last place of 2^-6, so the code goes to bits 6..9; bf16: 0x4180 and
+// 2^-3, bits 3..6.  The mask comes in a vector register: an instruction that joins after masking takes one constant, not two, and
+// with both constants known the compiler makes two instructions of it (one token, 5120 -> 27648: 20.8 us against 18.3).
 template <int DT>
-__device__ __forceinline__ uint4 widen(uint32_t w)
+__device__ __forceinline__ uint4 widen(uint32_t w, uint32_t mask)
 {
-    if constexpr (DT == DT_F16) {       // 16.0 = 0x4c00, unit of the last place 2^-6: the code goes to bits 6..9
-        constexpr uint32_t M = 0x03c003c0u, O = 0x4c004c00u;
-        return make_uint4(((w << 6) & M) | O, ((w << 2) & M) | O, ((w >> 2) & M) | O, ((w >> 6) & M) | O);
-    } else {                            // 16.0 = 0x4180, unit of the last place 2^-3: bits 3..6
-        constexpr uint32_t M = 0x00780078u, O = 0x41804180u;
-        return make_uint4(((w << 3) & M) | O, ((w >> 1) & M) | O, ((w >> 5) & M) | O, ((w >> 9) & M) | O);
+    if constexpr (DT == DT_F16) {
+        constexpr uint32_t O = 0x4c004c00u;
+        return make_uint4(((w << 6) & mask) | O, ((w << 2) & mask) | O, ((w >> 2) & mask) | O, ((w >> 6) & mask) | O);
+    } else {
+        constexpr uint32_t O = 0x41804180u;
+        return make_uint4(((w << 3) & mask) | O, ((w >> 1) & mask) | O, ((w >> 5) & mask) | O, ((w >> 9) & mask) | O);
     }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t widen_mask()
+{
+    uint32_t m = DT == DT_F16 ? 0x03c003c0u : 0x00780078u;
+    asm volatile("" : "+v"(m));
+    return m;
 }
 
 constexpr int W4_WAVES = 8;
@@ -120,6 +130,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
     const uint32_t x_row = ((uint32_t)min(c, p.T - 1 - t0) * (uint32_t)hin + q * 8) * 2;
     const uint32_t one = DT == DT_F16 ? 0x3c003c00u : 0x3f803f80u;
     const uint4 ones = make_uint4(one, one, one, one);
+    const uint32_t mask = widen_mask<DT>();
     const unsigned group_lane = (q / STEPS) * W4_TN + c;
 
     auto fetch = [&](W4Tile<NT> &b, uint4 (&x)[4], int kt) {
@@ -152,7 +163,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
             sum = mfma16<DT>(ones, x[s], begins ? none : sum);
 #pragma unroll
             for (int n = 0; n < NT; n++)
-                acc[n] = mfma16<DT>(widen<DT>(s == 0 ? b.code[n].x : s == 1 ? b.code[n].y : s == 2 ? b.code[n].z : b.code[n].w), x[s], begins ? none : acc[n]);
+                acc[n] = mfma16<DT>(widen<DT>(s == 0 ? b.code[n].x : s == 1 ? b.code[n].y : s == 2 ? b.code[n].z : b.code[n].w, mask), x[s], begins ? none : acc[n]);
             if ((s + 1) % STEPS == 0) {                           // and ends here
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
@@ -230,6 +241,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
                                                                   // waited for by the first instruction that touches what it brings
     const uint32_t one = DT == DT_F16 ? 0x3c003c00u : 0x3f803f80u;
     const uint4 ones = make_uint4(one, one, one, one);
+    const uint32_t mask = widen_mask<DT>();
     constexpr int PER_TILE = 4 / STEPS;
     const unsigned glane = (q / STEPS) * W4_TN + c;
 
@@ -296,7 +308,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
             for (int m = 0; m < MT; m++) sum[m] = mfma16<DT>(ones, x[m], begins ? none : sum[m]);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const uint4 a = widen<DT>(s == 0 ? b.code[n].x : s == 1 ? b.code[n].y : s == 2 ? b.code[n].z : b.code[n].w);
+                const uint4 a = widen<DT>(s == 0 ? b.code[n].x : s == 1 ? b.code[n].y : s == 2 ? b.code[n].z : b.code[n].w, mask);
 #pragma unroll
                 for (int m = 0; m < MT; m++) acc[m][n] = mfma16<DT>(a, x[m], begins ? none : acc[m][n]);
             }
@@ -312,10 +324,11 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
                     }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
-            if (s == 0) xload(kt + AHEAD * WK, (buf + AHEAD) % BUFS);
-            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (MT > 2) __builtin_amdgcn_sched_barrier(0);      // or the steps' operands are all made at once and the registers run out
         }
+        // behind this tile's products: before them it would be among the loads that the compiler counts as codes, and some of those would be waited for
+        __builtin_amdgcn_sched_barrier(0);
+        xload(kt + AHEAD * WK, (buf + AHEAD) % BUFS);
         // the next tile's x, asked for a tile ago: behind it came this tile's loads of codes, groups and x
         asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * NT + XLOADS) : "memory");
         __builtin_amdgcn_s_barrier();
