@@ -109,7 +109,7 @@ __device__ __forceinline__ W4Place w4_place(const W4Args &p)
 // a column tile's codes in one stretch) and are joined in LDS.  A wavefront asks for its next K tile's codes, groups and x before it
 // multiplies the present one.  A lane loads the scale and zero point of one column and K step; the result's layout wants those of
 // four columns, which it gets through LDS.  Bound by the way in and out at one projection (4096 -> 4096, one token: 4.7 us for 8.4 MB; the
-// launch alone takes half) and by vector instructions beyond (5120 -> 27648, 70.8 MB: 20.8 us, 3.4 TB/s).
+// launch alone takes half) and by vector instructions beyond (5120 -> 27648, 70.8 MB: 18.3 us, 3.9 TB/s).
 template <int DT, int NT, int STEPS>
 __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args p)
 {
@@ -431,26 +431,26 @@ static void wide_of(W4Args &a, hipStream_t s)
     hipLaunchKernelGGL((w4_wide_kernel<DT, MT, NT, WN, STEPS>), w4_grid(a), dim3(64 * W4_WAVES), 0, s, a);
 }
 
-// The projections of one group size.  Up to 16 tokens: two column tiles a workgroup once one each makes more workgroups than compute units
-// (16 tokens, 4096 -> 22016, group 128: 17.6 us against 26.2 with one and 18.0 with four; 4096 -> 4096: 8.0 against 6.7).
-// Beyond: the smallest workgroup whose number still runs in one round, since a round costs the walk over K (us, group 128, for
-// the forms in the order below; 4096 -> 4096, 32 tokens: 10.5 15.3 19.8 33.6 49.1; 4096 -> 22016, 32 tokens: 29.0 22.6 39.3 34.9 49.7,
-// 64: 55.6 34.1 39.4 35.1 51.0, 125: 95.9 58.3 57.9 67.6 51.8; 5120 -> 27648, 125: 145 86.8 92.8 83.9 64.0).  Two workgroups of the second
-// form fit a compute unit.  The last form's accumulators fit the registers with one group a K tile only.
+// The projections of one group size, by the workgroups (times of a launch in us, group 128, the forms in the order of the code):
+//   tokens, widths                one tile   two    shared x: 32 cols   64    256
+//     1  4096 ->  4096               4.7     5.6         8.5           12.8   46.5      one column tile a workgroup while that makes one round
+//    16  4096 -> 22016              26.3    17.4        26.0           20.2   47.3      of workgroups, two beyond
+//    32  4096 ->  4096              10.8     8.2         9.9           13.7   47.4      two, in two token blocks, while those make one round
+//    64  4096 ->  4096              18.8    12.4        10.3           13.9   48.1      then x shared over 32 columns, again for one round
+//    64  4096 -> 22016              86.3    49.6        50.5           30.4   49.1      then over 64, of which two workgroups fit a unit
+//   125  4096 -> 22016             165.1    93.6        90.3           54.3   49.6      (1376 of them), and from about four and a half
+//   125  5120 -> 27648             260.4   143.3       136.5           82.8   61.6      times the units' number on over 256
+// The last form's accumulators fit the registers with one group a K tile only.
 template <int DT, int STEPS>
 static void gemv_by_size(W4Args a, hipStream_t s)
 {
     const unsigned cus = (unsigned)device_compute_units();
-    if (a.T <= 16) {
-        if (w4_blocks(a, 1, 16) > cus) gemv_of<DT, 2, STEPS>(a, s); else gemv_of<DT, 1, STEPS>(a, s);
-        return;
-    }
+    if (a.T <= 16 && w4_blocks(a, 1, 16) <= cus) return gemv_of<DT, 1, STEPS>(a, s);
+    if (a.T <= 16 || (a.T <= 32 && w4_blocks(a, 2, 16) <= cus)) return gemv_of<DT, 2, STEPS>(a, s);
     if (w4_blocks(a, 2, 32) <= cus) return wide_of<DT, 2, 1, 2, STEPS>(a, s);
-    if (w4_blocks(a, 4, 32) <= 2 * cus) return wide_of<DT, 2, 1, 4, STEPS>(a, s);
-    if (w4_blocks(a, 4, 64) <= cus) return wide_of<DT, 4, 1, 4, STEPS>(a, s);
-    if (w4_blocks(a, 8, 64) <= cus) return wide_of<DT, 4, 1, 8, STEPS>(a, s);
-    if constexpr (STEPS == 4) wide_of<DT, 4, 2, 8, STEPS>(a, s);
-    else wide_of<DT, 4, 1, 4, STEPS>(a, s);
+    if constexpr (STEPS == 4)
+        if (2 * w4_blocks(a, 4, 32) > 9 * cus) return wide_of<DT, 4, 2, 8, STEPS>(a, s);
+    wide_of<DT, 2, 1, 4, STEPS>(a, s);
 }
 
 template <int DT>
