@@ -7,7 +7,8 @@
         ...
 
 The step allocates nothing after its first batch of a size, apart from what the calls take from torch's allocator for their own
-length, so it may be captured in a HIP graph once it has run eagerly.
+length, so it may be captured in a HIP graph once it has run eagerly.  Batches of up to 2^k tokens share one set of buffers: a graph's
+replay and other work of the same step object are ordered on one stream.
 """
 from __future__ import annotations
 
@@ -46,8 +47,9 @@ class TokenStep:
         self.pool, self.cache, self.weights, self.n_q_heads, self.rope, self.names = pool, cache, weights, n_q_heads, rope, list(names)
         self.batch: Optional[KVBatch] = None
         self.tok_adapter = None
-        # Batch size -> plans and buffers.  None is ever given back: a graph that was captured with them goes on using them.
-        self._kept = {}
+        # Batch size -> plans and views, power of two -> buffers.  None is ever given back: a graph that was captured with them goes on
+        # using them.  Buffers for every size would add up: to 4 GB over the sizes to 512, with four rows of 8 KB a token.
+        self._kept, self._buffers = {}, {}
         self._outgrown = []
 
     def begin(self, batch: KVBatch, tok_adapter: torch.Tensor) -> None:
@@ -57,9 +59,12 @@ class TokenStep:
         T, n_prefix = batch.T, 0 if batch.prefix_len is None else batch.prefix_len.numel()
         kept = self._kept.get(T)
         if kept is None:
-            new = dict(dtype=self.cache.dtype, device=self.cache.device)
-            kept = self._kept[T] = [ops.plan_decode(tok_adapter, self.pool, n_proj=3), None,
-                                    [torch.empty((T, w), **new) for w in self.widths], torch.zeros((T, self.n_q_heads, self.cache.head_dim), **new), -1]
+            room = max(1, 1 << (T - 1).bit_length()) if T else 1
+            if room not in self._buffers:
+                new = dict(dtype=self.cache.dtype, device=self.cache.device)
+                self._buffers[room] = [torch.empty((room, w), **new) for w in self.widths] + [torch.zeros((room, self.n_q_heads, self.cache.head_dim), **new)]
+            *qkv, out = (b[:T] for b in self._buffers[room])
+            kept = self._kept[T] = [ops.plan_decode(tok_adapter, self.pool, n_proj=3), None, qkv, out, -1]
         else:
             ops.plan_decode(tok_adapter, self.pool, out=kept[0])
         if n_prefix > kept[4]:            # room for twice as many, so that a growing number of prompts moves the plan a few times only

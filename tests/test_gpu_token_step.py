@@ -119,6 +119,25 @@ def test_a_captured_step_replays():
         assert torch.equal(once(), got) and torch.equal(cache.k, k)
 
 
+def test_buffers_do_not_add_up_over_batch_sizes():
+    """Steps of every size to 33, up and down, keep a buffer for a power of two each; results are those of a step of its own."""
+    pool, weights, cache, g = build(1, 128, 4, 2, 64, 3, torch.float16, 40, 1)
+    ws = [{n: mlora.W4Weight(*w, group=32) for n, w in layer.items()} for layer in weights]
+    rope = mlora.RopeTable(64, 64)
+    shared = mlora.TokenStep(pool, cache, ws, 4, rope)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for T in list(range(1, 34)) + list(range(33, 0, -4)):
+        batch = mlora.KVBatch(torch.arange(T, **i32), torch.full((T,), 15, **i32), torch.arange(T, **i32)[:, None])
+        x, slots = torch.randn((T, 128), device="cuda", generator=g).half(), torch.randint(-1, 3, (T,), generator=g, **i32)
+        alone = mlora.TokenStep(pool, cache, ws, 4, rope)
+        for step in (shared, alone):
+            step.begin(batch, slots)
+        want = alone.layer(0, x).clone()
+        got = shared.layer(0, x)
+        assert got.shape == (T, 4, 64) and torch.equal(got, want)
+    assert len({t.untyped_storage().data_ptr() for k in shared._kept.values() for t in k[2] + [k[3]]}) == 4 * 7
+
+
 def test_trace_with_prompts():
     """A short trace with keys and values: requests come and go, prompts are shared, every step's attention is that of the cache."""
     H, D, prompt = 256, 64, 40
