@@ -54,7 +54,7 @@ PyObject *s_page_tbl, *s_rank, *s_scaling, *s_work, *s_group, *s_perm, *s_seg_st
     *s_chunk_start, *s_chunk_len, *s_chunk_adapter, *s_counters, *s_row_off, *s_tok_rank, *s_tok_scale, *s_T, *s_workspace,
     *s_n_slots, *s_max_pages, *s_page_rows, *s_n_pages, *s_max_rank, *s_tok_adapter, *s_dtype_code, *s_projections, *s_a_rows, *s_b_rows, *s_buf,
     *s_packed, *s_hin, *s_hout, *s_has_zeros, *s_tok_req, *s_tok_pos, *s_pages, *s_req_prefix, *s_prefix_pages, *s_prefix_len, *s_k, *s_v,
-    *s_cos_sin, *s_interleaved, *s_batch, *s_n_q_heads, *s_n_kv_heads, *s_page_tokens;
+    *s_cos_sin, *s_interleaved, *s_batch, *s_n_q_heads, *s_n_kv_heads, *s_page_tokens, *s_n_req, *s_n_prefix;
 
 void *attr_ptr(PyObject *o, PyObject *name)          // data pointer of a tensor attribute, null for None
 {
@@ -665,8 +665,9 @@ PyObject *prefix_attention(PyObject *const *v, Py_ssize_t nargs)
     const Batch b = batch_of(batch.o);
     need_prefix_pages(b);
     const int64_t q_heads = attr_int(plan, s_n_q_heads);
-    if (attr_int(plan, s_n_kv_heads) != c.n_kv_heads || attr_int(plan, s_page_tokens) != c.page_tokens || attr_int(plan, s_T) != b.T)
-        raise(PyExc_ValueError, "the plan was made for another cache layout or batch size");
+    if (attr_int(plan, s_n_kv_heads) != c.n_kv_heads || attr_int(plan, s_page_tokens) != c.page_tokens || attr_int(plan, s_T) != b.T ||
+        attr_int(plan, s_n_req) != b.n_req || attr_int(plan, s_n_prefix) != b.n_prefix)
+        raise(PyExc_ValueError, "the plan was made for another cache layout, batch size or number of requests or prefixes");
     int64_t q_stride, o_stride;
     const void *q = token_rows("q", tensor(v[0]), b.T, q_heads, c, q_stride);
     void *out = token_rows("out", tensor(v[1]), b.T, q_heads, c, o_stride);
@@ -721,7 +722,8 @@ PyMODINIT_FUNC PyInit__host()
         {&s_packed, "packed"}, {&s_hin, "hin"}, {&s_hout, "hout"}, {&s_has_zeros, "has_zeros"}, {&s_tok_req, "tok_req"},
         {&s_tok_pos, "tok_pos"}, {&s_pages, "pages"}, {&s_req_prefix, "req_prefix"}, {&s_prefix_pages, "prefix_pages"},
         {&s_prefix_len, "prefix_len"}, {&s_k, "k"}, {&s_v, "v"}, {&s_cos_sin, "cos_sin"}, {&s_interleaved, "interleaved"},
-        {&s_batch, "batch"}, {&s_n_q_heads, "n_q_heads"}, {&s_n_kv_heads, "n_kv_heads"}, {&s_page_tokens, "page_tokens"}};
+        {&s_batch, "batch"}, {&s_n_q_heads, "n_q_heads"}, {&s_n_kv_heads, "n_kv_heads"}, {&s_page_tokens, "page_tokens"},
+        {&s_n_req, "n_req"}, {&s_n_prefix, "n_prefix"}};
     for (const auto &p : names)
         if (!(*p.first = PyUnicode_InternFromString(p.second))) return nullptr;
     return PyModule_Create(&module);

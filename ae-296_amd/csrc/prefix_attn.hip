@@ -380,6 +380,12 @@ struct Walk {
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) w[4 * h + i] = __builtin_amdgcn_exp2f(fmaf(s[n][h][i], scale2, -ref));
+            // The fused product is exact and the maximum is a rounded one: the largest key's weight is 2 to the power of that rounding, which the
+            // sum shares.  From scores of 2^24 on it is a power that a 16-bit weight does not hold, so there both are rounded.
+            if (__ballot(fabsf(ref) > 16777216.f)) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(__fsub_rn(__fmul_rn(s[n][i / 4][i % 4], scale2), ref));
+            }
             wf[n] = pack8<DT>(w);
             // the sum takes the weights as rounded: a rounding that is in both sums moves their quotient less, and four instructions do it
             const uint32_t one = DT == DT_F16 ? 0x3c003c00u : 0x3f803f80u;

@@ -117,6 +117,8 @@ class AttnPlan:
     n_kv_heads: int
     page_tokens: int
     buf: torch.Tensor
+    n_req: int = 0
+    n_prefix: int = 0
 
 
 def plan_attention(batch: KVBatch, cache: KVCache, n_q_heads: int, out: Optional[AttnPlan] = None, room: int = 0) -> AttnPlan:
@@ -137,9 +139,10 @@ def plan_attention(batch: KVBatch, cache: KVCache, n_q_heads: int, out: Optional
     if rc:
         _ext.check(rc)
     if out is None:
-        return AttnPlan(batch, batch.T, n_q_heads, cache.n_kv_heads, cache.page_tokens, buf)
+        return AttnPlan(batch, batch.T, n_q_heads, cache.n_kv_heads, cache.page_tokens, buf, batch.pages.shape[0], n_prefix)
     # only now: a batch that the buffer does not hold was refused and must not be taken for the plan's own
     out.batch, out.T, out.n_q_heads, out.n_kv_heads, out.page_tokens = batch, batch.T, n_q_heads, cache.n_kv_heads, cache.page_tokens
+    out.n_req, out.n_prefix = batch.pages.shape[0], n_prefix
     return out
 
 

@@ -5,7 +5,7 @@ import torch
 
 import mlora
 from gpu_common import say
-from step_ref import Scene
+from step_ref import U32, Scene, f64, store_bound
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -100,6 +100,32 @@ def test_peaked_rows():
     """Scores far apart: one key takes the whole weight, in any place of the context."""
     say("attention peaked")
     run(Scene([(0, 100), (-1, 700), (0, 1)], [200], 4, 2, 128, 16, F16, seed=4, std_q=30.0))
+
+
+@pytest.mark.parametrize("dtype, power", [(F16, 14), (BF16, 40)])
+@pytest.mark.parametrize("n_req, D", [(3, 64), (70, 128)])
+def test_scores_far_beyond_24_bits(n_req, D, dtype, power):
+    """Powers of two, so that every score is exact: the largest key has the whole weight, or shares it with its equals."""
+    say(f"attention scores of 2^{2 * power + 6} {dtype}")
+    s = Scene([(0, 5 + 7 * i) for i in range(n_req)], [900], 2, 1, D, 16, dtype, seed=n_req)
+    g = torch.Generator().manual_seed(5)
+    factor = torch.tensor([0.25, 0.5, 1.0])[torch.randint(0, 3, s.k.shape[:4] + (1,), generator=g)].expand(s.k.shape)
+    s.k = torch.where(s.k.isnan(), s.k, (factor * 2.0 ** power).to(dtype))
+    s.cache.k.copy_(s.k)
+    sign = torch.randint(0, 2, (n_req, 2, 1), generator=g) * 2 - 1
+    s.q = (sign * 2.0 ** power).expand(n_req, 2, D).to(dtype).contiguous()
+    s.dev_q = s.q.cuda()
+    plan = mlora.plan_attention(s.batch, s.cache, 2)
+    out = f64(mlora.prefix_attention(s.dev_q, s.cache, 0, plan))
+    for t in range(n_req):
+        k = np.concatenate([s.rows("k", 0, s.prefix_lists[0], 900, 0), s.rows("k", 0, s.req_lists[t], 5 + 7 * t, 0)])
+        v = np.concatenate([s.rows("v", 0, s.prefix_lists[0], 900, 0), s.rows("v", 0, s.req_lists[t], 5 + 7 * t, 0)])
+        for h in range(2):
+            score = k @ f64(s.q[t, h])
+            top = v[score == score.max()]
+            # n weights of one: fp32 sums of n values in any order, the quotient, the rounding of the result
+            bound = (len(top) + 2) * U32 * np.abs(top).sum(0) / len(top) * 1.001 + store_bound(top.mean(0), dtype) * 1.001
+            assert (np.abs(out[t, h] - top.mean(0)) <= bound).all(), (t, h)
 
 
 def test_positions_inside_the_prefix_and_before_the_start():
@@ -273,6 +299,11 @@ def test_refusals():
         mlora.prefix_attention(q, mlora.KVCache(1, 4, 4, 64), 0, plan)
     with pytest.raises(ValueError, match="another cache layout"):
         mlora.prefix_attention(q, mlora.KVCache(1, 4, 2, 64, page_tokens=32), 0, plan)
+    pages, of = s.batch.pages, s.batch.req_prefix
+    s.batch.pages, s.batch.req_prefix = pages[:1].contiguous(), of[:1].contiguous()       # a table that the plan has not seen
+    with pytest.raises(ValueError, match="number of requests"):
+        mlora.prefix_attention(q, s.cache, 0, plan)
+    s.batch.pages, s.batch.req_prefix = pages, of
     many = Scene([(0, 5)] * 400, [40], 4, 2, 64, 16, F16, seed=18)
     with pytest.raises(mlora.MloraError) as e:
         mlora.plan_attention(many.batch, many.cache, 4, out=plan)
