@@ -1,5 +1,6 @@
 // extern "C" surface of the decode step around the LoRA apply (declared in include/mlora.h): argument validation on the host,
 // then the kernel launches on the caller's stream.  No allocation, no synchronisation, no state kept between calls.
+#include <cmath>
 #include <cstring>
 
 #include "../../include/mlora.h"
@@ -17,6 +18,12 @@ int fail(int code, const char *fmt, ...)
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes)
+{
+    const uintptr_t u = reinterpret_cast<uintptr_t>(a), w = reinterpret_cast<uintptr_t>(b);
+    return u < w + b_bytes && w < u + a_bytes;
+}
 
 int log2_exact(int v)
 {
@@ -135,6 +142,12 @@ int mlora_w4_gemv_multi(int n_proj, void *const *y, const void *const *x, const 
         w.per_tile = sh.per_tile; w.zeros = zeros[p] != 0;
     }
     if (T == 0) return MLORA_OK;
+    for (int p = 0; p < n_proj; p++)                              // workgroups read and write in no order
+        for (int o = 0; o < n_proj; o++) {
+            const size_t yp = (size_t)T * hout[p] * 2;
+            if (overlap(y[p], yp, x[o], (size_t)T * hin[o] * 2) || (o < p && overlap(y[p], yp, y[o], (size_t)T * hout[o] * 2)))
+                return fail(MLORA_EINVAL, "projection %d: y overlaps x or y of projection %d", p, o);
+        }
     int64_t blocks = 0;
     for (int p = 0; p < n_proj; p++) blocks += a.pr[p].n_tiles;
     if ((blocks + 8) * ((T + 15) / 16) > (1LL << 30)) return fail(MLORA_ERANGE, "the call has more than 2^30 tiles of 16 tokens x 16 columns");
@@ -151,6 +164,7 @@ int mlora_kv_append(const void *q, int64_t q_stride, void *q_out, int64_t q_out_
 {
     if (dtype != MLORA_F16 && dtype != MLORA_BF16) return fail(MLORA_EDTYPE, "dtype must be MLORA_F16 or MLORA_BF16 (got %d)", dtype);
     if (T < 0) return fail(MLORA_EINVAL, "T must be >= 0 (got %d)", T);
+    if (T > (1 << 30)) return fail(MLORA_ERANGE, "T may be 2^30 at most (got %d)", T);
     int rc = check_cache(n_pages, page_tokens, n_q_heads, n_kv_heads, head_dim);
     if (rc) return rc;
     if (rot < 0 || rot > head_dim || (rot & 15)) return fail(MLORA_ERANGE, "rot must be a multiple of 16 in 0..head_dim (got %d)", rot);
@@ -226,6 +240,7 @@ int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t
     if (rc) return rc;
     if (T == 0) return MLORA_OK;
     if ((rc = check_prefix(req_prefix, prefix_len, n_prefix))) return rc;
+    if (!(fabsf(scale) <= 3.4e38f)) return fail(MLORA_EINVAL, "scale must be finite");
     if (n_prefix > 0 && !prefix_tbl) return fail(MLORA_EINVAL, "prefix_tbl is needed with n_prefix > 0");
     if (n_prefix > 0 && (rc = check_table("max_prefix_pages", max_prefix_pages, page_tokens))) return rc;
     if (!out || !q || !k_pages || !v_pages || !plan) return fail(MLORA_EINVAL, "out, q, k_pages, v_pages and plan must not be NULL");

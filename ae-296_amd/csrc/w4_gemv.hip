@@ -105,11 +105,11 @@ __device__ __forceinline__ W4Place w4_place(const W4Args &p)
     return at;                                                    // proj == n_proj: no such block
 }
 
-// Up to 16 tokens.  A workgroup: NT column tiles, its eight wavefronts share the K tiles (every eighth each, so that together they read
+// 16 tokens a token block.  A workgroup: NT column tiles, its eight wavefronts share the K tiles (every eighth each, so that together they read
 // a column tile's codes in one stretch) and are joined in LDS.  A wavefront asks for its next K tile's codes, groups and x before it
 // multiplies the present one.  A lane loads the scale and zero point of one column and K step; the result's layout wants those of
 // four columns, which it gets through LDS.  Bound by the way in and out at one projection (4096 -> 4096, one token: 4.7 us for 8.4 MB; the
-// launch alone takes half) and by vector instructions beyond (5120 -> 27648, 70.8 MB: 18.3 us, 3.9 TB/s).
+// launch alone takes half) and by vector instructions beyond (one token, 5120 -> 27648, 73 MB: 18.3 us, 4.0 TB/s).
 template <int DT, int NT, int STEPS>
 __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args p)
 {
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
 }
 
 // ------------------------------------------------------------------ product, more tokens
-// From 17 tokens on a wavefront of the kernel above would read more bytes of x than of codes.  Here WN wavefronts side by side (NT column
+// With more tokens the token blocks of the kernel above read the codes again, and a wavefront as many bytes of x as of codes.  Here WN wavefronts side by side (NT column
 // tiles each) share the x of a K tile through LDS, and the 8 / WN such parts of a workgroup take K tiles by turns.  x comes by loads
 // that fill LDS directly, whole rows of 256 bytes; 16-byte chunk `ch` of row r lies at chunk ch ^ (r % 16), so that the operand reads (one
 // chunk of sixteen rows) meet all banks.
@@ -220,6 +220,9 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
 // A K tile takes a wavefront less time than a load from HBM: codes are asked for three tiles ahead, x two.  The loads to LDS are
 // inline assembly, because the compiler would end them before any read of LDS; not knowing of them it waits for codes somewhat
 // earlier than it has to, one reason for the third tile.
+//
+// Bound by vector instructions (making operands of codes: 6 for 4 codes of 16 columns, the groups' sums) beside the matrix ones,
+// and from about 64 tokens on by those: 125 tokens, 5120 -> 27648, groups of 128 with zero points: 61.6 us for 35.4 GFLOP, 574 TFLOP/s.
 template <int DT, int MT, int NT, int WN, int STEPS>
 __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args p)
 {

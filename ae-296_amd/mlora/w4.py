@@ -88,7 +88,7 @@ class W4Weight:
 
 def w4_gemv(ys: Sequence[torch.Tensor], xs: Sequence[torch.Tensor], ws: Sequence[W4Weight], accumulate: bool = False) -> None:
     """Base products for up to 8 projections of one layer in one launch: ``ys[p] (+)= xs[p] @ ws[p]``, xs[p] [T, hin], ys[p]
-    [T, hout].  Made for decode batches (the weights are read once for every 64 tokens); ``bgmv(ys, xs, ...)`` then adds the
+    [T, hout], no y overlapping another one or an x.  Made for decode batches (the weights are read again every 16, 32 or 64 tokens); ``bgmv(ys, xs, ...)`` then adds the
     adapters' deltas."""
     rc = _ext.host().w4_gemv(ys, xs, ws, accumulate)
     if rc:

@@ -439,7 +439,7 @@ int mlora_prefill_reflayout(void *y, const void *x, const void *A_T, const void 
  *     the calls will use) and zeros (uint8 [groups, hout], or NULL) out as the kernel reads them: mlora_w4_packed_bytes(...)
  *     bytes, 16-byte aligned, once per weight; the sources are not needed afterwards.
  *   mlora_w4_gemv_multi takes y, x, packed, hin, hout, group and zeros (0 / 1: packed with zero points) as HOST arrays of n_proj
- *     entries.  Any T; made for the few rows of a decode batch (the weights are read once for every 64 of them).
+ *     entries; no y may overlap another y or an x.  Any T up to 2^20; made for the few rows of a decode batch (it reads the weights again every 16, 32 or 64 tokens, by its form).
  * No counterpart in the reference's LoRA path (its int4 base GEMMs: dequantize_gemm_int4.py:32,225,345).
  */
 int64_t mlora_w4_packed_bytes(int hin, int hout, int group, int zeros);
@@ -487,7 +487,7 @@ int mlora_kv_append(const void *q, int64_t q_stride, void *q_out, int64_t q_out_
  *   mlora_attn_plan divides the step's work: once per step, for every layer, into `plan` (mlora_attn_plan_bytes bytes).
  *   mlora_prefix_attention runs one layer against it; q and out as in mlora_kv_append (they must not overlap); workspace:
  *   mlora_attn_workspace_bytes bytes of fp32 partial results.  Calls that share a workspace, or write a plan that another
- *   reads, must be ordered on one stream.  The tables must be the ones the plan was made from.
+ *   reads, must be ordered on one stream.  The tables must be the ones the plan was made from.  scale: any finite value.
  * T <= MLORA_ATTN_MAX_T, n_prefix <= MLORA_ATTN_MAX_PREFIX.
  */
 #define MLORA_ATTN_MAX_T 8192

@@ -32,7 +32,8 @@ def gemv(**kw):
     (dict(T=0), OK), (dict(dtype=2), EDTYPE), (dict(n=0), ERANGE), (dict(n=9), ERANGE), (dict(T=-1), ERANGE), (dict(T=(1 << 20) + 1), ERANGE),
     (dict(y=None), EINVAL), (dict(group=None), EINVAL), (dict(hin=ints(60)), EALIGN), (dict(hout=ints(63)), EALIGN), (dict(hin=ints(0)), EINVAL),
     (dict(hout=ints(-8)), EINVAL), (dict(group=ints(16)), ERANGE), (dict(group=ints(256)), ERANGE), (dict(y=ptrs(16, 0)), EINVAL),
-    (dict(x=ptrs(16, 8)), EALIGN), (dict(w=ptrs(8)), EALIGN), (dict(hin=ints((1 << 24) + 8)), ERANGE)])
+    (dict(x=ptrs(16, 8)), EALIGN), (dict(w=ptrs(8)), EALIGN), (dict(hin=ints((1 << 24) + 8)), ERANGE),
+    (dict(x=ptrs(1 << 20), y=ptrs(1 << 20)), EINVAL), (dict(x=ptrs(1 << 20), y=ptrs((1 << 20) + 16)), EINVAL)])
 def test_gemv_arguments(kw, code):
     assert gemv(**kw) == code
 
@@ -92,7 +93,7 @@ def append(**kw):
     (dict(n_pos=0), EINVAL), (dict(k=None), EINVAL), (dict(vp=None), EINVAL), (dict(o=None), EINVAL), (dict(q=None), EINVAL), (dict(k=off), EALIGN),
     (dict(cs=off), EALIGN), (dict(ks=120), EINVAL), (dict(vs=132), EALIGN), (dict(qs=504), EINVAL), (dict(os=520), EINVAL), (dict(req=None), EINVAL),
     (dict(tbl=None), EINVAL), (dict(n_req=0), EINVAL), (dict(mp=0), EINVAL), (dict(mp=1 << 27), ERANGE), (dict(n_prefix=1), EINVAL),
-    (dict(n_prefix=-1), ERANGE), (dict(n_prefix=4097), ERANGE)])
+    (dict(n_prefix=-1), ERANGE), (dict(n_prefix=4097), ERANGE), (dict(T=2 ** 31 - 1), ERANGE)])
 def test_append_arguments(kw, code):
     assert append(**kw) == code
 
@@ -115,10 +116,10 @@ def test_plan_arguments(kw, code):
 
 def attention(**kw):
     a = dict(o=one, os=512, q=one, qs=512, kp=one, vp=one, n_pages=4, P=16, Hq=8, Hkv=2, D=64, req=one, pos=one, T=3, tbl=one, n_req=2, mp=4, of=None,
-             pt=None, pl=None, n_prefix=0, mpp=0, plan=one, pn=1 << 30, ws=one, wn=1 << 40, dtype=1)
+             pt=None, pl=None, n_prefix=0, mpp=0, plan=one, pn=1 << 30, ws=one, wn=1 << 40, dtype=1, scale=0.1)
     a.update(kw)
     return _ext.lib().mlora_prefix_attention(a["o"], a["os"], a["q"], a["qs"], a["kp"], a["vp"], a["n_pages"], a["P"], a["Hq"], a["Hkv"], a["D"], a["req"],
-                                             a["pos"], a["T"], a["tbl"], a["n_req"], a["mp"], a["of"], a["pt"], a["pl"], a["n_prefix"], a["mpp"], 0.1,
+                                             a["pos"], a["T"], a["tbl"], a["n_req"], a["mp"], a["of"], a["pt"], a["pl"], a["n_prefix"], a["mpp"], a["scale"],
                                              a["plan"], a["pn"], a["ws"], a["wn"], a["dtype"], None)
 
 
@@ -126,7 +127,8 @@ def attention(**kw):
     (dict(T=0), OK), (dict(dtype=3), EDTYPE), (dict(T=-1), ERANGE), (dict(T=9000), ERANGE), (dict(D=80), ERANGE), (dict(Hq=6, Hkv=4), EINVAL),
     (dict(n_pages=-1), ERANGE), (dict(q=None), EINVAL), (dict(o=off), EALIGN), (dict(qs=500), EINVAL), (dict(os=516), EALIGN), (dict(plan=None), EINVAL),
     (dict(pn=8), ENOSPACE), (dict(wn=8), ENOSPACE), (dict(ws=None), ENOSPACE), (dict(n_prefix=2, of=one, pl=one), EINVAL),
-    (dict(n_prefix=2, of=one, pl=one, pt=one), EINVAL), (dict(tbl=None), EINVAL), (dict(mp=0), EINVAL)])
+    (dict(n_prefix=2, of=one, pl=one, pt=one), EINVAL), (dict(tbl=None), EINVAL), (dict(mp=0), EINVAL), (dict(scale=float("nan")), EINVAL),
+    (dict(scale=float("inf")), EINVAL), (dict(scale=float("-inf")), EINVAL)])
 def test_attention_arguments(kw, code):
     assert attention(**kw) == code
 
