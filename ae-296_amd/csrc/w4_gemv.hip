@@ -87,11 +87,25 @@ __device__ __forceinline__ uint32_t widen_mask()
 
 constexpr int W4_WAVES = 8;
 
+// What a row of x reads past its last column: loaded like the rest, it costs the product nothing (zeros put in place of loaded values there
+// took a quarter of the vector instructions of the kernel for more tokens).
+__device__ const uint4 w4_no_x = {0u, 0u, 0u, 0u};
+
 // What the product of one K tile needs besides x.  `group`: the group of this lane's column c and K step q, scale and 16 + zero point.
 template <int NT> struct W4Tile {
     uint4 code[NT];
     uint32_t group[NT];
 };
+
+// From a group's word, scale and 16 + zero point: what its sum of (16 + c) x and its sum of x are multiplied by.  Both are exact, and made once a
+// lane before the result's layout spreads them over four columns a lane.
+template <int DT>
+__device__ __forceinline__ void w4_factors(float (*to)[64], int lane, uint32_t word)
+{
+    const float f = lo_f32<DT>(word);
+    to[0][lane] = f;
+    to[1][lane] = -f * (float)(word >> 16);
+}
 
 // The column block, token block and projection of a workgroup.  Eight neighbouring ids go to the eight XCDs: the token blocks of one
 // column block follow each other on one of them.
@@ -115,7 +129,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
 {
     constexpr int PER_TILE = 4 / STEPS;
     __shared__ float part[W4_WAVES][16][17];
-    __shared__ __attribute__((aligned(16))) uint32_t words[W4_WAVES][NT][64];
+    __shared__ __attribute__((aligned(16))) float factors[W4_WAVES][NT][2][64];
     const W4Place place = w4_place(p);
     if (place.proj == p.n_proj) return;
     const W4Proj &w = p.pr[place.proj];
@@ -123,7 +137,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
     const unsigned char *codes = w.packed, *groups = w.packed + w.groups_at;
     const int hin = w.hin, k_tiles = w.k_tiles, n_last = w.n_tiles - 1;
     const bool zeros = w.zeros != 0;
-    const uint32_t middle = zeros ? 0u : 24u << 16;               // 16 + 8 where no zero points are stored; joined where it is used: a load is
+    const uint32_t middle = zeros ? 0u : 24u << 16;               // 16 + 8 where no zero points are stored; joined on the way to LDS: a load is
                                                                   // waited for by the first instruction that touches what it brings
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
     const unsigned char *x_block = static_cast<const unsigned char *>(w.x) + (size_t)t0 * hin * 2;
@@ -144,7 +158,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             const int k = kt * W4_TK + s * 32;
-            x[s] = k + q * 8 < hin ? ldg16(x_block + (x_row + (uint32_t)k * 2)) : zero16();
+            x[s] = ldg16(k + q * 8 < hin ? x_block + (x_row + (uint32_t)k * 2) : reinterpret_cast<const unsigned char *>(&w4_no_x));
         }
     };
 
@@ -153,7 +167,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
     for (int n = 0; n < NT; n++) out[n] = float4_t{0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](const W4Tile<NT> &b, const uint4 (&x)[4]) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) words[wave][n][lane] = b.group[n];
+        for (int n = 0; n < NT; n++) w4_factors<DT>(factors[wave][n], lane, b.group[n] | middle);
         __builtin_amdgcn_wave_barrier();
         float4_t acc[NT], sum;
 #pragma unroll
@@ -167,10 +181,10 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
             if ((s + 1) % STEPS == 0) {                           // and ends here
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    const uint4 g = *reinterpret_cast<const uint4 *>(&words[wave][n][s / STEPS * STEPS * 16 + q * 4]);
-                    const uint32_t u[4] = {g.x, g.y, g.z, g.w};
+                    const float4_t f = *reinterpret_cast<const float4_t *>(&factors[wave][n][0][s / STEPS * STEPS * 16 + q * 4]);
+                    const float4_t z = *reinterpret_cast<const float4_t *>(&factors[wave][n][1][s / STEPS * STEPS * 16 + q * 4]);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) out[n][i] += lo_f32<DT>(u[i]) * (acc[n][i] - (float)((u[i] | middle) >> 16) * sum[i]);
+                    for (int i = 0; i < 4; i++) out[n][i] = fmaf(z[i], sum[i], fmaf(f[i], acc[n][i], out[n][i]));
                 }
             }
             __builtin_amdgcn_sched_barrier(0);                    // or the steps' operands are all made at once and the registers run out
@@ -217,7 +231,10 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
 // that fill LDS directly, whole rows of 256 bytes; 16-byte chunk `ch` of row r lies at chunk ch ^ (r % 16), so that the operand reads (one
 // chunk of sixteen rows) meet all banks.
 //
-// A K tile takes a wavefront less time than a load from HBM: codes are asked for three tiles ahead, x two.  The loads to LDS are
+// The sums of x of the next tile are shared: a wavefront makes those of 4 MT / WN steps and leaves them in LDS for the others (125 tokens,
+// 5120 -> 27648, each wavefront its own: 62.7 us).
+//
+// A K tile takes a wavefront less time than a load from HBM: codes and x are asked for three tiles ahead.  The loads to LDS are
 // inline assembly, because the compiler would end them before any read of LDS; not knowing of them it waits for codes somewhat
 // earlier than it has to, one reason for the third tile.
 //
@@ -226,7 +243,9 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
 template <int DT, int MT, int NT, int WN, int STEPS>
 __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args p)
 {
-    constexpr int WK = W4_WAVES / WN, BUFS = 4, AHEAD = 2;
+    constexpr int WK = W4_WAVES / WN, BUFS = 4, AHEAD = 3;
+    constexpr int XS = 4 * MT / WN, SUMS = 4 / (STEPS < XS ? STEPS : XS);    // K steps whose x a wavefront adds up, sums of a token and K tile
+    static_assert(XS >= 1 && XS <= 4, "a wavefront adds up x of one token tile");
     constexpr int XTILE = MT * 16 * W4_TK * 2, XLOADS = MT * 4 / WN;     // bytes of x of a K tile, loads of a wavefront for it
     static_assert(XLOADS >= 1, "a wavefront's loads to LDS");
     constexpr int EXCHANGE = (W4_WAVES - WN) * MT * 16 * 17 * 4, RINGS = WK * BUFS * XTILE;
@@ -240,7 +259,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
     const unsigned char *codes = w.packed, *groups = w.packed + w.groups_at;
     const int hin = w.hin, k_tiles = w.k_tiles, n_last = w.n_tiles - 1;
     const bool zeros = w.zeros != 0;
-    const uint32_t middle = zeros ? 0u : 24u << 16;               // 16 + 8 where no zero points are stored; joined where it is used: a load is
+    const uint32_t middle = zeros ? 0u : 24u << 16;               // 16 + 8 where no zero points are stored; joined on the way to LDS: a load is
                                                                   // waited for by the first instruction that touches what it brings
     const uint32_t one = DT == DT_F16 ? 0x3c003c00u : 0x3f803f80u;
     const uint4 ones = make_uint4(one, one, one, one);
@@ -262,17 +281,31 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
     const unsigned char *x0 = static_cast<const unsigned char *>(w.x) + (size_t)t0 * hin * 2;
     unsigned char *tiles = lds + wk * (BUFS * XTILE);
     const uint32_t tiles_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)tiles;
-    __shared__ __attribute__((aligned(16))) uint32_t all_words[W4_WAVES][NT * 64];
-    uint32_t *words = all_words[wave];
-    const unsigned char *mine = reinterpret_cast<const unsigned char *>(words + q * 4);
-    auto xload = [&](int at_kt, int buf) {
-        const int kt = min(at_kt, k_tiles - 1);
+    __shared__ __attribute__((aligned(16))) float all_factors[W4_WAVES][NT][2][64];
+    float (*factors)[2][64] = all_factors[wave];
+    __shared__ __attribute__((aligned(16))) float all_sums[WK][2][MT * 16][SUMS];
+    float (*sums)[MT * 16][SUMS] = all_sums[wk];
+    auto xload = [&](int kt, int buf) {
 #pragma unroll
         for (int m = 0; m < XLOADS; m++) {
             const int r = (wn * XLOADS + m) * 4 + q;
-            const int k = min(kt * W4_TK + (c ^ (r & 15)) * 8, hin - 8);          // columns past the last: taken for zeros where they are used
+            const int k = kt * W4_TK + (c ^ (r & 15)) * 8;
             const unsigned char *src = x0 + ((uint32_t)min(r, p.T - 1 - t0) * (uint32_t)hin + k) * 2;
+            if (k >= hin) src = reinterpret_cast<const unsigned char *>(&w4_no_x);
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(tiles_at + buf * XTILE + (wn * XLOADS + m) * 1024), "v"(src) : "memory");
+        }
+    };
+
+    // operand of K step s: 16 tokens' x from a buffer
+    auto x_of = [&](int buf, int m, int s) { return *reinterpret_cast<const uint4 *>(tiles + buf * XTILE + (m * 16 + c) * 256 + ((s * 4 + q) ^ c) * 16); };
+    // this wavefront's sums of tile kt's x: every row of a product with ones is the sum, so a lane has its token's
+    auto add_up = [&](int buf) {
+        const int m = wn * XS / 4, s0 = wn * XS % 4;
+        float4_t sum;
+#pragma unroll
+        for (int i = 0; i < XS; i++) {
+            sum = mfma16<DT>(ones, x_of(buf, m, s0 + i), i % STEPS ? sum : float4_t{0.f, 0.f, 0.f, 0.f});
+            if ((i + 1) % STEPS == 0 || i == XS - 1) sums[buf & 1][m * 16 + c][(s0 + i) / (STEPS < XS ? STEPS : XS)] = sum[0];
         }
     };
 
@@ -286,29 +319,31 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
         load(ahead, kt + 3 * WK);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int n = 0; n < NT; n++) words[n * 64 + lane] = b.group[n];
+        for (int n = 0; n < NT; n++) w4_factors<DT>(factors[n], lane, b.group[n] | middle);
         __builtin_amdgcn_wave_barrier();
-        float4_t acc[MT][NT], sum[MT];
+        add_up((buf + 1) % BUFS);
+        float4_t acc[MT][NT];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             const bool begins = s % STEPS == 0, ends = (s + 1) % STEPS == 0;      // of a group
             const float4_t none = {0.f, 0.f, 0.f, 0.f};
             uint4 x[MT];
 #pragma unroll
-            for (int m = 0; m < MT; m++) x[m] = *reinterpret_cast<const uint4 *>(tiles + buf * XTILE + (m * 16 + c) * 256 + ((s * 4 + q) ^ c) * 16);
-            const int k = kt * W4_TK + s * 32;
-            if (k + 32 > hin) {
-                const uint32_t keep = k + q * 8 < hin ? ~0u : 0u;
-#pragma unroll
-                for (int m = 0; m < MT; m++) x[m] = make_uint4(x[m].x & keep, x[m].y & keep, x[m].z & keep, x[m].w & keep);
-            }
-            uint4 group[NT];
+            for (int m = 0; m < MT; m++) x[m] = x_of(buf, m, s);
+            float4_t f[NT], z[NT];
+            float sum[MT];
             if (ends) {
 #pragma unroll
-                for (int n = 0; n < NT; n++) group[n] = *reinterpret_cast<const uint4 *>(mine + (n * 64 + s / STEPS * STEPS * 16) * 4);
-            }
+                for (int n = 0; n < NT; n++) {
+                    f[n] = *reinterpret_cast<const float4_t *>(&factors[n][0][s / STEPS * STEPS * 16 + q * 4]);
+                    z[n] = *reinterpret_cast<const float4_t *>(&factors[n][1][s / STEPS * STEPS * 16 + q * 4]);
+                }
 #pragma unroll
-            for (int m = 0; m < MT; m++) sum[m] = mfma16<DT>(ones, x[m], begins ? none : sum[m]);
+                for (int m = 0; m < MT; m++) {
+                    const float *of = sums[buf & 1][m * 16 + c];
+                    sum[m] = STEPS > XS ? of[0] + of[SUMS - 1] : of[s / STEPS];
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const uint4 a = widen<DT>(s == 0 ? b.code[n].x : s == 1 ? b.code[n].y : s == 2 ? b.code[n].z : b.code[n].w, mask);
@@ -317,28 +352,24 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
             }
             if (ends) {
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const uint32_t u[4] = {group[n].x, group[n].y, group[n].z, group[n].w};
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float f = lo_f32<DT>(u[i]), z = (float)((u[i] | middle) >> 16);
+                    for (int m = 0; m < MT; m++)
 #pragma unroll
-                        for (int m = 0; m < MT; m++) out[m][n][i] += f * (acc[m][n][i] - z * sum[m][i]);
-                    }
-                }
+                        for (int i = 0; i < 4; i++) out[m][n][i] = fmaf(z[n][i], sum[m], fmaf(f[n][i], acc[m][n][i], out[m][n][i]));
             }
             if constexpr (MT > 2) __builtin_amdgcn_sched_barrier(0);      // or the steps' operands are all made at once and the registers run out
         }
         // behind this tile's products: before them it would be among the loads that the compiler counts as codes, and some of those would be waited for
         __builtin_amdgcn_sched_barrier(0);
         xload(kt + AHEAD * WK, (buf + AHEAD) % BUFS);
-        // the next tile's x, asked for a tile ago: behind it came this tile's loads of codes, groups and x
-        asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * NT + XLOADS) : "memory");
+        // x of the tile after the next, asked for a tile ago: behind it came this tile's loads of codes, groups and x
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(2 * NT + XLOADS) : "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
     W4Tile<NT> b0, b1, b2, b3;
-    // all parts pass the same barriers: where one has no last tile it multiplies by zeros (k is past the last column)
+    // all parts pass the same barriers: where one has no last tile it multiplies by zeros, x being past the last column
     load(b0, wk);
     __builtin_amdgcn_sched_barrier(0);
     xload(wk, 0);
@@ -349,7 +380,13 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
     __builtin_amdgcn_sched_barrier(0);
     load(b2, wk + 2 * WK);
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(4 * NT + XLOADS) : "memory");
+    xload(wk + 2 * WK, 2);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * NT + XLOADS) : "memory");      // x of the first two tiles
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    add_up(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
