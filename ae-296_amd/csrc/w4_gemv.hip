@@ -238,8 +238,8 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
 // inline assembly, because the compiler would end them before any read of LDS; not knowing of them it waits for codes somewhat
 // earlier than it has to, one reason for the third tile.
 //
-// Bound by vector instructions (making operands of codes: 6 for 4 codes of 16 columns, the groups' sums) beside the matrix ones,
-// and from about 64 tokens on by those: 125 tokens, 5120 -> 27648, groups of 128 with zero points: 61.6 us for 35.4 GFLOP, 574 TFLOP/s.
+// Bound by vector instructions (making operands of codes, the groups' factors), matrix instructions and the operand reads of x from LDS, none of
+// which fills its unit: 125 tokens, 5120 -> 27648, groups of 128: 55.1 us for 35.4 GFLOP, 640 TFLOP/s.
 template <int DT, int MT, int NT, int WN, int STEPS>
 __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args p)
 {
@@ -471,26 +471,47 @@ static void wide_of(W4Args &a, hipStream_t s)
     hipLaunchKernelGGL((w4_wide_kernel<DT, MT, NT, WN, STEPS>), w4_grid(a), dim3(64 * W4_WAVES), 0, s, a);
 }
 
-// The projections of one group size, by the workgroups (times of a launch in us, group 128, the forms in the order of the code):
-//   tokens, widths                one tile   two    shared x: 32 cols   64    256
-//     1  4096 ->  4096               4.7     5.6         8.5           12.8   46.5      one column tile a workgroup while that makes one round
-//    16  4096 -> 22016              26.3    17.4        26.0           20.2   47.3      of workgroups, two beyond
-//    32  4096 ->  4096              10.8     8.2         9.9           13.7   47.4      two, in two token blocks, while those make one round
-//    64  4096 ->  4096              18.8    12.4        10.3           13.9   48.1      then x shared over 32 columns, again for one round
-//    64  4096 -> 22016              86.3    49.6        50.5           30.4   49.1      then over 64, of which two workgroups fit a unit
-//   125  4096 -> 22016             165.1    93.6        90.3           54.3   49.6      (1376 of them), and from about four and a half
-//   125  5120 -> 27648             260.4   143.3       136.5           82.8   61.6      times the units' number on over 256
-// The last form's accumulators fit the registers with one group a K tile only.
+// The forms for more than 16 tokens: columns (in tiles) and tokens of a workgroup, and what a launch of them takes (tenths of a microsecond,
+// 5120 rows, groups of 128; it grows with the rows alike) where the busiest compute unit has one workgroup, or w: base + w each.  A form with room
+// for two on a unit takes less than twice as long for two.
+struct W4Form { int cols, rows, alone, base, each; };
+constexpr W4Form W4_FORMS[] = {{2, 16, 89, 34, 55}, {2, 32, 123, 20, 103}, {4, 32, 178, 30, 104}, {8, 32, 242, 30, 165}, {8, 64, 318, 20, 295}, {16, 64, 540, 20, 520}};
+
+// Up to 16 tokens: one column tile a workgroup while that makes one round of workgroups, two beyond (one token, 4096 -> 4096: 4.6 us against 5.7;
+// 4096 -> 22016: 15.9 against 13.2).  Beyond: the form of the least time by the table, which is the fastest at all of 21 sizes of 32 to 200 tokens but
+// four, there within 3 % (us, the forms in the table's order):
+//     32 tokens,  4096 ->  4096      8.0    10.1    13.0    19.2    24.9    42.6
+//     64          4096 ->  4096     12.7    10.7    13.3    19.2    25.6    43.4
+//     32          5120 -> 15360     26.8    23.6    17.8    24.0    31.5    53.2
+//    200          5120 -> 27648    225.9   234.7   127.6   103.5   118.0   106.7
+//    125          5120 -> 15360     86.6    82.5    44.9    35.8    32.1    53.7
+//    125          5120 -> 27648    143.8   141.1    75.1    65.5    61.3    55.1
+// With groups of 64 or 32 the accumulators and factors of the last three leave less room for workgroups (125 tokens, 5120 -> 15360, groups of
+// 64: 45.7 with the fourth, 45.9 with the third): the third is the widest there, at most 11 % behind what others reached.
 template <int DT, int STEPS>
 static void gemv_by_size(W4Args a, hipStream_t s)
 {
     const unsigned cus = (unsigned)device_compute_units();
-    if (a.T <= 16 && w4_blocks(a, 1, 16) <= cus) return gemv_of<DT, 1, STEPS>(a, s);
-    if (a.T <= 16 || (a.T <= 32 && w4_blocks(a, 2, 16) <= cus)) return gemv_of<DT, 2, STEPS>(a, s);
-    if (w4_blocks(a, 2, 32) <= cus) return wide_of<DT, 2, 1, 2, STEPS>(a, s);
-    if constexpr (STEPS == 4)
-        if (2 * w4_blocks(a, 4, 32) > 9 * cus) return wide_of<DT, 4, 2, 8, STEPS>(a, s);
-    wide_of<DT, 2, 1, 4, STEPS>(a, s);
+    if (a.T <= 16) {
+        if (w4_blocks(a, 1, 16) <= cus) gemv_of<DT, 1, STEPS>(a, s);
+        else gemv_of<DT, 2, STEPS>(a, s);
+        return;
+    }
+    int best = 0;
+    unsigned least = ~0u;
+    for (int i = 0; i < (STEPS == 4 ? 6 : 3); i++) {
+        const W4Form &f = W4_FORMS[i];
+        const unsigned w = (w4_blocks(a, f.cols, f.rows) + cus - 1) / cus, time = w == 1 ? f.alone : f.base + f.each * w;
+        if (time < least) { least = time; best = i; }
+    }
+    if (best == 0) gemv_of<DT, 2, STEPS>(a, s);
+    else if (best == 1) wide_of<DT, 2, 1, 2, STEPS>(a, s);
+    else if (best == 2) wide_of<DT, 2, 1, 4, STEPS>(a, s);
+    if constexpr (STEPS == 4) {
+        if (best == 3) wide_of<DT, 2, 2, 4, STEPS>(a, s);
+        else if (best == 4) wide_of<DT, 4, 2, 4, STEPS>(a, s);
+        else if (best == 5) wide_of<DT, 4, 2, 8, STEPS>(a, s);
+    }
 }
 
 template <int DT>

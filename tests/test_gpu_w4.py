@@ -63,7 +63,8 @@ def test_output_widths(hout):
     (17, 904, 72), (32, 1416, 2048),       # the same in two token blocks
     (20, 520, 4104), (64, 1032, 4096),     # x shared over 32 columns
     (40, 776, 4104), (21, 264, 8200), (130, 2056, 2056),      # over 64
-    (300, 1000, 8200), (330, 8, 8192), (300, 136, 8248), (320, 640, 8192)])   # over 256 at groups of 128, else over 64
+    (300, 1000, 8200), (330, 8, 8192), (300, 136, 8248), (320, 640, 8192),    # at groups of 128 over 128
+    (60, 392, 16400), (64, 1016, 16384), (190, 264, 16400)])                  # 64 tokens, over 128 and 256
 def test_every_form(T, hin, hout, group, zeros):
     """Sizes on either side of the lines between the kernel's forms, on a device of 256 compute units."""
     run(T, hin, hout, group, zeros, F16 if hout % 16 else BF16, seed=T, accumulate=hin % 16 != 0)
