@@ -122,8 +122,8 @@ __device__ __forceinline__ W4Place w4_place(const W4Args &p)
 // 16 tokens a token block.  A workgroup: NT column tiles, its eight wavefronts share the K tiles (every eighth each, so that together they read
 // a column tile's codes in one stretch) and are joined in LDS.  A wavefront asks for its next K tile's codes, groups and x before it
 // multiplies the present one.  A lane loads the scale and zero point of one column and K step; the result's layout wants those of
-// four columns, which it gets through LDS.  Bound by the way in and out at one projection (4096 -> 4096, one token: 4.7 us for 8.4 MB; the
-// launch alone takes half) and by vector instructions beyond (one token, 5120 -> 27648, 73 MB: 18.3 us, 4.0 TB/s).
+// four columns, which it gets through LDS.  Bound by the way in and out at one projection (4096 -> 4096, one token: 4.4 us for 8.7 MB; the
+// launch alone takes half) and by vector instructions beyond (one token, 5120 -> 27648, 73 MB: 17.7 us, 4.1 TB/s).
 template <int DT, int NT, int STEPS>
 __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args p)
 {
@@ -155,10 +155,14 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
             b.code[n] = ldg16_stream(codes + tile * W4_TILE_BYTES + lane * 16);
             b.group[n] = zeros ? reinterpret_cast<const uint32_t *>(groups)[at] : reinterpret_cast<const uint16_t *>(groups)[at];
         }
+        const unsigned char *x_tile = x_block + (uint32_t)kt * (W4_TK * 2);
+        if ((kt + 1) * W4_TK <= hin) {                            // chosen lane by lane in every tile: 1 to 2 % slower
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-            const int k = kt * W4_TK + s * 32;
-            x[s] = ldg16(k + q * 8 < hin ? x_block + (x_row + (uint32_t)k * 2) : reinterpret_cast<const unsigned char *>(&w4_no_x));
+            for (int s = 0; s < 4; s++) x[s] = ldg16(x_tile + (x_row + s * 64));
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+                x[s] = ldg16(kt * W4_TK + s * 32 + q * 8 < hin ? x_tile + (x_row + s * 64) : reinterpret_cast<const unsigned char *>(&w4_no_x));
         }
     };
 
