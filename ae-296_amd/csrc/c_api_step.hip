@@ -205,11 +205,11 @@ int64_t mlora_attn_workspace_bytes(int T, int n_prefix, int n_q_heads, int n_kv_
 }
 
 int mlora_attn_plan(const int32_t *tok_req, const int32_t *tok_pos, int T, int n_req, int max_pages, const int32_t *req_prefix,
-                    const int32_t *prefix_len, int n_prefix, int max_prefix_pages, int page_tokens, int n_q_heads, int n_kv_heads,
+                    const int32_t *prefix_len, int n_prefix, int max_prefix_pages, int page_tokens, int n_q_heads, int n_kv_heads, int head_dim,
                     void *plan, int64_t plan_bytes, void *stream)
 {
     if (T < 0 || T > MLORA_ATTN_MAX_T) return fail(MLORA_ERANGE, "T must be in 0..%d (got %d)", MLORA_ATTN_MAX_T, T);
-    int rc = check_cache(1, page_tokens, n_q_heads, n_kv_heads, 64);
+    int rc = check_cache(1, page_tokens, n_q_heads, n_kv_heads, head_dim);
     if (rc) return rc;
     if (T == 0) return MLORA_OK;
     if (n_req <= 0) return fail(MLORA_EINVAL, "n_req must be positive (got %d)", n_req);
@@ -222,7 +222,7 @@ int mlora_attn_plan(const int32_t *tok_req, const int32_t *tok_pos, int T, int n
     memset(&b, 0, sizeof(b));
     b.tok_req = tok_req; b.tok_pos = tok_pos; b.req_prefix = n_prefix > 0 ? req_prefix : nullptr; b.prefix_len = prefix_len;
     b.T = T; b.n_req = n_req; b.max_pages = max_pages; b.n_prefix = n_prefix; b.max_prefix_pages = max_prefix_pages;
-    rc = mlora::launch_attn_plan(b, log2_exact(page_tokens), n_q_heads, n_kv_heads, plan, static_cast<hipStream_t>(stream));
+    rc = mlora::launch_attn_plan(b, log2_exact(page_tokens), n_q_heads, n_kv_heads, head_dim, plan, static_cast<hipStream_t>(stream));
     if (rc) return fail(MLORA_ELAUNCH, "plan launch failed: %s", hipGetErrorString((hipError_t)rc));
     return MLORA_OK;
 }

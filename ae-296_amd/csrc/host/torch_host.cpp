@@ -644,15 +644,15 @@ void *plan_buf(const at::Tensor &t)
     return t.data_ptr();
 }
 
-// attn_plan(batch, buf, page_tokens, n_q_heads, n_kv_heads)
+// attn_plan(batch, buf, page_tokens, n_q_heads, n_kv_heads, head_dim)
 PyObject *attn_plan(PyObject *const *v, Py_ssize_t nargs)
 {
-    if (nargs != 5) raise(PyExc_TypeError, "attn_plan takes 5 arguments");
+    if (nargs != 6) raise(PyExc_TypeError, "attn_plan takes 6 arguments");
     const Batch b = batch_of(v[0]);
     need_prefix_pages(b);
     const at::Tensor &buf = tensor(v[1]);
     return PyLong_FromLong(launch(mlora_attn_plan, b.tok_req, b.tok_pos, b.T, b.n_req, b.max_pages, b.req_prefix, b.prefix_len, b.n_prefix,
-                                  b.max_prefix_pages, (int)as_int(v[2]), (int)as_int(v[3]), (int)as_int(v[4]), plan_buf(buf), buf.numel(), stream()));
+                                  b.max_prefix_pages, (int)as_int(v[2]), (int)as_int(v[3]), (int)as_int(v[4]), (int)as_int(v[5]), plan_buf(buf), buf.numel(), stream()));
 }
 
 // prefix_attention(q, out, cache, layer, plan, scale)

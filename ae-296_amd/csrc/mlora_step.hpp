@@ -93,7 +93,7 @@ int launch_w4_gemv(const W4Args &a, int dtype, hipStream_t s);
 int launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s);
 int64_t attn_plan_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads);
 int64_t attn_workspace_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads, int head_dim);
-int launch_attn_plan(const KvBatch &b, int page_shift, int n_q_heads, int n_kv_heads, void *plan, hipStream_t s);
+int launch_attn_plan(const KvBatch &b, int page_shift, int n_q_heads, int n_kv_heads, int head_dim, void *plan, hipStream_t s);
 int launch_prefix_attention(const AttnArgs &a, int dtype, const void *plan, void *workspace, hipStream_t s);
 
 // sets the calling thread's error text and returns `code` (defined with the other entry points)

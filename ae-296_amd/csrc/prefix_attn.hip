@@ -64,14 +64,15 @@ __host__ __device__ inline int pa_target(int n_kv_heads) { const int t = 512 / n
 
 // With C keys a range where C >= (sum of own keys + sum over groups of keys x row tiles) / target, a list is cut into at most
 // keys / C + 1 ranges, which bounds the items and the slots by sizes the host knows.
+// Groups may be cut up to twice as finely.
 inline int64_t pa_items_cap(int T, int n_prefix, int gq, int n_kv_heads)
 {
     const int64_t groups = T < n_prefix ? T : n_prefix, tiles = (int64_t)T * gq / PA_ROWS + groups, own_tiles = (gq + PA_ROWS - 1) / PA_ROWS;
-    return T * own_tiles + (n_prefix ? tiles : 0) + pa_target(n_kv_heads) * own_tiles + 1;
+    return T * own_tiles + (n_prefix ? tiles + pa_target(n_kv_heads) : 0) + pa_target(n_kv_heads) * own_tiles + 1;
 }
 inline int64_t pa_slots_cap(int T, int n_prefix, int gq, int n_kv_heads)
 {
-    const int64_t target = pa_target(n_kv_heads), per_tile = (PA_WIDE + gq - 1) / gq;
+    const int64_t target = pa_target(n_kv_heads) * (n_prefix ? 2 : 1), per_tile = (PA_WIDE + gq - 1) / gq;
     return (int64_t)T * (n_prefix ? 2 : 1) + target * (n_prefix ? per_tile : 1) + 1;
 }
 
@@ -84,7 +85,7 @@ __host__ __device__ inline PlanView pa_plan_view(void *plan, int T)
 struct PlanArgs {
     KvBatch b;
     void *plan;
-    int page_shift, gq, target;
+    int page_shift, gq, target, head_dim;
     long long items_cap, slots_cap;
 };
 
@@ -164,15 +165,19 @@ __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
     if ((threadIdx.x & 63) == 0 && work) atomicAdd(&s_work, work);
     __syncthreads();
     // keys of a range, a multiple of what the wavefronts take at a time
-    // (lists have 2^30 keys at most, so longer ranges than 2^30 are one range; and 32-bit divisions, of which a thread makes a handful in a chain:
+    // (lists have 2^30 keys at most: a range of nearly 2^31, or two thirds of it, holds any; and 32-bit divisions, of which a thread makes a handful in a chain:
     // with 64-bit ones the plan of one request took 5.7 us, that of 256 behind 8 prefixes 9.2)
     constexpr unsigned step = PA_WAVES * PA_KEYS;
     const unsigned long long all = s_work;
-    const unsigned each = all >> 31 ? (unsigned)min(all / (unsigned)p.target, 1ULL << 30) : ((unsigned)all + (unsigned)p.target - 1u) / (unsigned)p.target;
+    const unsigned each = all >> 31 ? (unsigned)min(all / (unsigned)p.target, (1ULL << 31) - step) : ((unsigned)all + (unsigned)p.target - 1u) / (unsigned)p.target;
     const unsigned C = max((each + step - 1) / step, 1u) * step;
     auto range_of = [&](int keys, int cuts) { return (((unsigned)keys + cuts - 1) / (unsigned)cuts + step - 1) / step * step; };
+    // At 64 elements a head three workgroups fit a unit, and the longest ranges of the groups end last: two thirds of the length (256 requests
+    // behind 8 prefixes of 1500, 32 heads on 4: 30.1 us a layer against 33.8; 64 requests: 19.1 against 17.6; at 128 elements, 128 requests behind one
+    // of 8191, 91 against 86, so not there).
+    const unsigned G = p.head_dim == 64 ? max(C / step * 2 / 3, 1u) * step : C;
     // a wide tile leaves as much behind as it reads in 130 keys: its ranges are 256 at least
-    auto group_cuts_of = [&](int f) { const unsigned c = rows_of(f) == PA_WIDE ? max(C, 256u) : C; return (int)((prefix_keys(f) + c - 1) / c); };
+    auto group_cuts_of = [&](int f) { const unsigned c = rows_of(f) == PA_WIDE ? max(G, 256u) : G; return (int)((prefix_keys(f) + c - 1) / c); };
     auto cuts_of = [&](int keys) { return keys > 0 ? (int)(((unsigned)keys + C - 1) / C) : 0; };
     // groups: their lists, slots and items
     int n_list = 0, n_slot = 0, n_item = 0;
@@ -743,10 +748,10 @@ int64_t attn_workspace_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads,
     return pa_slots_cap(T, n_prefix, n_q_heads / n_kv_heads, n_kv_heads) * n_q_heads * (head_dim + 2) * 4;
 }
 
-int launch_attn_plan(const KvBatch &b, int page_shift, int n_q_heads, int n_kv_heads, void *plan, hipStream_t s)
+int launch_attn_plan(const KvBatch &b, int page_shift, int n_q_heads, int n_kv_heads, int head_dim, void *plan, hipStream_t s)
 {
     PlanArgs a;
-    a.b = b; a.plan = plan; a.page_shift = page_shift; a.gq = n_q_heads / n_kv_heads; a.target = pa_target(n_kv_heads);
+    a.b = b; a.plan = plan; a.page_shift = page_shift; a.head_dim = head_dim; a.gq = n_q_heads / n_kv_heads; a.target = pa_target(n_kv_heads);
     a.items_cap = pa_items_cap(b.T, b.n_prefix, a.gq, n_kv_heads);
     hipLaunchKernelGGL(pa_plan_kernel, dim3(1), dim3(PL_THREADS), 0, s, a);
     return (int)hipGetLastError();

@@ -86,7 +86,7 @@ SIGNATURES = {
                                _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _i32, _vp]),
     "mlora_attn_plan_bytes": (_i64, [_i32, _i32, _i32, _i32]),
     "mlora_attn_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
-    "mlora_attn_plan": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "mlora_attn_plan": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
     "mlora_prefix_attention": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp,
                                       _vp, _vp, _i32, _i32, _f32, _vp, _i64, _vp, _i64, _i32, _vp]),
     "mlora_prefill_reflayout": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),

@@ -135,7 +135,7 @@ def plan_attention(batch: KVBatch, cache: KVCache, n_q_heads: int, out: Optional
         buf = torch.empty(need, dtype=torch.uint8, device=batch.tok_req.device)
     else:
         buf = out.buf
-    rc = _ext.host().attn_plan(batch, buf, cache.page_tokens, n_q_heads, cache.n_kv_heads)
+    rc = _ext.host().attn_plan(batch, buf, cache.page_tokens, n_q_heads, cache.n_kv_heads, cache.head_dim)
     if rc:
         _ext.check(rc)
     if out is None:

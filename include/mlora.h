@@ -495,7 +495,7 @@ int mlora_kv_append(const void *q, int64_t q_stride, void *q_out, int64_t q_out_
 int64_t mlora_attn_plan_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads);
 int64_t mlora_attn_workspace_bytes(int T, int n_prefix, int n_q_heads, int n_kv_heads, int head_dim);
 int mlora_attn_plan(const int32_t *tok_req, const int32_t *tok_pos, int T, int n_req, int max_pages, const int32_t *req_prefix,
-                    const int32_t *prefix_len, int n_prefix, int max_prefix_pages, int page_tokens, int n_q_heads, int n_kv_heads,
+                    const int32_t *prefix_len, int n_prefix, int max_prefix_pages, int page_tokens, int n_q_heads, int n_kv_heads, int head_dim,
                     void *plan, int64_t plan_bytes, void *stream);
 int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t q_stride, const void *k_pages,
                            const void *v_pages, int64_t n_pages, int page_tokens, int n_q_heads, int n_kv_heads, int head_dim,

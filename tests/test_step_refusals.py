@@ -100,16 +100,16 @@ def test_append_arguments(kw, code):
 
 # ---------------------------------------------------------------- attention
 def plan(**kw):
-    a = dict(req=one, pos=one, T=3, n_req=2, mp=4, of=None, pl=None, n_prefix=0, mpp=0, P=16, Hq=8, Hkv=2, buf=one, n=1 << 30)
+    a = dict(req=one, pos=one, T=3, n_req=2, mp=4, of=None, pl=None, n_prefix=0, mpp=0, P=16, Hq=8, Hkv=2, D=64, buf=one, n=1 << 30)
     a.update(kw)
-    return _ext.lib().mlora_attn_plan(a["req"], a["pos"], a["T"], a["n_req"], a["mp"], a["of"], a["pl"], a["n_prefix"], a["mpp"], a["P"], a["Hq"], a["Hkv"],
+    return _ext.lib().mlora_attn_plan(a["req"], a["pos"], a["T"], a["n_req"], a["mp"], a["of"], a["pl"], a["n_prefix"], a["mpp"], a["P"], a["Hq"], a["Hkv"], a["D"],
                                       a["buf"], a["n"], None)
 
 
 @pytest.mark.parametrize("kw, code", [
     (dict(T=0), OK), (dict(T=-1), ERANGE), (dict(T=8193), ERANGE), (dict(n_req=0), EINVAL), (dict(mp=0), EINVAL), (dict(mp=1 << 27), ERANGE),
     (dict(n_prefix=1, mpp=1), EINVAL), (dict(n_prefix=1, of=one, pl=one), EINVAL), (dict(P=20), EINVAL), (dict(Hq=9), EINVAL), (dict(buf=None), EINVAL),
-    (dict(buf=off), EALIGN), (dict(n=8), ENOSPACE), (dict(req=None), EINVAL)])
+    (dict(buf=off), EALIGN), (dict(n=8), ENOSPACE), (dict(req=None), EINVAL), (dict(D=96), ERANGE)])
 def test_plan_arguments(kw, code):
     assert plan(**kw) == code
 
