@@ -513,7 +513,7 @@ __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const_i32_ptr 
 #pragma unroll
         for (int w = 0; w < PA_WAVES; w++) m = fmaxf(m, s_m[w][r]);
 #pragma unroll
-        for (int w = 0; w < PA_WAVES; w++) l += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - m);
+        for (int w = 0; w < PA_WAVES; w++) l += s_l[w][r] * (s_m[w][r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w][r] - m));
         float v[E];
 #pragma unroll
         for (int k = 0; k < E; k += 4) {
@@ -698,7 +698,7 @@ __global__ __launch_bounds__(256) void pa_join_kernel(const AttnKernelArgs ka)
             if (slot < 0 || slot >= ka.slots_cap) continue;
             const size_t at = (size_t)slot * p.n_q_heads + row;
             const float2 x = *reinterpret_cast<const float2 *>(ml + at * 2);
-            if (x.x == -INFINITY) continue;
+            if (x.x == -INFINITY && x.y == 0.f) continue;       // no keys; scores that are all NaN leave no maximum, but a sum that is NaN
             const float top = fmaxf(m, x.x), a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), b = __builtin_amdgcn_exp2f(x.x - top);
             m = top;
             l = l * a + x.y * b;

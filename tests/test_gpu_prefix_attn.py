@@ -128,6 +128,22 @@ def test_scores_far_beyond_24_bits(n_req, D, dtype, power):
             assert (np.abs(out[t, h] - top.mean(0)) <= bound).all(), (t, h)
 
 
+@pytest.mark.parametrize("n_req", [1, 6, 70])
+@pytest.mark.parametrize("prefix, own", [(0, 20), (0, 3000), (400, 30)])
+def test_a_nan_query_stays_nan_and_alone(n_req, prefix, own):
+    """One head of one token is NaN: it has no maximum, cut into parts or not.  The rows beside it in its tile are what they are without it."""
+    say(f"attention NaN query, {n_req} requests, prefix {prefix}, own {own}")
+    s = Scene([(0 if prefix else -1, own + i % 5) for i in range(n_req)], [prefix] if prefix else [], 4, 2, 64, 16, BF16, seed=own)
+    plan = mlora.plan_attention(s.batch, s.cache, 4)
+    want = mlora.prefix_attention(s.dev_q, s.cache, 0, plan)
+    t = n_req // 2
+    s.dev_q[t, 1] = float("nan")
+    got = mlora.prefix_attention(s.dev_q, s.cache, 0, plan)
+    assert got[t, 1].isnan().all()
+    got[t, 1] = want[t, 1]
+    assert torch.equal(got, want)
+
+
 def test_positions_inside_the_prefix_and_before_the_start():
     """A token at a position of its own prefix sees the prefix up to itself; one before the start sees nothing and is zeros."""
     say("attention positions inside the prefix")
