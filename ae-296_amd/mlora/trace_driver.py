@@ -167,6 +167,8 @@ class TraceContext:
 
     def advance(self, requests: Sequence[int], lora_ids: Sequence[int]) -> dict:
         """One more token for every request listed; those no longer listed give their pages back.  The batch as host lists."""
+        if len(requests) != len(lora_ids) or len({int(r) for r in requests}) != len(requests):
+            raise ValueError("every request of a step is listed once, with one adapter")
         P = self.cache.page_tokens
         gone = set(self.pages) - {int(r) for r in requests}
         for r in gone:

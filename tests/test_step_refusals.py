@@ -239,6 +239,9 @@ def test_trace_context_pages():
     assert b["tok_pos"] == [33, 33] and len(b["pages"][0]) == 2 and c.cache.free_pages == 12 - 2 - 4
     b = c.advance([9, 7], [2, 4])                     # 5 is gone, 7 came with another adapter
     assert b["req_prefix"] == [0, 1] and b["tok_pos"] == [34, 17] and b["pages"][1][1] == -1 and c.cache.free_pages == 12 - 4 - 2 - 1
+    for requests, adapters in (([9, 9], [2, 2]), ([9, 7], [2])):
+        with pytest.raises(ValueError, match="listed once"):
+            c.advance(requests, adapters)
     with pytest.raises(MemoryError):
         c.advance(range(20, 40), [2] * 20)
     steps = simulate([0.0, 0.0, 0.1], [1, 2, 3], [4, 2, 3])
