@@ -482,8 +482,8 @@ struct W4Form { int cols, rows, alone, base, each; };
 constexpr W4Form W4_FORMS[] = {{2, 16, 89, 34, 55}, {2, 32, 123, 20, 103}, {4, 32, 178, 30, 104}, {8, 32, 242, 30, 165}, {8, 64, 318, 20, 295}, {16, 64, 540, 20, 520}};
 
 // Up to 16 tokens: one column tile a workgroup while that makes one round of workgroups, two beyond (one token, 4096 -> 4096: 4.6 us against 5.7;
-// 4096 -> 22016: 15.9 against 13.2).  Beyond: the form of the least time by the table, which is the fastest at all of 21 sizes of 32 to 200 tokens but
-// four, there within 3 % (us, the forms in the table's order):
+// 4096 -> 22016: 15.9 against 13.2).  Beyond: the form of the least time by the table.  It is the fastest of the six at 73 of 76 sizes (20 to 256
+// tokens, 1024 to 14336 rows, 1024 to 28672 columns), at the others 0.1 to 0.4 us behind; some of them (us, the forms in the table's order):
 //     32 tokens,  4096 ->  4096      8.0    10.1    13.0    19.2    24.9    42.6
 //     64          4096 ->  4096     12.7    10.7    13.3    19.2    25.6    43.4
 //     32          5120 -> 15360     26.8    23.6    17.8    24.0    31.5    53.2
