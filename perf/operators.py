@@ -28,16 +28,12 @@ PROJS = {"q": [["q"]], "qkvo": [["q", "k", "v"], ["o"]], "all": [["q", "k", "v"]
 ROPE_BASE = 10000.0
 
 
-_package = []
-
-
 def _mlora():
-    """The package, imported on the first use: a program has it at hand."""
-    if not _package:
-        sys.path.insert(0, os.path.join(os.getcwd(), "ae-296_amd"))
-        import mlora
-        _package.append(mlora)
-    return _package[0]
+    folder = os.path.join(os.getcwd(), "ae-296_amd")
+    if folder not in sys.path:
+        sys.path.insert(0, folder)
+    import mlora
+    return mlora
 
 
 def listed():
