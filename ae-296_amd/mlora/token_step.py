@@ -53,7 +53,9 @@ class TokenStep:
         self._outgrown = []
 
     def begin(self, batch: KVBatch, tok_adapter: torch.Tensor) -> None:
-        """A step's batch: its tokens, pages and prefixes, and the adapter slot of every token (int32, negative: none)."""
+        """A step's batch: its tokens, pages and prefixes, and the adapter slot of every token (int32, negative: none).  After a batch that
+        was refused ``layer`` raises until the next ``begin``."""
+        self.batch = None            # until all of it is accepted: after a refusal the kept plans may be those of two batches
         if tok_adapter.numel() != batch.T:
             raise ValueError("tok_adapter must have one entry for every token of the batch")
         T, n_prefix = batch.T, 0 if batch.prefix_len is None else batch.prefix_len.numel()
@@ -64,15 +66,19 @@ class TokenStep:
                 new = dict(dtype=self.cache.dtype, device=self.cache.device)
                 self._buffers[room] = [torch.empty((room, w), **new) for w in self.widths] + [torch.zeros((room, self.n_q_heads, self.cache.head_dim), **new)]
             *qkv, out = (b[:T] for b in self._buffers[room])
-            kept = self._kept[T] = [ops.plan_decode(tok_adapter, self.pool, n_proj=3), None, qkv, out, -1]
-        else:
-            ops.plan_decode(tok_adapter, self.pool, out=kept[0])
+            kept = self._kept[T] = [None, None, qkv, out, -1]
         if n_prefix > kept[4]:            # room for twice as many, so that a growing number of prompts moves the plan a few times only
-            self._outgrown.append(kept[1])
-            kept[4] = n_prefix if kept[1] is None else min(2 * n_prefix, 4096)
-            kept[1] = plan_attention(batch, self.cache, self.n_q_heads, room=kept[4])
+            holds = n_prefix if kept[1] is None else min(2 * n_prefix, 4096)
+            plan = plan_attention(batch, self.cache, self.n_q_heads, room=holds)
+            if kept[1] is not None:
+                self._outgrown.append(kept[1])
+            kept[1], kept[4] = plan, holds        # only now: a batch that was refused must not count as room
         else:
             plan_attention(batch, self.cache, self.n_q_heads, out=kept[1])
+        if kept[0] is None:
+            kept[0] = ops.plan_decode(tok_adapter, self.pool, n_proj=3)
+        else:
+            ops.plan_decode(tok_adapter, self.pool, out=kept[0])
         self.decode_plan, self.attn_plan, self.qkv, self.out = kept[:4]
         self.batch, self.tok_adapter = batch, tok_adapter
 
