@@ -266,7 +266,7 @@ template <int D> struct KeyBlock {
 // What a wavefront holds of 16 query rows.
 template <int D> struct RowState {
     uint4 q[D / 32];
-    float m, l;                // of row lane % 16: the maximum, in powers of two, over all lanes; the sum of this lane's keys
+    float m, l;                // of row lane % 16: the maximum, in powers of two (fp16: less 14), over all lanes; the sum of this lane's keys
     float4_t acc[D / 16];      // out^T: columns 16 i + 4 g .. + 3 of row lane % 16
 };
 
@@ -367,13 +367,16 @@ struct Walk {
     __device__ __forceinline__ void sums(RowState<D> (&st)[NR], const float4_t (&s)[NR][2])
     {
         const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+        // fp16 has steps of 2^-24 below 2^-14, and a row's result may be made of many weights down there (8192 keys 16.2 below a few others: off by
+        // 3 % where these others' values are zero), so its largest weight is 2^14 instead of 1: the maximum is kept 14 lower.  bf16 has fp32's range.
+        constexpr float TOP = DT == DT_F16 ? 14.f : 0.f;
         uint4 wf[NR];
 #pragma unroll
         for (int n = 0; n < NR; n++) {
             float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])), fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            top *= scale2;
+            top = DT == DT_F16 ? fmaf(top, scale2, -TOP) : top * scale2;
             // A higher maximum in some row: what was summed so far shrinks.  Letting the sums stand until a maximum has grown by 2^8 takes 3 to
             // 5 % off the prefix items and nothing off the others, and costs the exact weight of 1 of a row's largest key (0.0022 of the
             // result's norm off the 64-bit result in bf16 instead of 0.0019).
@@ -390,14 +393,19 @@ struct Walk {
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) w[4 * h + i] = __builtin_amdgcn_exp2f(fmaf(s[n][h][i], scale2, -ref));
-            // The fused product is exact and the maximum is a rounded one: the largest key's weight is 2 to the power of that rounding, which the
-            // sum shares.  From scores of 2^24 on it is a power that a 16-bit weight does not hold, so there both are rounded.
+            // The fused product is exact and the maximum is a rounded one: the largest key's weight is 2 to the power of that rounding (and of TOP),
+            // which the sum shares.  From scores of 2^24 on it is a power that a 16-bit weight does not hold, so there both are rounded alike.
             if (__ballot(fabsf(ref) > 16777216.f)) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(__fsub_rn(__fmul_rn(s[n][i / 4][i % 4], scale2), ref));
+                for (int i = 0; i < 8; i++) {
+                    const float x = s[n][i / 4][i % 4];
+                    w[i] = __builtin_amdgcn_exp2f(DT == DT_F16 ? __fsub_rn(fmaf(x, scale2, -TOP), ref) + TOP : __fsub_rn(__fmul_rn(x, scale2), ref));
+                }
             }
             wf[n] = pack8<DT>(w);
-            // the sum takes the weights as rounded: a rounding that is in both sums moves their quotient less, and four instructions do it
+            // A matrix instruction takes weights of 16 bits (a second product with what the rounding left would be half as many again); a weight's
+            // rounding moves the result by a part of the result's own.  The sum takes the weights as rounded: a rounding that is in both sums moves
+            // their quotient less, and four instructions do it.
             const uint32_t one = DT == DT_F16 ? 0x3c003c00u : 0x3f803f80u;
             st[n].l = dot8<DT>(wf[n], make_uint4(one, one, one, one), st[n].l);
         }
