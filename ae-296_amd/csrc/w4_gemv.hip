@@ -5,6 +5,8 @@
 // 16.0 it reads 16 + c, exactly, in fp16 and in bf16 alike (two instructions for two codes).  The 16 and the zero point come off after the
 // products: with X = sum of x over the group, sum (c - z) x = sum (16 + c) x - (16 + z) X.  X is one more MFMA per K step whose weight operand is
 // ones, so it lands in the lanes that need it; products are exact in fp32 and the difference costs about two bits of its 24.
+// Where x is infinite, or so large that 16 x leaves fp32, the difference is infinity less infinity: a result that is not finite is computed again
+// from the formula itself (w4_again).
 #include "mlora_dev.hpp"
 #include "mlora_step.hpp"
 
@@ -105,6 +107,46 @@ __device__ __forceinline__ void w4_factors(float (*to)[64], int lane, uint32_t w
     const float f = lo_f32<DT>(word);
     to[0][lane] = f;
     to[1][lane] = -f * (float)(word >> 16);
+}
+
+__device__ __forceinline__ bool w4_finite(float v) { return fabsf(v) < INFINITY; }
+
+// Results of a wavefront that are not finite, from the formula in 64 bits, one after the other, the wavefront's lanes along k.  `mine`: a bit for
+// each such result of this lane; at(lane, bit, t, n): its token and column.  y holds there what is to be accumulated.  All 64 lanes come here.
+// 32 tokens, 11008 -> 4096: 17 us where all is finite, as without it; 227 with one infinite row.
+template <int DT, typename At>
+__device__ __forceinline__ void w4_again(const W4Proj &w, bool accumulate, uint32_t mine, At at)
+{
+    const int lane = threadIdx.x & 63;
+    const int per_tile = w.per_tile, group_shift = per_tile == 1 ? 7 : per_tile == 2 ? 6 : 5;
+    for (uint64_t lanes = __ballot(mine != 0); lanes; lanes = __ballot(mine != 0)) {
+        const int from = __builtin_ctzll(lanes), bit = __builtin_ctz(__builtin_amdgcn_readlane((int)mine, from));
+        int t, n;
+        at(from, bit, t, n);
+        const uint16_t *x = static_cast<const uint16_t *>(w.x) + (size_t)t * w.hin;
+        const unsigned char *groups = w.packed + w.groups_at;
+        double sum = 0.0;
+        for (int k = lane * 8; k < w.hin; k += 512) {
+            const size_t tile = (size_t)(n / W4_TN) * w.k_tiles + k / W4_TK;
+            const uint32_t code = *reinterpret_cast<const uint32_t *>(w.packed + tile * W4_TILE_BYTES + ((k >> 3 & 3) * 16 + n % W4_TN) * 16 + (k >> 5 & 3) * 4);
+            const size_t g = (tile * per_tile + ((k & (W4_TK - 1)) >> group_shift)) * W4_TN + n % W4_TN;
+            const uint32_t word = w.zeros ? reinterpret_cast<const uint32_t *>(groups)[g] : reinterpret_cast<const uint16_t *>(groups)[g] | 24u << 16;
+            const float scale = lo_f32<DT>(word);
+            const int zero = (int)(word >> 16) - 16;
+            float f[8];
+            unpack8<DT>(ldg16(x + k), f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) sum += (double)(scale * (float)((int)(code >> (4 * (j >> 1) + 16 * (j & 1)) & 15u) - zero)) * (double)f[j];
+        }
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        if (lane == from) {
+            uint16_t *y = static_cast<uint16_t *>(w.y) + (size_t)t * w.hout + n;
+            float v = (float)sum;
+            if (accumulate) v += lo_f32<DT>(*y);
+            *y = (uint16_t)pack2<DT>(v, 0.f);
+            mine &= mine - 1;
+        }
+    }
 }
 
 // The column block, token block and projection of a workgroup.  Eight neighbouring ids go to the eight XCDs: the token blocks of one
@@ -211,6 +253,7 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
             if (kt >= k_tiles) break;
         }
     }
+    uint32_t again = 0;                                           // bit 2 n + i: this lane's i-th result of column tile n
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         if (n) __syncthreads();
@@ -224,9 +267,20 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
 #pragma unroll
         for (int k = 0; k < W4_WAVES; k++) { v0 += part[k][r][col]; v1 += part[k][r][col + 1]; }
         uint32_t *y = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(w.y) + (size_t)(t0 + r) * w.hout + at);
-        if (p.accumulate) { v0 += lo_f32<DT>(*y); v1 += hi_f32<DT>(*y); }
+        const bool ok0 = w4_finite(v0), ok1 = w4_finite(v1);
+        again |= (ok0 ? 0u : 1u) << 2 * n | (ok1 ? 0u : 2u) << 2 * n;
+        if (p.accumulate) {                                       // what is computed again finds y as it was
+            const float y0 = lo_f32<DT>(*y), y1 = hi_f32<DT>(*y);
+            v0 = ok0 ? v0 + y0 : y0;
+            v1 = ok1 ? v1 + y1 : y1;
+        }
         *y = pack2<DT>(v0, v1);
     }
+    w4_again<DT>(w, p.accumulate, again, [&](int from, int bit, int &t, int &n) {
+        const int thread = wave * 64 + from;
+        t = t0 + (thread >> 3);
+        n = (nt0 + (bit >> 1)) * W4_TN + (thread & 7) * 2 + (bit & 1);
+    });
 }
 
 // ------------------------------------------------------------------ product, more tokens
@@ -411,6 +465,8 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
     __builtin_amdgcn_s_waitcnt(0);                                // loads to the ring may still be on their way
     // the parts' sums, one column tile of each wavefront at a time
     float (*part)[MT * 16][17] = reinterpret_cast<float (*)[MT * 16][17]>(lds);
+    static_assert(MT * NT * 4 <= 32, "a bit for each of a lane's results");
+    uint32_t again = 0;                                           // bit 4 (n MT + m) + i: this lane's i-th result of column tile n and token tile m
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         if constexpr (WK > 1) {
@@ -437,13 +493,23 @@ __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args 
             if (r >= p.T || col >= w.hout) continue;
             uint2 *y = reinterpret_cast<uint2 *>(static_cast<uint16_t *>(w.y) + (size_t)r * w.hout + col);
             float4_t v = out[m][n];
-            if (p.accumulate) {
-                const uint2 old = *y;
-                v += float4_t{lo_f32<DT>(old.x), hi_f32<DT>(old.x), lo_f32<DT>(old.y), hi_f32<DT>(old.y)};
+            uint32_t bad = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) bad |= (w4_finite(v[i]) ? 0u : 1u) << i;
+            again |= bad << 4 * (n * MT + m);
+            if (p.accumulate) {                                   // what is computed again finds y as it was
+                const uint2 word = *y;
+                const float4_t old = {lo_f32<DT>(word.x), hi_f32<DT>(word.x), lo_f32<DT>(word.y), hi_f32<DT>(word.y)};
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = bad >> i & 1 ? old[i] : v[i] + old[i];
             }
             *y = make_uint2(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
         }
     }
+    w4_again<DT>(w, p.accumulate, again, [&](int from, int bit, int &t, int &n) {
+        t = t0 + (bit / 4 % MT) * 16 + (from & 15);
+        n = (nt0 + bit / 4 / MT) * W4_TN + (from >> 4) * 4 + (bit & 3);
+    });
 }
 
 // ------------------------------------------------------------------ launches

@@ -3,7 +3,8 @@ decode batch, whose LoRA deltas ``bgmv`` adds.
 
     y[t, n] = sum_g scales[g, n] * sum_{k in group g} (codes[k, n] - zeros[g, n]) * x[t, k]
 
-with a scale (and optionally a zero point, 8 otherwise) for every `group` rows of a column.  Launches go to
+with a scale (and optionally a zero point, 8 otherwise) for every `group` rows of a column.  A row with an infinite or NaN x gives what the
+formula gives, but takes longer (32 tokens, 11008 -> 4096: 17 us, 230 with one such row): rows of x that nobody reads should hold numbers.  Launches go to
 ``torch.cuda.current_stream()`` and do not synchronise.
 """
 from __future__ import annotations

@@ -434,7 +434,8 @@ int mlora_prefill_reflayout(void *y, const void *x, const void *A_T, const void 
  *     y_p[t][n] = (accumulate ? y_p[t][n] : 0) + sum_g s_p[g][n] * sum_{k in group g} (c_p[k][n] - z_p[g][n]) * x_p[t][k]
  * with codes c in 0..15, a 16-bit scale for every `group` (32, 64 or 128) rows of a column and a zero point z in 0..15 (8
  * where none are given).  hin and hout are multiples of 8; the last group of a column may be shorter.  Products and sums in
- * fp32, rounded once.
+ * fp32, rounded once; a result that is not finite so (an infinite or NaN x, a bf16 x from about 10^37 on) is computed again in 64 bits from the
+ * formula, which takes longer (32 tokens, 11008 -> 4096: 17 us, 230 with one such row): rows of x that nobody reads should hold numbers.
  *   mlora_w4_pack lays codes (uint8 [hin, hout], one code a byte, the low four bits count), scales ([groups, hout], of the type
  *     the calls will use) and zeros (uint8 [groups, hout], or NULL) out as the kernel reads them: mlora_w4_packed_bytes(...)
  *     bytes, 16-byte aligned, once per weight; the sources are not needed afterwards.
