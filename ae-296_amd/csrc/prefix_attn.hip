@@ -280,6 +280,7 @@ struct Walk {
     float scale2;
     int n_listed, first, last, head;
     int window, ids;                   // 64 pages from page `window` on; -1: none yet
+    int seen;                          // 0 until there was a key
 
     // Pages of the sixteens of keys from key0 on, -1 for those that are absent; bit i of the result: the i-th has one.
     template <int N>
@@ -300,6 +301,7 @@ struct Walk {
             page[i] = __builtin_amdgcn_readlane(ids, ((key0 + 16 * i) >> p.page_shift) - window);
             have |= key0 + 16 * i < last && page[i] >= 0 ? 1 << i : 0;
         }
+        seen |= have;
         return have;
     }
 
@@ -457,6 +459,11 @@ struct Walk {
     }
 };
 
+// A part's maximum as it is handed on.  Where there were keys it is finite even if their scores are all minus infinity, so a row without a maximum
+// has no key.  Such scores have no weight beside others; alone they leave a sum of zero, and the softmax is 0 / 0.
+__device__ __forceinline__ float pa_top(float m, int seen) { return seen ? fmaxf(m, -3.402823466e38f) : m; }
+__device__ __forceinline__ float pa_inverse(float m, float l) { return m == -INFINITY && l == 0.f ? 0.f : l == 0.f ? NAN : 1.f / l; }
+
 constexpr int pa_pitch(int D) { return D + 4; }            // floats of a row in the LDS exchange: a float4 of 16 rows meets all banks
 
 // Scale and q as the walk takes them: the scale in powers of two, positive (a maximum of scores is one of scaled scores then, and a masked
@@ -496,10 +503,11 @@ __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const_i32_ptr 
     const int mine = first + wave * share;
     const int listed = e[5] ? p.b.max_prefix_pages : p.b.max_pages;
     Walk<DT, D> walk{p, (e[5] ? p.b.prefix_tbl : p.b.page_tbl) + (size_t)e[4] * listed, lds + wave * (PA_KEYS * D * 2), pa_scale2(p.scale),
-                     listed, mine, min(mine + share, last), head, -1, -1};
+                     listed, mine, min(mine + share, last), head, -1, -1, 0};
     walk.template all<NR, STREAM>(st);
 #pragma unroll
     for (int n = 0; n < NR; n++) {
+        st[n].m = pa_top(st[n].m, walk.seen);
         float l = st[n].l;
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
@@ -533,7 +541,7 @@ __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const_i32_ptr 
         }
         const int row = row0 + n * 16 + r, idx = row / p.gq, sub = row - idx * p.gq;
         if (slot < 0) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = pa_inverse(m, l);
             uint16_t *out = p.out + token_of(idx) * p.out_stride + ((size_t)head * p.gq + sub) * D + col;
 #pragma unroll
             for (int k = 0; k < E; k += 4) *reinterpret_cast<uint2 *>(out + k) = make_uint2(pack2<DT>(v[k] * inv, v[k + 1] * inv), pack2<DT>(v[k + 2] * inv, v[k + 3] * inv));
@@ -574,7 +582,7 @@ __device__ __forceinline__ void pa_wide(const AttnKernelArgs &ka, const_i32_ptr 
         for (int d = 0; d < D / 16; d++) st[n].acc[d] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
     const int listed = p.b.max_prefix_pages;
-    Walk<DT, D> walk{p, p.b.prefix_tbl + (size_t)e[4] * listed, nullptr, pa_scale2(p.scale), listed, e[6], last, head, -1, -1};
+    Walk<DT, D> walk{p, p.b.prefix_tbl + (size_t)e[4] * listed, nullptr, pa_scale2(p.scale), listed, e[6], last, head, -1, -1, 0};
     uint4 kr[PER], vr[PER];
     const unsigned mine = (lane / CH) * D + (lane % CH) * 8;
     int have, have_next;                                   // sixteens of the tile at hand, and of the one on its way, that have a page
@@ -659,7 +667,7 @@ __device__ __forceinline__ void pa_wide(const AttnKernelArgs &ka, const_i32_ptr 
         const size_t at = ((size_t)(slot + idx) * p.n_kv_heads + head) * p.gq + sub;
 #pragma unroll
         for (int d = 0; d < D / 16; d++) *reinterpret_cast<float4_t *>(ka.parts + at * D + d * 16 + g * 4) = st[n].acc[d];
-        if (g == 0) *reinterpret_cast<float2 *>(ka.parts + (size_t)ka.slots_cap * p.n_q_heads * D + at * 2) = make_float2(st[n].m, l);
+        if (g == 0) *reinterpret_cast<float2 *>(ka.parts + (size_t)ka.slots_cap * p.n_q_heads * D + at * 2) = make_float2(pa_top(st[n].m, walk.seen), l);
     }
 }
 
@@ -736,9 +744,10 @@ __global__ __launch_bounds__(256) void pa_join_kernel(const AttnKernelArgs ka)
             for (int k = 0; k < E; k++) v[k] += s_v[slice + q][col + k] * f;
         }
         l = all;
+        m = top;
     }
     if (row >= p.n_q_heads) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = pa_inverse(m, l);
     uint16_t *out = p.out + t * p.out_stride + (size_t)row * D + col;
 #pragma unroll
     for (int k = 0; k < E; k += 4) *reinterpret_cast<uint2 *>(out + k) = make_uint2(pack2<DT>(v[k] * inv, v[k + 1] * inv), pack2<DT>(v[k + 2] * inv, v[k + 3] * inv));

@@ -482,8 +482,8 @@ int mlora_kv_append(const void *q, int64_t q_stride, void *q_out, int64_t q_out_
  *     out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j,  j over positions 0 .. tok_pos[t] of t's request,
  * query head h reading key head h / (n_q_heads / n_kv_heads).  Scores, softmax statistics and sums in fp32; the softmax weights are
  * rounded to the 16-bit type for their product with v; the result is rounded once.  Keys on page ids outside [0, n_pages), or on pages
- * behind a table's end, count as absent; a row that sees no key at all is zeros; what lies on a page behind the last position
- * is never used, whatever it holds.  Made for one new token per request; several tokens of one request are computed rightly,
+ * behind a table's end, count as absent; a row that sees no key at all is zeros, one whose scores are all minus infinity is NaN; what
+ * lies on a page behind the last position is never used, whatever it holds.  Made for one new token per request; several tokens of one request are computed rightly,
  * their own keys read once for each.
  *   mlora_attn_plan divides the step's work: once per step, for every layer, into `plan` (mlora_attn_plan_bytes bytes).
  *   mlora_prefix_attention runs one layer against it; q and out as in mlora_kv_append (they must not overlap); workspace:

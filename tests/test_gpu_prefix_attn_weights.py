@@ -1,4 +1,4 @@
-"""Rows whose result is made of small softmax weights."""
+"""Rows whose result is made of small softmax weights, and keys whose scores are infinite."""
 import numpy as np
 import pytest
 import torch
@@ -8,7 +8,8 @@ from gpu_common import say
 from step_ref import HALF, TINY, U32, check, f64, store_bound
 
 pytestmark = pytest.mark.gpu
-F16 = torch.float16
+F16, BF16 = torch.float16, torch.bfloat16
+INF = float("inf")
 
 
 def i32(a):
@@ -86,3 +87,34 @@ def test_many_small_weights(heads, kv, own, behind, D):
             rel = 2 * np.expm1(8 * U32 * 16.5 * 1.4427) + 2 * 2.0 ** -22 + 2 * HALF[F16] / (1 - HALF[F16]) + 2 * (n + 80) * U32
             bound = rel * want + 2 * n * TINY[F16] * 2.0 ** -14 * np.abs(v).max(0) / l
             check(out[t, h], want, bound + store_bound(want + bound, F16), f"token {t} head {h}")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads, kv, own, behind", LAYOUTS + [(4, 2, 2, 0), (4, 2, 0, 6), (2, 1, 1, 80)])
+def test_rows_whose_scores_are_all_minus_infinity(heads, kv, own, behind, dtype):
+    """The softmax of nothing but minus infinities is NaN; one finite score among them has the whole weight, wherever it lies."""
+    say(f"attention minus infinity heads {heads}/{kv} own {own} behind {behind} {dtype}")
+    n = 700
+    s = Scores(np.full(n, -INF), heads, kv, 64, dtype, own, behind)
+    assert s.run().isnan().all()
+    for at in (0, 333, n - 1):
+        s.cache.k[0, at // 64, :, at % 64, 0] = 2.0
+        out = s.run()
+        for h in (0, heads - 1):
+            want = torch.from_numpy(s.values(h)[at]).to(dtype).cuda()
+            assert (out[:, h] == want).all()
+        s.cache.k[0, at // 64, :, at % 64, 0] = -INF
+
+
+def test_absent_keys_are_not_infinite_ones():
+    """Every page missing: no key at all, and zeros.  One page there, and its scores minus infinity: NaN."""
+    s = Scores(np.full(200, -INF), 4, 2, 64, F16, 2, 3)
+    s.batch.pages.fill_(-1)
+    s.batch.prefix_pages.fill_(-1)
+    assert (s.run() == 0).all()
+    s.batch.pages[1, 2] = 1
+    out = s.run()
+    assert out[1].isnan().all() and (out[0] == 0).all() and (out[2:] == 0).all()
+    s.batch.prefix_pages[0, 3] = 0
+    out = s.run()
+    assert out[1:].isnan().all() and (out[0] == 0).all()
