@@ -266,7 +266,7 @@ template <int D> struct KeyBlock {
 // What a wavefront holds of 16 query rows.
 template <int D> struct RowState {
     uint4 q[D / 32];
-    float m, l;                // of row lane % 16: the maximum, in powers of two (fp16: less 14), over all lanes; the sum of this lane's keys
+    float m, l;                // of row lane % 16: the maximum score, unscaled, over all lanes; the sum of this lane's keys
     float4_t acc[D / 16];      // out^T: columns 16 i + 4 g .. + 3 of row lane % 16
 };
 
@@ -370,7 +370,7 @@ struct Walk {
     {
         const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
         // fp16 has steps of 2^-24 below 2^-14, and a row's result may be made of many weights down there (8192 keys 16.2 below a few others: off by
-        // 3 % where these others' values are zero), so its largest weight is 2^14 instead of 1: the maximum is kept 14 lower.  bf16 has fp32's range.
+        // 3 % where these others' values are zero), so its largest weight is 2^14 instead of 1.  bf16 has fp32's range.
         constexpr float TOP = DT == DT_F16 ? 14.f : 0.f;
         uint4 wf[NR];
 #pragma unroll
@@ -378,31 +378,24 @@ struct Walk {
             float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])), fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            top = DT == DT_F16 ? fmaf(top, scale2, -TOP) : top * scale2;
             // A higher maximum in some row: what was summed so far shrinks.  Letting the sums stand until a maximum has grown by 2^8 takes 3 to
             // 5 % off the prefix items and nothing off the others, and costs the exact weight of 1 of a row's largest key (0.0022 of the
             // result's norm off the 64-bit result in bf16 instead of 0.0019).
             if (__ballot(top > st[n].m)) {
-                const float m = fmaxf(st[n].m, top), keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[n].m - m);
+                const float m = fmaxf(st[n].m, top), keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st[n].m - m) * scale2);
                 st[n].l *= keep;
 #pragma unroll
                 for (int d = 0; d < DTILES; d++) st[n].acc[d] *= keep;
                 st[n].m = m;
             }
             const float ref = st[n].m == -INFINITY ? 0.f : st[n].m;
+            // The maximum comes off before the scaling, or the largest key's weight would be 2 to the power of a rounding of its scaled score:
+            // nothing or infinity from 2^24 on.  The parts are joined so, too (128 requests behind one prefix of 8191, two layers: 175.7 us, scaled first 172.4).
             float w[8];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[4 * h + i] = __builtin_amdgcn_exp2f(fmaf(s[n][h][i], scale2, -ref));
-            // The fused product is exact and the maximum is a rounded one: the largest key's weight is 2 to the power of that rounding (and of TOP),
-            // which the sum shares.  From scores of 2^24 on it is a power that a 16-bit weight does not hold, so there both are rounded alike.
-            if (__ballot(fabsf(ref) > 16777216.f)) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float x = s[n][i / 4][i % 4];
-                    w[i] = __builtin_amdgcn_exp2f(DT == DT_F16 ? __fsub_rn(fmaf(x, scale2, -TOP), ref) + TOP : __fsub_rn(__fmul_rn(x, scale2), ref));
-                }
+            for (int i = 0; i < 8; i++) {
+                const float x = s[n][i / 4][i % 4] - ref;
+                w[i] = __builtin_amdgcn_exp2f(DT == DT_F16 ? fmaf(x, scale2, TOP) : x * scale2);
             }
             wf[n] = pack8<DT>(w);
             // A matrix instruction takes weights of 16 bits (a second product with what the rounding left would be half as many again); a weight's
@@ -517,7 +510,7 @@ __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const_i32_ptr 
         float m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < PA_WAVES; w++) m = fmaxf(m, s_m[w][c]);
-        const float f = st[n].m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[n].m - m);
+        const float f = st[n].m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st[n].m - m) * walk.scale2);
         float *part = reinterpret_cast<float *>(lds) + (wave * 16 + c) * PITCH;
 #pragma unroll
         for (int d = 0; d < D / 16; d++) *reinterpret_cast<float4_t *>(part + d * 16 + g * 4) = st[n].acc[d] * f;
@@ -529,7 +522,7 @@ __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const_i32_ptr 
 #pragma unroll
         for (int w = 0; w < PA_WAVES; w++) m = fmaxf(m, s_m[w][r]);
 #pragma unroll
-        for (int w = 0; w < PA_WAVES; w++) l += s_l[w][r] * (s_m[w][r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w][r] - m));
+        for (int w = 0; w < PA_WAVES; w++) l += s_l[w][r] * (s_m[w][r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((s_m[w][r] - m) * walk.scale2));
         float v[E];
 #pragma unroll
         for (int k = 0; k < E; k += 4) {
@@ -706,6 +699,7 @@ __global__ __launch_bounds__(256) void pa_join_kernel(const AttnKernelArgs ka)
     if (own == 1 && shared == 0) return;                         // written by its only item
     const int slice = threadIdx.x >> 4, col = (threadIdx.x & 15) * E, part0 = slice % G;
     const int row = blockIdx.y * ROWS + slice / G;               // query head
+    const float scale2 = pa_scale2(p.scale);
     float m = -INFINITY, l = 0.f, v[E] = {};
     if (row < p.n_q_heads) {
         const float *ml = ka.parts + (size_t)ka.slots_cap * p.n_q_heads * D;
@@ -715,7 +709,7 @@ __global__ __launch_bounds__(256) void pa_join_kernel(const AttnKernelArgs ka)
             const size_t at = (size_t)slot * p.n_q_heads + row;
             const float2 x = *reinterpret_cast<const float2 *>(ml + at * 2);
             if (x.x == -INFINITY && x.y == 0.f) continue;       // no keys; scores that are all NaN leave no maximum, but a sum that is NaN
-            const float top = fmaxf(m, x.x), a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), b = __builtin_amdgcn_exp2f(x.x - top);
+            const float top = fmaxf(m, x.x), a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * scale2), b = __builtin_amdgcn_exp2f((x.x - top) * scale2);
             m = top;
             l = l * a + x.y * b;
 #pragma unroll
@@ -738,7 +732,7 @@ __global__ __launch_bounds__(256) void pa_join_kernel(const AttnKernelArgs ka)
 #pragma unroll
         for (int k = 0; k < E; k++) v[k] = 0.f;
         for (int q = 0; q < G; q++) {
-            const float f = s_m[slice + q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[slice + q] - top);
+            const float f = s_m[slice + q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((s_m[slice + q] - top) * scale2);
             all += s_l[slice + q] * f;
 #pragma unroll
             for (int k = 0; k < E; k++) v[k] += s_v[slice + q][col + k] * f;
