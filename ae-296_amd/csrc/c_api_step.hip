@@ -240,7 +240,9 @@ int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t
     if (rc) return rc;
     if (T == 0) return MLORA_OK;
     if ((rc = check_prefix(req_prefix, prefix_len, n_prefix))) return rc;
-    if (!(fabsf(scale) <= 3.4e38f)) return fail(MLORA_EINVAL, "scale must be finite");
+    if (!std::isfinite(scale)) return fail(MLORA_EINVAL, "scale must be finite");
+    // it is applied in powers of two: times 1.44 it has to be a normal number still
+    if (scale != 0.f && (fabsf(scale) < 0x1p-126f || fabsf(scale) > 0x1p127f)) return fail(MLORA_ERANGE, "scale must be 0 or between 2^-126 and 2^127 (got %g)", scale);
     if (n_prefix > 0 && !prefix_tbl) return fail(MLORA_EINVAL, "prefix_tbl is needed with n_prefix > 0");
     if (n_prefix > 0 && (rc = check_table("max_prefix_pages", max_prefix_pages, page_tokens))) return rc;
     if (!out || !q || !k_pages || !v_pages || !plan) return fail(MLORA_EINVAL, "out, q, k_pages, v_pages and plan must not be NULL");

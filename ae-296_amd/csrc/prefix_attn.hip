@@ -460,13 +460,13 @@ __device__ __forceinline__ float pa_inverse(float m, float l) { return m == -INF
 constexpr int pa_pitch(int D) { return D + 4; }            // floats of a row in the LDS exchange: a float4 of 16 rows meets all banks
 
 // Scale and q as the walk takes them: the scale in powers of two, positive (a maximum of scores is one of scaled scores then, and a masked
-// score stays minus infinity), its sign in q.
-__device__ __forceinline__ float pa_scale2(float scale) { return fmaxf(fabsf(scale) * PA_LOG2E, 1e-30f); }
+// score stays minus infinity), its sign in q; a scale of zero as zeros for q.
+__device__ __forceinline__ float pa_scale2(float scale) { return scale == 0.f ? 1.f : fabsf(scale) * PA_LOG2E; }
 __device__ __forceinline__ uint4 pa_load_q(const uint16_t *q, float scale)
 {
-    const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
+    const uint32_t flip = scale < 0.f ? 0x80008000u : 0u, keep = scale == 0.f ? 0u : ~0u;
     const uint4 v = ldg16(q);
-    return make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+    return make_uint4((v.x ^ flip) & keep, (v.y ^ flip) & keep, (v.z ^ flip) & keep, (v.w ^ flip) & keep);
 }
 
 // One item for one key head: NR tiles of 16 query rows, the keys shared by the four wavefronts and joined in LDS.  Bound by HBM on

@@ -149,7 +149,7 @@ def plan_attention(batch: KVBatch, cache: KVCache, n_q_heads: int, out: Optional
 def prefix_attention(q: torch.Tensor, cache: KVCache, layer: int, plan: AttnPlan, scale: Optional[float] = None,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[t, h] = softmax(scale * q[t, h] . K) V over positions 0 .. tok_pos[t] of token t's request, its prefix's among them;
-    q and out [T, Hq, D] (rows may be apart), scale 1 / sqrt(D) by default.  A row that sees no key is zeros (one whose
+    q and out [T, Hq, D] (rows may be apart), scale 1 / sqrt(D) by default (0, or 2^-126 to 2^127 of either sign).  A row that sees no key is zeros (one whose
     scores are all minus infinity is NaN, as the softmax is); rows without a request keep what `out` held (zeros in a new one)."""
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)

@@ -488,7 +488,8 @@ int mlora_kv_append(const void *q, int64_t q_stride, void *q_out, int64_t q_out_
  *   mlora_attn_plan divides the step's work: once per step, for every layer, into `plan` (mlora_attn_plan_bytes bytes).
  *   mlora_prefix_attention runs one layer against it; q and out as in mlora_kv_append (they must not overlap); workspace:
  *   mlora_attn_workspace_bytes bytes of fp32 partial results.  Calls that share a workspace, or write a plan that another
- *   reads, must be ordered on one stream.  The tables must be the ones the plan was made from.  scale: any finite value.
+ *   reads, must be ordered on one stream.  The tables must be the ones the plan was made from.  scale: 0, or
+ *   2^-126 to 2^127 of either sign.
  * T <= MLORA_ATTN_MAX_T, n_prefix <= MLORA_ATTN_MAX_PREFIX.
  */
 #define MLORA_ATTN_MAX_T 8192

@@ -1,11 +1,11 @@
-"""Rows whose result is made of small softmax weights, and keys whose scores are infinite."""
+"""Rows whose result is made of small softmax weights, keys whose scores are infinite, and scales at the ends of their range."""
 import numpy as np
 import pytest
 import torch
 
 import mlora
 from gpu_common import say
-from step_ref import HALF, TINY, U32, check, f64, store_bound
+from step_ref import HALF, TINY, U32, Scene, check, f64, store_bound
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -118,3 +118,29 @@ def test_absent_keys_are_not_infinite_ones():
     s.batch.prefix_pages[0, 3] = 0
     out = s.run()
     assert out[1:].isnan().all() and (out[0] == 0).all()
+
+
+@pytest.mark.parametrize("n_req", [3, 70])
+def test_scales_at_the_ends_of_their_range(n_req):
+    """A scale of zero gives every key the same weight however far the scores are apart; one near the smallest float meets scores that make up for
+    it; 2^127 leaves the largest score the whole weight."""
+    say(f"attention scales {n_req}")
+    s = Scene([(0, 9 + i) for i in range(n_req)], [150], 2, 1, 64, 16, BF16, seed=n_req)
+    s.k = (s.k.double() * 2.0 ** 60).to(BF16)
+    s.cache.k.copy_(s.k)
+    s.q = (s.q.double() * 2.0 ** 55).to(BF16)
+    s.dev_q = s.q.cuda()
+    plan = mlora.plan_attention(s.batch, s.cache, 2)
+    for scale in (0.0, 2.0 ** -118, -2.0 ** -118):
+        s.compare(mlora.prefix_attention(s.dev_q, s.cache, 0, plan, scale=scale), scale=scale, what=f"scale {scale}")
+    s.q, s.k = (s.q.double() * 2.0 ** -65).to(BF16), (s.k.double() * 2.0 ** -60).to(BF16)
+    s.dev_q = s.q.cuda()
+    s.cache.k.copy_(s.k)
+    out = f64(mlora.prefix_attention(s.dev_q, s.cache, 0, plan, scale=2.0 ** 127))
+    for t in range(n_req):
+        k, v = (np.concatenate([s.rows(w, 0, s.prefix_lists[0], 150, 0), s.rows(w, 0, s.req_lists[t], 9 + t, 0)]) for w in "kv")
+        for h in range(2):
+            score = k @ f64(s.q[t, h])
+            second, first = np.sort(score)[-2:]
+            if first - second > 1e-4 * np.abs(score).max():      # or fp32 may not tell the two apart
+                assert (out[t, h] == v[score.argmax()]).all()
