@@ -95,6 +95,6 @@ class TokenStep:
         ops.bgmv(ys, [x] * 3, self.pool, layer, self.names, self.tok_adapter, plan=self.decode_plan,
                  accumulate=qkv is not None or self.weights is not None)
         D, T = self.cache.head_dim, self.batch.T
-        q, k, v = (y.view(T, -1, D) for y in ys)
+        q, k, v = (y.view(T, w // D, D) for y, w in zip(ys, self.widths))
         kv_append(q, k, v, self.cache, layer, self.batch, self.rope)
         return prefix_attention(q, self.cache, layer, self.attn_plan, scale=scale, out=self.out)

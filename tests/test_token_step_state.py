@@ -118,3 +118,9 @@ def test_a_batch_and_adapters_of_unlike_length(step):
     with pytest.raises(RuntimeError, match="begin"):
         step.layer(0, torch.zeros((3, 64), dtype=torch.float16))
     runs(step, batch(4), adapters(4))
+
+
+def test_a_batch_without_tokens(step):
+    runs(step, batch(0), adapters(0))
+    runs(step, batch(2), adapters(2))
+    runs(step, batch(0), adapters(0))
