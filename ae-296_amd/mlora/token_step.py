@@ -64,7 +64,7 @@ class TokenStep:
             room = max(1, 1 << (T - 1).bit_length()) if T else 1
             if room not in self._buffers:
                 new = dict(dtype=self.cache.dtype, device=self.cache.device)
-                self._buffers[room] = [torch.empty((room, w), **new) for w in self.widths] + [torch.zeros((room, self.n_q_heads, self.cache.head_dim), **new)]
+                self._buffers[room] = [torch.empty((room, w), **new) for w in self.widths] + [torch.empty((room, self.n_q_heads, self.cache.head_dim), **new)]
             *qkv, out = (b[:T] for b in self._buffers[room])
             kept = self._kept[T] = [None, None, qkv, out, -1]
         if n_prefix > kept[4]:            # room for twice as many, so that a growing number of prompts moves the plan a few times only
@@ -79,12 +79,13 @@ class TokenStep:
             kept[0] = ops.plan_decode(tok_adapter, self.pool, n_proj=3)
         else:
             ops.plan_decode(tok_adapter, self.pool, out=kept[0])
+        kept[3].zero_()              # rows without a request: the attention leaves them alone, and other batches share the buffer
         self.decode_plan, self.attn_plan, self.qkv, self.out = kept[:4]
         self.batch, self.tok_adapter = batch, tok_adapter
 
     def layer(self, layer: int, x: torch.Tensor, qkv: Optional[Sequence[torch.Tensor]] = None, scale: Optional[float] = None) -> torch.Tensor:
         """Attention output [T, Hq, D] of one layer for its input x [T, hin]; the buffer is the step's own and holds it until the next
-        call.  q, k and v are left in `self.qkv` (or `qkv`), q rotated."""
+        call; rows without a request are zeros.  q, k and v are left in `self.qkv` (or `qkv`), q rotated."""
         if self.batch is None:
             raise RuntimeError("begin() names the step's batch first")
         if qkv is not None and self.weights is not None:

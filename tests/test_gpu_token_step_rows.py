@@ -17,3 +17,34 @@ def test_a_batch_without_tokens(scene):  # noqa: F811
         step.begin(mlora.KVBatch(e, e, i32([[0]])), e)
         assert step.layer(0, torch.empty((0, 128), device="cuda", dtype=torch.float16)).shape == (0, 4, 64)
         runs_as_alone(step, scene, batch(3, 2), i32([0, -1, 2]), "after a batch without tokens")
+
+
+def test_rows_without_a_request_are_zeros(scene):  # noqa: F811
+    """Whatever batch of a size up to the same power of two ran before, and captured as well."""
+    say("token step: rows without a request")
+    step = scene()
+    x = torch.randn((4, 128), device="cuda").half()
+    step.begin(batch(4, 2), i32([0, 1, 2, 0]))
+    assert (step.layer(0, x) != 0).any(-1).all()
+    for T, gone in ((4, 2), (3, 0), (4, 3)):
+        b = batch(T, 1)
+        b.tok_req[gone] = -1
+        step.begin(b, i32([0] * T))
+        out = step.layer(0, x[:T])
+        assert (out[gone] == 0).all() and (out[[t for t in range(T) if t != gone]] != 0).any(-1).all()
+    full = batch(4, 2)
+    step.begin(full, i32([0, 1, 2, 0]))
+    step.layer(0, x)
+    torch.cuda.synchronize()
+    b, slots = batch(4, 1), i32([1, 1, 0, 2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.begin(b, slots)
+        out = step.layer(0, x)
+    for gone in (1, 3, 0):
+        step.begin(full, i32([0, 1, 2, 0]))
+        step.layer(0, x)
+        b.tok_req.copy_(i32([-1 if t == gone else t for t in range(4)]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out[gone] == 0).all() and (out[[t for t in range(4) if t != gone]] != 0).any(-1).all()

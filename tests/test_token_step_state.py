@@ -124,3 +124,13 @@ def test_a_batch_without_tokens(step):
     runs(step, batch(0), adapters(0))
     runs(step, batch(2), adapters(2))
     runs(step, batch(0), adapters(0))
+
+
+def test_rows_without_a_request_hold_nothing_of_earlier_batches(step):
+    """Batches of three and four tokens share a buffer; what a row without a request holds of it is zeros."""
+    step.begin(batch(4), adapters(4))
+    step.out.fill_(5.0)
+    for T in (3, 4, 4):
+        step.begin(batch(T), adapters(T))
+        assert (step.out == 0).all()
+        step.out.fill_(5.0)
