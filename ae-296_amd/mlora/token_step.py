@@ -51,6 +51,7 @@ class TokenStep:
         # using them.  Buffers for every size would add up: to 4 GB over the sizes to 512, with four rows of 8 KB a token.
         self._kept, self._buffers = {}, {}
         self._outgrown = []
+        self.bad = torch.zeros(1, dtype=torch.int32, device=cache.device)      # tokens that kv_append left out since begin, added up over the layers
 
     def begin(self, batch: KVBatch, tok_adapter: torch.Tensor) -> None:
         """A step's batch: its tokens, pages and prefixes, and the adapter slot of every token (int32, negative: none).  After a batch that
@@ -79,13 +80,15 @@ class TokenStep:
             kept[0] = ops.plan_decode(tok_adapter, self.pool, n_proj=3)
         else:
             ops.plan_decode(tok_adapter, self.pool, out=kept[0])
+        self.bad.zero_()
         kept[3].zero_()              # rows without a request: the attention leaves them alone, and other batches share the buffer
         self.decode_plan, self.attn_plan, self.qkv, self.out = kept[:4]
         self.batch, self.tok_adapter = batch, tok_adapter
 
     def layer(self, layer: int, x: torch.Tensor, qkv: Optional[Sequence[torch.Tensor]] = None, scale: Optional[float] = None) -> torch.Tensor:
         """Attention output [T, Hq, D] of one layer for its input x [T, hin]; the buffer is the step's own and holds it until the next
-        call; rows without a request are zeros.  q, k and v are left in `self.qkv` (or `qkv`), q rotated."""
+        call; rows without a request are zeros.  q, k and v are left in `self.qkv` (or `qkv`), q rotated.  A token whose page or position no table
+        holds is counted in `self.bad` (int32, on the device; every layer counts it again): its key is missing and its q not rotated."""
         if self.batch is None:
             raise RuntimeError("begin() names the step's batch first")
         if qkv is not None and self.weights is not None:
@@ -97,5 +100,5 @@ class TokenStep:
                  accumulate=qkv is not None or self.weights is not None)
         D, T = self.cache.head_dim, self.batch.T
         q, k, v = (y.view(T, w // D, D) for y, w in zip(ys, self.widths))
-        kv_append(q, k, v, self.cache, layer, self.batch, self.rope)
+        kv_append(q, k, v, self.cache, layer, self.batch, self.rope, bad=self.bad)
         return prefix_attention(q, self.cache, layer, self.attn_plan, scale=scale, out=self.out)

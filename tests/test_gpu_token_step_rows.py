@@ -48,3 +48,28 @@ def test_rows_without_a_request_are_zeros(scene):  # noqa: F811
         graph.replay()
         torch.cuda.synchronize()
         assert (out[gone] == 0).all() and (out[[t for t in range(4) if t != gone]] != 0).any(-1).all()
+
+
+def test_tokens_that_no_page_holds_are_counted(scene):  # noqa: F811
+    say("token step: missing pages")
+    step = scene()
+    x = torch.randn((4, 128), device="cuda").half()
+    for missing in (1, 3, 0):
+        b = batch(4, 1)
+        b.pages[:missing] = -1
+        b.tok_req[3] = -1                                      # a row without a request is not missing anything
+        step.begin(b, i32([0] * 4))
+        assert int(step.bad) == 0
+        for _ in range(2):
+            step.layer(0, x)
+        assert int(step.bad) == 2 * missing
+    slots = i32([0] * 4)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.begin(b, slots)
+        step.layer(0, x)
+    for missing in (2, 0, 1):
+        b.pages.copy_(i32([[-1 if t < missing else t] for t in range(4)]))
+        graph.replay()
+        assert int(step.bad) == missing

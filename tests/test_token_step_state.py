@@ -134,3 +134,14 @@ def test_rows_without_a_request_hold_nothing_of_earlier_batches(step):
         step.begin(batch(T), adapters(T))
         assert (step.out == 0).all()
         step.out.fill_(5.0)
+
+
+def test_tokens_left_out_are_counted_per_step(step, monkeypatch):
+    given = []
+    monkeypatch.setattr(ts, "kv_append", lambda *a, bad: given.append(bad) or bad.add_(3))
+    for _ in range(2):
+        step.begin(batch(4), adapters(4))
+        assert int(step.bad) == 0 and step.bad.dtype == torch.int32
+        for _ in range(2):
+            step.layer(0, torch.zeros((4, 64), dtype=torch.float16))
+        assert int(step.bad) == 6 and all(b is step.bad for b in given)
