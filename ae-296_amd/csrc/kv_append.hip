@@ -106,17 +106,30 @@ static void append_of(const KvAppendArgs &a, dim3 grid, hipStream_t s)
     else hipLaunchKernelGGL((kv_append_kernel<DT, D, false>), grid, dim3(256), 0, s, a);
 }
 
-int launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s)
+// A launch has fewer than 2^32 threads: this many tokens each.
+constexpr int KV_LAUNCH_TOKENS = 1 << 23;
+
+int launch_kv_append(const KvAppendArgs &all, int dtype, hipStream_t s)
 {
-    const int rows = a.n_q_heads + 2 * a.n_kv_heads, per = 256 / (a.head_dim / 16);
-    const int all = (rows + per - 1) / per;
-    // a token's heads are shared by several workgroups while that adds workgroups the device has room for
-    int parts = (4 * device_compute_units() + a.b.T - 1) / a.b.T;
-    if (parts > all) parts = all;
-    const dim3 grid((unsigned)a.b.T, (unsigned)parts);
-    if (dtype == DT_F16) { if (a.head_dim == 64) append_of<DT_F16, 64>(a, grid, s); else append_of<DT_F16, 128>(a, grid, s); }
-    else { if (a.head_dim == 64) append_of<DT_BF16, 64>(a, grid, s); else append_of<DT_BF16, 128>(a, grid, s); }
-    return (int)hipGetLastError();
+    const int rows = all.n_q_heads + 2 * all.n_kv_heads, per = 256 / (all.head_dim / 16), cover = (rows + per - 1) / per;
+    for (int t0 = 0; t0 < all.b.T; t0 += KV_LAUNCH_TOKENS) {
+        KvAppendArgs a = all;
+        a.b.T = all.b.T - t0 < KV_LAUNCH_TOKENS ? all.b.T - t0 : KV_LAUNCH_TOKENS;
+        a.b.tok_req += t0;
+        a.b.tok_pos += t0;
+        a.k += t0 * a.k_stride;
+        a.v += t0 * a.v_stride;
+        if (a.q) { a.q += t0 * a.q_stride; a.q_out += t0 * a.q_out_stride; }
+        // a token's heads are shared by several workgroups while that adds workgroups the device has room for
+        int parts = (4 * device_compute_units() + a.b.T - 1) / a.b.T;
+        if (parts > cover) parts = cover;
+        const dim3 grid((unsigned)a.b.T, (unsigned)parts);
+        if (dtype == DT_F16) { if (a.head_dim == 64) append_of<DT_F16, 64>(a, grid, s); else append_of<DT_F16, 128>(a, grid, s); }
+        else { if (a.head_dim == 64) append_of<DT_BF16, 64>(a, grid, s); else append_of<DT_BF16, 128>(a, grid, s); }
+        const int rc = (int)hipGetLastError();
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 }  // namespace mlora

@@ -467,7 +467,7 @@ int mlora_w4_gemv_multi(int n_proj, void *const *y, const void *const *x, const 
  *   that they may be views of one fused projection output); q_out may be q itself, otherwise they must not overlap; q and
  *   q_out may both be NULL.  Computed in fp32, rounded once.  A token whose request or position no table holds, or whose page
  *   id is outside [0, n_pages), is left out as a whole and counted in *bad (device int32, or NULL).  (request, position)
- *   pairs must differ: of two equal ones either may be kept.
+ *   pairs must differ: what two equal ones leave there is a mixture of both.  T <= 2^30.
  * Replaces rotary_emb_fwd and destindex_copy_kv of the reference's layer (rotary_emb.py:8, destindex_copy_kv.py:8).
  */
 int mlora_kv_append(const void *q, int64_t q_stride, void *q_out, int64_t q_out_stride, const void *k, int64_t k_stride,

@@ -1,0 +1,37 @@
+"""Batches of more workgroups than one launch takes."""
+import pytest
+import torch
+
+import mlora
+from gpu_common import say
+
+pytestmark = pytest.mark.gpu
+F16 = torch.float16
+
+
+def test_append_of_more_tokens_than_a_launch_has_workgroups():
+    T = (1 << 24) + 1003
+    say(f"append T={T}")
+    P, D = 256, 64
+    pages = -(-T // P)
+    cache = mlora.KVCache(1, pages, 1, D, page_tokens=P, dtype=F16)
+    cache.v.zero_()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    req = torch.zeros(T, **i32)
+    req[5] = req[T - 2] = -1
+    bad = torch.zeros(1, **i32)
+    order = torch.randperm(pages, device="cuda").to(torch.int32)
+    order[3] = pages                                                    # 256 tokens whose page is none
+    batch = mlora.KVBatch(req, torch.arange(T, **i32), order[None])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn((T, 1, D), device="cuda", dtype=F16, generator=g) for _ in range(2))
+    assert mlora.kv_append(None, k, v, cache, 0, batch, None, bad=bad) is None
+    assert int(bad) == P
+    keep = torch.ones(T, dtype=torch.bool, device="cuda")
+    keep[5] = keep[T - 2] = False
+    keep[3 * P:4 * P] = False
+    order[3] = 0
+    for got, want in ((cache.k, k), (cache.v, v)):
+        rows = got[0, order.long(), 0].view(-1, D)[:T]
+        assert torch.equal(rows[keep], want[keep, 0])
+    assert (cache.v[0, order.long(), 0].view(-1, D)[[5, T - 2]] == 0).all()
