@@ -599,10 +599,26 @@ static void gemv_by_group(const W4Args &all, hipStream_t s)
     }
 }
 
-int launch_w4_gemv(const W4Args &a, int dtype, hipStream_t s)
+int launch_w4_gemv(const W4Args &all, int dtype, hipStream_t s)
 {
-    if (dtype == DT_F16) gemv_by_group<DT_F16>(a, s); else gemv_by_group<DT_BF16>(a, s);
-    return (int)hipGetLastError();
+    // A launch has fewer than 2^32 threads.  The form with the most workgroups has one for 32 columns and 16 tokens, and up to eight column blocks
+    // more to fill a row of XCDs: so many tokens each (whole token blocks of every form, where it is more than one).
+    int64_t cols = 8;
+    for (int p = 0; p < all.n_proj; p++) cols += (all.pr[p].n_tiles + 1) / 2;
+    const int64_t blocks = ((1LL << 32) / (64 * W4_WAVES) - 1) / cols;
+    const int each = (int)(blocks >= 1 << 16 ? 1 << 20 : blocks >= 4 ? blocks / 4 * 64 : 16);
+    for (int t0 = 0; t0 < all.T; t0 += each) {
+        W4Args a = all;
+        a.T = all.T - t0 < each ? all.T - t0 : each;
+        for (int p = 0; p < a.n_proj; p++) {
+            a.pr[p].x = static_cast<const uint16_t *>(a.pr[p].x) + (int64_t)t0 * a.pr[p].hin;
+            a.pr[p].y = static_cast<uint16_t *>(a.pr[p].y) + (int64_t)t0 * a.pr[p].hout;
+        }
+        if (dtype == DT_F16) gemv_by_group<DT_F16>(a, s); else gemv_by_group<DT_BF16>(a, s);
+        const int rc = (int)hipGetLastError();
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 }  // namespace mlora

@@ -1,12 +1,15 @@
 """Batches of more workgroups than one launch takes."""
+import numpy as np
 import pytest
 import torch
 
 import mlora
 from gpu_common import say
+from step_ref import check, store_bound, w4_exact
+from test_gpu_w4 import weight
 
 pytestmark = pytest.mark.gpu
-F16 = torch.float16
+F16, BF16 = torch.float16, torch.bfloat16
 
 
 def test_append_of_more_tokens_than_a_launch_has_workgroups():
@@ -35,3 +38,23 @@ def test_append_of_more_tokens_than_a_launch_has_workgroups():
         rows = got[0, order.long(), 0].view(-1, D)[:T]
         assert torch.equal(rows[keep], want[keep, 0])
     assert (cache.v[0, order.long(), 0].view(-1, D)[[5, T - 2]] == 0).all()
+
+
+@pytest.mark.parametrize("group", [64, 128])
+def test_product_of_more_blocks_than_a_launch_has_workgroups(group):
+    T, hin, hout = (1 << 20) - 5, 8, 16456
+    say(f"w4 T={T} {hin}->{hout} group={group}")
+    codes, scales, z = weight(hin, hout, group, True, BF16, 1)
+    w = mlora.W4Weight(codes, scales, z, group=group)
+    x = torch.randn((T, hin), device="cuda").to(BF16)
+    y = torch.full((T, hout), float("nan"), device="cuda", dtype=BF16)
+    mlora.w4_gemv([y], [x], [w])
+    for a in range(0, T, 1 << 16):
+        assert torch.isfinite(y[a:a + (1 << 16)].sum(1, dtype=torch.float32)).all(), f"rows from {a}"
+    rng = np.random.default_rng(1)
+    rows = torch.from_numpy(np.sort(np.concatenate([rng.integers(0, T, 200), [0, T - 1], np.arange(1, T // 64, 997) * 64]))).cuda()
+    want, bound = w4_exact(x[rows], codes, scales, z, group)
+    check(y[rows], want, bound + store_bound(np.abs(want) + bound, BF16))
+    before = y[rows].clone()
+    mlora.w4_gemv([y], [x], [w], accumulate=True)
+    check(y[rows], want + before.double().cpu().numpy(), bound + store_bound(np.abs(want) + bound + np.abs(before.double().cpu().numpy()), BF16))
