@@ -171,13 +171,14 @@ class TraceContext:
             raise ValueError("every request of a step is listed once, with one adapter")
         P = self.cache.page_tokens
         gone = set(self.pages) - {int(r) for r in requests}
+        prompt_pages = -(-self.prompt // P)
+        need = prompt_pages * len({int(a) for a in lora_ids} - set(self.prompts)) + sum(self.length.get(int(r), 0) % P == 0 for r in requests)
+        have = self.cache.free_pages + sum(len(self.pages[r]) for r in gone)
+        if need > have:                               # before anything changes
+            raise MemoryError(f"the step needs {need} more pages of keys, {have} are free")
         for r in gone:
             self.cache.release(self.pages.pop(r))
             del self.length[r]
-        prompt_pages = -(-self.prompt // P)
-        need = prompt_pages * len({int(a) for a in lora_ids} - set(self.prompts)) + sum(self.length.get(int(r), 0) % P == 0 for r in requests)
-        if need > self.cache.free_pages:              # before anything changes
-            raise MemoryError(f"the step needs {need} more pages of keys, {self.cache.free_pages} are free")
         of = [self._prompt_of(int(a)) for a in lora_ids]
         for r in map(int, requests):
             mine = self.pages.setdefault(r, [])
