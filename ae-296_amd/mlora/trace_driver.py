@@ -144,42 +144,51 @@ class AdapterResidency:
 
 
 class TraceContext:
-    """Keys and values of a trace's running requests: pages of a cache, one prompt of `prompt` tokens per adapter (written on its
-    first use and kept), and per request the pages of the tokens decoded so far, given back when it no longer runs."""
+    """Keys and values of a trace's running requests: pages of a cache, one prompt of `prompt` tokens per adapter (written on its first use
+    and kept until its pages are needed and none of its requests runs), and per request the pages of the tokens decoded so far, given back
+    when it no longer runs."""
 
     def __init__(self, cache, prompt: int, seed: int = 0):
         self.cache, self.prompt, self.seed = cache, prompt, seed
-        self.prompts: "OrderedDict[int, List[int]]" = OrderedDict()        # adapter -> pages; its place is its prefix id
+        self.prompts: "OrderedDict[int, List[int]]" = OrderedDict()        # adapter -> pages, the last used last
         self.pages: Dict[int, List[int]] = {}                              # request -> pages
         self.length: Dict[int, int] = {}                                   # request -> tokens of its own
 
-    def _prompt_of(self, adapter: int) -> int:
+    def _write_prompt(self, adapter: int) -> None:
         import torch
-        if adapter not in self.prompts:
-            c = self.cache
-            pages = c.allocate(-(-self.prompt // c.page_tokens))
-            g = torch.Generator().manual_seed(self.seed * 1000003 + adapter)
-            for p in pages:
-                for t in (c.k, c.v):
-                    t[:, p].copy_(torch.randn(t[:, p].shape, generator=g))
-            self.prompts[adapter] = pages
-        return list(self.prompts).index(adapter)
+        c = self.cache
+        pages = c.allocate(-(-self.prompt // c.page_tokens))
+        g = torch.Generator().manual_seed(self.seed * 1000003 + adapter)
+        for p in pages:
+            for t in (c.k, c.v):
+                t[:, p].copy_(torch.randn(t[:, p].shape, generator=g))
+        self.prompts[adapter] = pages
 
     def advance(self, requests: Sequence[int], lora_ids: Sequence[int]) -> dict:
-        """One more token for every request listed; those no longer listed give their pages back.  The batch as host lists."""
+        """One more token for every request listed; those no longer listed give their pages back.  The batch as host lists; its prefixes are
+        the prompts of its own requests' adapters."""
         if len(requests) != len(lora_ids) or len({int(r) for r in requests}) != len(requests):
             raise ValueError("every request of a step is listed once, with one adapter")
         P = self.cache.page_tokens
         gone = set(self.pages) - {int(r) for r in requests}
+        adapters = list(dict.fromkeys(int(a) for a in lora_ids))
+        new, idle = [a for a in adapters if a not in self.prompts], [a for a in self.prompts if a not in set(adapters)]
         prompt_pages = -(-self.prompt // P)
-        need = prompt_pages * len({int(a) for a in lora_ids} - set(self.prompts)) + sum(self.length.get(int(r), 0) % P == 0 for r in requests)
-        have = self.cache.free_pages + sum(len(self.pages[r]) for r in gone)
+        need = prompt_pages * len(new) + sum(self.length.get(int(r), 0) % P == 0 for r in requests)
+        have = self.cache.free_pages + sum(len(self.pages[r]) for r in gone) + prompt_pages * len(idle)
         if need > have:                               # before anything changes
-            raise MemoryError(f"the step needs {need} more pages of keys, {have} are free")
+            raise MemoryError(f"the step needs {need} more pages of keys, {have} are free or hold prompts of adapters it does not run")
         for r in gone:
             self.cache.release(self.pages.pop(r))
             del self.length[r]
-        of = [self._prompt_of(int(a)) for a in lora_ids]
+        for a in idle:
+            if need <= self.cache.free_pages:
+                break
+            self.cache.release(self.prompts.pop(a))
+        for a in new:
+            self._write_prompt(a)
+        for a in adapters:
+            self.prompts.move_to_end(a)
         for r in map(int, requests):
             mine = self.pages.setdefault(r, [])
             self.length[r] = self.length.get(r, 0) + 1
@@ -188,8 +197,8 @@ class TraceContext:
         lists = [self.pages[int(r)] for r in requests]
         width = max(map(len, lists))
         return dict(tok_req=list(range(len(lists))), tok_pos=[self.prompt + self.length[int(r)] - 1 for r in requests],
-                    pages=[p + [-1] * (width - len(p)) for p in lists], req_prefix=of,
-                    prefix_pages=list(self.prompts.values()), prefix_len=[self.prompt] * len(self.prompts))
+                    pages=[p + [-1] * (width - len(p)) for p in lists], req_prefix=[adapters.index(int(a)) for a in lora_ids],
+                    prefix_pages=[self.prompts[a] for a in adapters], prefix_len=[self.prompt] * len(adapters))
 
 
 class TraceRunner:
