@@ -172,10 +172,12 @@ __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
     const unsigned each = all >> 31 ? (unsigned)min(all / (unsigned)p.target, (1ULL << 31) - step) : ((unsigned)all + (unsigned)p.target - 1u) / (unsigned)p.target;
     const unsigned C = max((each + step - 1) / step, 1u) * step;
     auto range_of = [&](int keys, int cuts) { return (((unsigned)keys + cuts - 1) / (unsigned)cuts + step - 1) / step * step; };
-    // At 64 elements a head three workgroups fit a unit, and the longest ranges of the groups end last: two thirds of the length (256 requests
-    // behind 8 prefixes of 1500, 32 heads on 4: 30.1 us a layer against 33.8; 64 requests: 19.1 against 17.6; at 128 elements, 128 requests behind one
-    // of 8191, 91 against 86, so not there).
-    const unsigned G = p.head_dim == 64 ? max(C / step * 2 / 3, 1u) * step : C;
+    // At 64 elements a head three workgroups fit a unit, not two, and the longest ranges of the groups end last: two thirds of the length, in whole steps
+    // upwards, so 256 keys stay 256.  Against the whole length, at 240 sizes (1 to 8 prefixes of 300 to 8000, 8 to 256 requests with up to 100 or 512 keys of
+    // their own, 8 to 64 heads on 1 to 8): 0.80 to 1.08 of the time, 0.98 in the mean; most where own lists are long (256 requests behind 8 prefixes of
+    // 1500, 32 heads on 4: 28.7 us for 33.1), least where they are short (the same with up to 100 keys: 25.7 for 24.8).  Downwards 256 became 128: 19.2 us
+    // for 14.3 at 64 requests, 32 heads on 8.  At 128 elements it does not pay (128 requests behind one of 8191: 91 us a layer for 86).
+    const unsigned G = p.head_dim == 64 ? (C / step * 2 + 2) / 3 * step : C;
     // a wide tile leaves as much behind as it reads in 130 keys: its ranges are 256 at least
     auto group_cuts_of = [&](int f) { const unsigned c = rows_of(f) == PA_WIDE ? max(G, 256u) : G; return (int)((prefix_keys(f) + c - 1) / c); };
     auto cuts_of = [&](int keys) { return keys > 0 ? (int)(((unsigned)keys + C - 1) / C) : 0; };
