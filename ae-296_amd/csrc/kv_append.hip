@@ -6,7 +6,7 @@
 // A thread owns one pair of 16-byte chunks of a head - the two halves of eight rotation pairs - in several heads of one token, so it
 // reads its eight cosines and sines once; a workgroup covers 256 / (head_dim / 16) heads at a time.  Bound by HBM for prompts (8191 tokens of
 // 64 + 2 x 8 heads of 128, half of a head turning: 65 us for 336 MB, 5.2 TB/s read + written, a copy's rate) and by the launch and the
-// chain tables -> page -> rows for decode batches (7 tokens of 3 x 32 heads: 3.4 us).
+// chain tables -> page -> rows for decode batches (7 tokens of 3 x 32 heads: 3.7 us).
 #include "mlora_dev.hpp"
 #include "mlora_step.hpp"
 

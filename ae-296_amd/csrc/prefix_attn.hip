@@ -59,7 +59,7 @@ struct PlanView {
 };
 
 // Ranges of keys that fill the device: two workgroups a compute unit.  Twice as many cost more in parts than they level out (128 requests
-// over one prefix of 8191 keys: 82 us a layer against 90).
+// over one prefix of 8191 keys: a tenth more a layer).
 __host__ __device__ inline int pa_target(int n_kv_heads) { const int t = 512 / n_kv_heads; return t < 1 ? 1 : t; }
 
 // With C keys a range where C >= (sum of own keys + sum over groups of keys x row tiles) / target, a list is cut into at most
@@ -133,7 +133,7 @@ __device__ __forceinline__ int pl_find(const int *first, int n, int i)       // 
     return lo;
 }
 
-// One workgroup, bound by its scans and barriers: 5.2 us for one request, 8.4 for 256 requests behind 8 prefixes, once a step.
+// One workgroup, bound by its scans and barriers: 5.5 us for one request, 8.4 for 256 requests behind 8 prefixes, once a step.
 // Tokens enter their group's list in any order (LDS atomics): a row's arithmetic does not depend on its place in a tile.
 __global__ __launch_bounds__(PL_THREADS) void pa_plan_kernel(const PlanArgs p)
 {
@@ -472,7 +472,7 @@ __device__ __forceinline__ uint4 pa_load_q(const uint16_t *q, float scale)
 }
 
 // One item for one key head: NR tiles of 16 query rows, the keys shared by the four wavefronts and joined in LDS.  Bound by HBM on
-// long lists (two requests of 131071 keys, 8 heads of 128: 169 us for 1.07 GB, 6.4 TB/s; 61 of 1 to 2048, 32 heads: 5.8 TB/s) and on short
+// long lists (two requests of 131071 keys, 8 heads of 128: 169 us for 1.07 GB, 6.3 TB/s; 61 of 1 to 2048, 32 heads: 5.8 TB/s) and on short
 // ones by the chain page id -> keys -> softmax.
 template <int DT, int D, int NR, bool STREAM>
 __device__ __forceinline__ void pa_item(const AttnKernelArgs &ka, const_i32_ptr e, const PlanView &pv, int head, unsigned char *lds, float (*s_m)[16], float (*s_l)[16])
@@ -555,8 +555,9 @@ template <int D> __device__ __forceinline__ int pa_kswizzle(int r, int ch) { ret
 constexpr int PA_TILE = 64;                                // keys in LDS at a time
 
 // One wide item for one key head: 32 rows a wavefront, every key tile brought to LDS once for all of them, the next one on its way meanwhile.
-// Bound by the softmax's vector instructions.  128 requests over a prefix of 8191, 32 heads on 8: with their own keys (270 MB) 86 us a layer;
-// 111 before there were such tiles, with rows of own keys not yet streamed past L2.
+// Bound by what a wavefront waits for, with two on a SIMD: scores, maximum, exponentials, second product and barrier follow each other (128 requests with
+// one key of their own over a prefix of 8191, 32 heads on 8: 45.7 us; vector instructions take 44 % of the cycles, matrix instructions 19, and wavefronts
+// wait 38 % of theirs).  With own keys (270 MB) 86 us a layer; 111 before there were such tiles, with rows of own keys not yet streamed past L2.
 template <int DT, int D>
 __device__ __forceinline__ void pa_wide(const AttnKernelArgs &ka, const_i32_ptr e, const PlanView &pv, int head, unsigned char *lds)
 {

@@ -164,8 +164,8 @@ __device__ __forceinline__ W4Place w4_place(const W4Args &p)
 // 16 tokens a token block.  A workgroup: NT column tiles, its eight wavefronts share the K tiles (every eighth each, so that together they read
 // a column tile's codes in one stretch) and are joined in LDS.  A wavefront asks for its next K tile's codes, groups and x before it
 // multiplies the present one.  A lane loads the scale and zero point of one column and K step; the result's layout wants those of
-// four columns, which it gets through LDS.  Bound by the way in and out at one projection (4096 -> 4096, one token: 4.4 us for 8.7 MB; the
-// launch alone takes half) and by vector instructions beyond (one token, 5120 -> 27648, 73 MB: 17.7 us, 4.1 TB/s).
+// four columns, which it gets through LDS.  Bound by the way in and out at one projection (4096 -> 4096, one token, 8.7 MB: 5.0 us, 5.7
+// with the weights from HBM; the launch alone takes half) and by vector instructions beyond (one token, 5120 -> 27648, 73 MB: 19.3 us, 3.8 TB/s).
 template <int DT, int NT, int STEPS>
 __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args p)
 {
@@ -290,14 +290,15 @@ __global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_gemv_kernel(const W4Args 
 // chunk of sixteen rows) meet all banks.
 //
 // The sums of x of the next tile are shared: a wavefront makes those of 4 MT / WN steps and leaves them in LDS for the others (125 tokens,
-// 5120 -> 27648, each wavefront its own: 62.7 us).
+// 5120 -> 27648, each wavefront its own: 14 % longer).
 //
 // A K tile takes a wavefront less time than a load from HBM: codes and x are asked for three tiles ahead.  The loads to LDS are
 // inline assembly, because the compiler would end them before any read of LDS; not knowing of them it waits for codes somewhat
 // earlier than it has to, one reason for the third tile.
 //
 // Bound by vector instructions (making operands of codes, the groups' factors), matrix instructions and the operand reads of x from LDS, none of
-// which fills its unit: 125 tokens, 5120 -> 27648, groups of 128: 55.1 us for 35.4 GFLOP, 640 TFLOP/s.
+// which fills its unit: 125 tokens, 5120 -> 27648, groups of 128: 55.7 us for 35.4 GFLOP, 635 TFLOP/s, launch after launch
+// (62.7 among a layer's others in ten passes after a pause).
 template <int DT, int MT, int NT, int WN, int STEPS>
 __global__ __launch_bounds__(64 * W4_WAVES, 2) void w4_wide_kernel(const W4Args p)
 {
@@ -548,16 +549,20 @@ struct W4Form { int cols, rows, alone, base, each; };
 constexpr W4Form W4_FORMS[] = {{2, 16, 89, 34, 55}, {2, 32, 123, 20, 103}, {4, 32, 178, 30, 104}, {8, 32, 242, 30, 165}, {8, 64, 318, 20, 295}, {16, 64, 540, 20, 520}};
 
 // Up to 16 tokens: one column tile a workgroup while that makes one round of workgroups, two beyond (one token, 4096 -> 4096: 4.6 us against 5.7;
-// 4096 -> 22016: 15.9 against 13.2).  Beyond: the form of the least time by the table.  It is the fastest of the six at 73 of 76 sizes (20 to 256
-// tokens, 1024 to 14336 rows, 1024 to 28672 columns), at the others 0.1 to 0.4 us behind; some of them (us, the forms in the table's order):
-//     32 tokens,  4096 ->  4096      8.0    10.1    13.0    19.2    24.9    42.6
-//     64          4096 ->  4096     12.7    10.7    13.3    19.2    25.6    43.4
-//     32          5120 -> 15360     26.8    23.6    17.8    24.0    31.5    53.2
-//    200          5120 -> 27648    225.9   234.7   127.6   103.5   118.0   106.7
-//    125          5120 -> 15360     86.6    82.5    44.9    35.8    32.1    53.7
-//    125          5120 -> 27648    143.8   141.1    75.1    65.5    61.3    55.1
+// 4096 -> 22016: 15.9 against 13.2).  Beyond: the form of the least time by the table.  Against all six at 216 sizes (20 to 512 tokens, 1024 to 13824
+// rows, 1024 to 27648 columns) it is the fastest at 192 and 0.6 % behind in the mean; all but twelve are within 3 %, and these have 1024 rows and take
+// up to 1.5 us longer, 512 tokens, 1024 -> 27648, 10 (69 for 59).  Some sizes (us, the forms in the table's order, weights from HBM):
+//     32 tokens,  4096 ->  4096      8.1    10.4    13.0    19.2    24.7    42.9
+//     64          4096 ->  4096     12.5    10.7    13.1    19.1    25.4    43.4
+//     32          5120 -> 15360     26.7    23.8    17.5    24.8    31.0    52.9
+//    200          5120 -> 27648    234.9   233.9   132.2   103.8   124.7   108.7
+//    125          5120 -> 15360     81.6    81.9    44.0    36.3    35.0    54.1
+//    125          5120 -> 27648    144.1   142.0    78.2    69.6    63.4    55.7
 // With groups of 64 or 32 the accumulators and factors of the last three leave less room for workgroups (125 tokens, 5120 -> 15360, groups of
-// 64: 45.7 with the fourth, 45.9 with the third): the third is the widest there, at most 11 % behind what others reached.
+// 64: 45.7 with the fourth, 45.9 with the third): the third is the widest there, at most 11 % behind what others reached.  Of the three, at the same 216
+// sizes with groups of 64 and again of 32, the table's choice is the fastest at 210, and up to 1.2 us behind at six of 1024 rows.  Groups of 64, and 32:
+//     32 tokens,  4096 ->  4096      8.3    11.1    13.3
+//    125          5120 -> 15360     85.0    86.4    47.3            84.1    95.8    56.5
 template <int DT, int STEPS>
 static void gemv_by_size(W4Args a, hipStream_t s)
 {

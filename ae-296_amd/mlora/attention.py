@@ -101,7 +101,8 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache
     """Rotate q [T, Hq, D] and k [T, Hkv, D] by their tokens' positions and place k and v on their pages, in one launch;
     returns the rotated q (`q_out`, or q itself in place).  The tokens' rows may be apart (views of one fused projection output).
     ``rope=None`` places k and v as they are.  A token with a request whose position no table holds is left out as a whole and counted in `bad`
-    (int32, one value)."""
+    (int32, one value).  `q_out` may be q itself and otherwise overlaps neither q, k nor v; two tokens at one position of one request leave a mixture
+    of both there."""
     rc = _ext.host().kv_append(q, k, v, q_out, cache, layer, batch, rope, bad)
     if rc:
         _ext.check(rc)
@@ -149,7 +150,7 @@ def plan_attention(batch: KVBatch, cache: KVCache, n_q_heads: int, out: Optional
 def prefix_attention(q: torch.Tensor, cache: KVCache, layer: int, plan: AttnPlan, scale: Optional[float] = None,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[t, h] = softmax(scale * q[t, h] . K) V over positions 0 .. tok_pos[t] of token t's request, its prefix's among them;
-    q and out [T, Hq, D] (rows may be apart), scale 1 / sqrt(D) by default (0, or 2^-126 to 2^127 of either sign).  A row that sees no key is zeros (one whose
+    q and out [T, Hq, D] (rows may be apart), scale 1 / sqrt(D) by default (0, or 2^-126 to 2^127 of either sign); out must not overlap q.  A row that sees no key is zeros (one whose
     scores are all minus infinity is NaN, as the softmax is); rows without a request keep what `out` held (zeros in a new one)."""
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
