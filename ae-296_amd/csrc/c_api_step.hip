@@ -41,6 +41,43 @@ int check_w4(int hin, int hout, int group)
     return MLORA_OK;
 }
 
+int check_mx4(int rows, int k, int most)
+{
+    if (rows < 0 || k <= 0) return fail(MLORA_EINVAL, "rows must be >= 0 and k positive (got %d, %d)", rows, k);
+    if (k & 7) return fail(MLORA_EALIGN, "k must be a multiple of 8 (got %d)", k);
+    if (rows > most || k > (1 << 24)) return fail(MLORA_ERANGE, "at most %d rows and 2^24 columns (got %d, %d)", most, rows, k);
+    return MLORA_OK;
+}
+
+int check_mx4_packed(const void *packed, int64_t bytes, const mlora::Mx4Shape &sh)
+{
+    if (!packed) return fail(MLORA_EINVAL, "packed must not be NULL");
+    if (!aligned16(packed)) return fail(MLORA_EALIGN, "packed must be 16-byte aligned");
+    if (bytes < sh.bytes) return fail(MLORA_ENOSPACE, "packed has %lld bytes, %lld needed", (long long)bytes, (long long)sh.bytes);
+    return MLORA_OK;
+}
+
+// The sizes of a call's products; the pointers follow.
+int mx4_sizes(mlora::Mx4Args &a, int n_proj, const int32_t *hin, const int32_t *hout, int T)
+{
+    if (n_proj < 1 || n_proj > MLORA_MAX_PROJ) return fail(MLORA_ERANGE, "n_proj must be in 1..%d (got %d)", MLORA_MAX_PROJ, n_proj);
+    if (T < 0 || T > (1 << 20)) return fail(MLORA_ERANGE, "T must be in 0..2^20 (got %d)", T);
+    if (!hin || !hout) return fail(MLORA_EINVAL, "hin and hout must not be NULL");
+    memset(&a, 0, sizeof(a));
+    a.n_proj = n_proj; a.T = T;
+    for (int p = 0; p < n_proj; p++) {
+        if (hout[p] <= 0) return fail(MLORA_EINVAL, "projection %d: hout must be positive (got %d)", p, hout[p]);
+        const int rc = check_mx4(hout[p], hin[p], 1 << 24);
+        if (rc) return rc;
+        if (hout[p] & 7) return fail(MLORA_EALIGN, "projection %d: hout must be a multiple of 8 (got %d)", p, hout[p]);
+        const mlora::Mx4Shape sw = mlora::mx4_shape(hout[p], hin[p]), sx = mlora::mx4_shape(T, hin[p]);
+        mlora::Mx4Proj &w = a.pr[p];
+        w.w_scales_at = sw.scales_at; w.x_scales_at = sx.scales_at;
+        w.hin = hin[p]; w.hout = hout[p]; w.k_tiles = sw.k_tiles; w.quads = sw.quads;
+    }
+    return MLORA_OK;
+}
+
 int check_cache(int64_t n_pages, int page_tokens, int n_q_heads, int n_kv_heads, int head_dim)
 {
     if (head_dim != 64 && head_dim != 128) return fail(MLORA_ERANGE, "head_dim must be 64 or 128 (got %d)", head_dim);
@@ -91,6 +128,48 @@ int check_attn_sizes(int T, int n_prefix, int n_q_heads, int n_kv_heads)
     if (T < 0 || T > MLORA_ATTN_MAX_T) return fail(MLORA_ERANGE, "T must be in 0..%d (got %d)", MLORA_ATTN_MAX_T, T);
     if (n_prefix < 0 || n_prefix > MLORA_ATTN_MAX_PREFIX) return fail(MLORA_ERANGE, "n_prefix must be in 0..%d (got %d)", MLORA_ATTN_MAX_PREFIX, n_prefix);
     return check_cache(1, 16, n_q_heads, n_kv_heads, 64);
+}
+
+// The parts of a page table's two buffers.
+int pages_args(mlora::PagesArgs &a, void *state, int64_t state_words, void *scratch, int64_t scratch_words, const int32_t *want, bool wants,
+               int n_req, int max_pages, int64_t n_pages, int page_tokens)
+{
+    int64_t at[MLORA_PAGES_LAYOUT_WORDS];
+    const int rc = mlora_pages_layout(n_req, max_pages, n_pages, at);
+    if (rc) return rc;
+    if (log2_exact(page_tokens) < 4 || page_tokens > 256) return fail(MLORA_EINVAL, "page_tokens must be a power of two in 16..256 (got %d)", page_tokens);
+    if ((int64_t)max_pages * page_tokens > (1 << 30)) return fail(MLORA_ERANGE, "max_pages * page_tokens may be 2^30 at most");
+    if (!state || !scratch || (wants && !want)) return fail(MLORA_EINVAL, "state, scratch and the rows' values must not be NULL");
+    if (!aligned16(state) || !aligned16(scratch)) return fail(MLORA_EALIGN, "state and scratch must be 16-byte aligned");
+    if (state_words < at[6] || scratch_words < at[7])
+        return fail(MLORA_ENOSPACE, "state and scratch have %lld and %lld words, %lld and %lld needed", (long long)state_words, (long long)scratch_words,
+                    (long long)at[6], (long long)at[7]);
+    const mlora::PagesLayout l = mlora::pages_layout(n_req, max_pages, n_pages);
+    int32_t *s = static_cast<int32_t *>(state), *c = static_cast<int32_t *>(scratch);
+    memset(&a, 0, sizeof(a));
+    a.free_bits = s; a.table = s + l.table; a.lens = s + l.lens; a.refs = s + l.refs; a.failed = s + l.failed; a.live = s + l.live;
+    a.managed = c; a.head = c + l.head; a.writers = c + l.writers; a.last_writer = c + l.last_writer; a.picked = c + l.picked;
+    a.move_from = c + l.move_from; a.word_movers = c + l.word_movers; a.word_rank = c + l.word_rank; a.row_page = c + l.row_page;
+    a.row_new = c + l.row_new; a.copies = c + l.copies; a.rows = c + l.rows;
+    a.want = want; a.n_pages = n_pages; a.n_req = n_req; a.max_pages = max_pages; a.page_shift = log2_exact(page_tokens);
+    return MLORA_OK;
+}
+
+int pages_slabs(mlora::PagesArgs &a, void *k, void *v, int n_layers, int n_kv_heads, int page_tokens, int head_dim)
+{
+    if (head_dim != 64 && head_dim != 128) return fail(MLORA_ERANGE, "head_dim must be 64 or 128 (got %d)", head_dim);
+    if (n_layers <= 0 || n_kv_heads <= 0) return fail(MLORA_EINVAL, "n_layers and n_kv_heads must be positive (got %d, %d)", n_layers, n_kv_heads);
+    if (n_layers > (1 << 20) || n_kv_heads > (1 << 14)) return fail(MLORA_ERANGE, "at most 2^20 layers and 2^14 key heads");
+    if (!k || !v) return fail(MLORA_EINVAL, "k_pages and v_pages must not be NULL");
+    if (!aligned16(k) || !aligned16(v)) return fail(MLORA_EALIGN, "device pointers must be 16-byte aligned");
+    a.k = static_cast<uint16_t *>(k); a.v = static_cast<uint16_t *>(v);
+    a.n_layers = n_layers; a.n_kv_heads = n_kv_heads; a.head_elems = page_tokens * head_dim;
+    return MLORA_OK;
+}
+
+int launched(int rc, const char *what)
+{
+    return rc ? fail(MLORA_ELAUNCH, "%s launch failed: %s", what, hipGetErrorString((hipError_t)rc)) : MLORA_OK;
 }
 
 }  // namespace
@@ -261,6 +340,131 @@ int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t
     rc = mlora::launch_prefix_attention(a, dtype, plan, workspace, static_cast<hipStream_t>(stream));
     if (rc) return fail(MLORA_ELAUNCH, "attention launch failed: %s", hipGetErrorString((hipError_t)rc));
     return MLORA_OK;
+}
+
+int64_t mlora_mx4_bytes(int rows, int k)
+{
+    const int rc = check_mx4(rows, k, 1 << 24);
+    return rc ? rc : mlora::mx4_shape(rows, k).bytes;
+}
+
+int mlora_mx4_quantize(const void *x, int64_t x_stride, int rows, int k, int dtype, void *packed, int64_t packed_bytes, void *stream)
+{
+    if (dtype != MLORA_F16 && dtype != MLORA_BF16) return fail(MLORA_EDTYPE, "dtype must be MLORA_F16 or MLORA_BF16 (got %d)", dtype);
+    int rc = check_mx4(rows, k, 1 << 24);
+    if (rc) return rc;
+    if (rows == 0) return MLORA_OK;
+    mlora::Mx4QuantArgs a;
+    a.sh = mlora::mx4_shape(rows, k);
+    if (!x) return fail(MLORA_EINVAL, "x must not be NULL");
+    if (!aligned16(x) || (x_stride & 7)) return fail(MLORA_EALIGN, "x must be 16-byte aligned and x_stride a multiple of 8 (got %lld)", (long long)x_stride);
+    if (x_stride < k && rows > 1) return fail(MLORA_EINVAL, "x_stride must be at least k (got %lld)", (long long)x_stride);
+    if ((rc = check_mx4_packed(packed, packed_bytes, a.sh))) return rc;
+    a.x = static_cast<const uint16_t *>(x); a.x_stride = x_stride; a.packed = static_cast<unsigned char *>(packed);
+    return launched(mlora::launch_mx4_quantize(a, dtype, static_cast<hipStream_t>(stream)), "quantize");
+}
+
+int mlora_mx4_pack(const uint8_t *codes, const uint8_t *scales, int rows, int k, void *packed, int64_t packed_bytes, void *stream)
+{
+    int rc = check_mx4(rows, k, 1 << 24);
+    if (rc) return rc;
+    if (rows == 0) return MLORA_OK;
+    mlora::Mx4PackArgs a;
+    a.sh = mlora::mx4_shape(rows, k);
+    if (!codes || !scales) return fail(MLORA_EINVAL, "codes and scales must not be NULL");
+    if ((rc = check_mx4_packed(packed, packed_bytes, a.sh))) return rc;
+    a.codes = codes; a.scales = scales; a.packed = static_cast<unsigned char *>(packed);
+    return launched(mlora::launch_mx4_pack(a, static_cast<hipStream_t>(stream)), "pack");
+}
+
+int mlora_mx4_values(const void *packed, int64_t packed_bytes, int rows, int k, void *out, int64_t out_stride, int dtype, void *stream)
+{
+    if (dtype != MLORA_F16 && dtype != MLORA_BF16) return fail(MLORA_EDTYPE, "dtype must be MLORA_F16 or MLORA_BF16 (got %d)", dtype);
+    int rc = check_mx4(rows, k, 1 << 24);
+    if (rc) return rc;
+    if (rows == 0) return MLORA_OK;
+    mlora::Mx4ValuesArgs a;
+    a.sh = mlora::mx4_shape(rows, k);
+    if (!out) return fail(MLORA_EINVAL, "out must not be NULL");
+    if (!aligned16(out) || (out_stride & 7)) return fail(MLORA_EALIGN, "out must be 16-byte aligned and out_stride a multiple of 8 (got %lld)", (long long)out_stride);
+    if (out_stride < k && rows > 1) return fail(MLORA_EINVAL, "out_stride must be at least k (got %lld)", (long long)out_stride);
+    if ((rc = check_mx4_packed(packed, packed_bytes, a.sh))) return rc;
+    a.packed = static_cast<const unsigned char *>(packed); a.out = static_cast<uint16_t *>(out); a.out_stride = out_stride;
+    return launched(mlora::launch_mx4_values(a, dtype, static_cast<hipStream_t>(stream)), "values");
+}
+
+int64_t mlora_mx4_workspace_bytes(int n_proj, const int32_t *hin, const int32_t *hout, int T)
+{
+    mlora::Mx4Args a;
+    const int rc = mx4_sizes(a, n_proj, hin, hout, T);
+    return rc ? rc : T == 0 ? 0 : mlora::mx4_workspace_bytes(a);
+}
+
+int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const void *const *w, const int32_t *hin, const int32_t *hout,
+                         int T, int dtype, int accumulate, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    if (dtype != MLORA_F16 && dtype != MLORA_BF16) return fail(MLORA_EDTYPE, "dtype must be MLORA_F16 or MLORA_BF16 (got %d)", dtype);
+    mlora::Mx4Args a;
+    const int rc = mx4_sizes(a, n_proj, hin, hout, T);
+    if (rc) return rc;
+    if (!y || !x || !w) return fail(MLORA_EINVAL, "y, x and w must not be NULL");
+    if (T == 0) return MLORA_OK;
+    a.accumulate = accumulate != 0;
+    for (int p = 0; p < n_proj; p++) {
+        if (!y[p] || !x[p] || !w[p]) return fail(MLORA_EINVAL, "projection %d: NULL device pointer", p);
+        if (!aligned16(y[p]) || !aligned16(x[p]) || !aligned16(w[p])) return fail(MLORA_EALIGN, "projection %d: device pointers must be 16-byte aligned", p);
+        a.pr[p].y = y[p]; a.pr[p].x = static_cast<const unsigned char *>(x[p]); a.pr[p].w = static_cast<const unsigned char *>(w[p]);
+    }
+    for (int p = 0; p < n_proj; p++)                              // workgroups read and write in no order
+        for (int o = 0; o < n_proj; o++) {
+            const size_t yp = (size_t)T * hout[p] * 2;
+            if (overlap(y[p], yp, x[o], mlora::mx4_shape(T, hin[o]).bytes) || overlap(y[p], yp, w[o], mlora::mx4_shape(hout[o], hin[o]).bytes) ||
+                (o < p && overlap(y[p], yp, y[o], (size_t)T * hout[o] * 2)))
+                return fail(MLORA_EINVAL, "projection %d: y overlaps y, x or the weight of projection %d", p, o);
+        }
+    const int64_t need = mlora::mx4_workspace_bytes(a);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return fail(MLORA_ENOSPACE, "workspace has %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    if (!aligned16(workspace)) return fail(MLORA_EALIGN, "workspace must be 16-byte aligned");
+    return launched(mlora::launch_mx4_gemm(a, dtype, workspace, static_cast<hipStream_t>(stream)), "product");
+}
+
+int mlora_pages_layout(int n_req, int max_pages, int64_t n_pages, int64_t *at)
+{
+    if (n_req <= 0 || max_pages <= 0 || n_pages <= 0) return fail(MLORA_EINVAL, "n_req, max_pages and n_pages must be positive (got %d, %d, %lld)", n_req, max_pages, (long long)n_pages);
+    if ((int64_t)n_req * max_pages > (1 << 30) || n_req > (1 << 24) || n_pages > (1 << 24))
+        return fail(MLORA_ERANGE, "at most 2^24 rows and pages and 2^30 table entries (got %d, %lld, %lld)", n_req, (long long)n_pages, (long long)n_req * max_pages);
+    if (!at) return fail(MLORA_EINVAL, "at must not be NULL");
+    const mlora::PagesLayout l = mlora::pages_layout(n_req, max_pages, n_pages);
+    const int64_t words[MLORA_PAGES_LAYOUT_WORDS] = {0, l.table, l.lens, l.refs, l.failed, l.live, l.state_words, l.scratch_words};
+    memcpy(at, words, sizeof(words));
+    return MLORA_OK;
+}
+
+int mlora_pages_resize(void *state, int64_t state_words, void *scratch, int64_t scratch_words, const int32_t *want, int n_req, int max_pages,
+                       void *k_pages, void *v_pages, int n_layers, int64_t n_pages, int n_kv_heads, int page_tokens, int head_dim, void *stream)
+{
+    mlora::PagesArgs a;
+    int rc = pages_args(a, state, state_words, scratch, scratch_words, want, true, n_req, max_pages, n_pages, page_tokens);
+    if (rc || (rc = pages_slabs(a, k_pages, v_pages, n_layers, n_kv_heads, page_tokens, head_dim))) return rc;
+    return launched(mlora::launch_pages_resize(a, static_cast<hipStream_t>(stream)), "resize");
+}
+
+int mlora_pages_fork(void *state, int64_t state_words, void *scratch, int64_t scratch_words, const int32_t *parent, int n_req, int max_pages,
+                     int64_t n_pages, int page_tokens, void *stream)
+{
+    mlora::PagesArgs a;
+    const int rc = pages_args(a, state, state_words, scratch, scratch_words, parent, true, n_req, max_pages, n_pages, page_tokens);
+    if (rc) return rc;
+    return launched(mlora::launch_pages_fork(a, static_cast<hipStream_t>(stream)), "fork");
+}
+
+int mlora_pages_compact(void *state, int64_t state_words, void *scratch, int64_t scratch_words, int n_req, int max_pages,
+                        void *k_pages, void *v_pages, int n_layers, int64_t n_pages, int n_kv_heads, int page_tokens, int head_dim, void *stream)
+{
+    mlora::PagesArgs a;
+    int rc = pages_args(a, state, state_words, scratch, scratch_words, nullptr, false, n_req, max_pages, n_pages, page_tokens);
+    if (rc || (rc = pages_slabs(a, k_pages, v_pages, n_layers, n_kv_heads, page_tokens, head_dim))) return rc;
+    return launched(mlora::launch_pages_compact(a, static_cast<hipStream_t>(stream)), "compact");
 }
 
 }  // extern "C"

@@ -54,7 +54,8 @@ PyObject *s_page_tbl, *s_rank, *s_scaling, *s_work, *s_group, *s_perm, *s_seg_st
     *s_chunk_start, *s_chunk_len, *s_chunk_adapter, *s_counters, *s_row_off, *s_tok_rank, *s_tok_scale, *s_T, *s_workspace,
     *s_n_slots, *s_max_pages, *s_page_rows, *s_n_pages, *s_max_rank, *s_tok_adapter, *s_dtype_code, *s_projections, *s_a_rows, *s_b_rows, *s_buf,
     *s_packed, *s_hin, *s_hout, *s_has_zeros, *s_tok_req, *s_tok_pos, *s_pages, *s_req_prefix, *s_prefix_pages, *s_prefix_len, *s_k, *s_v,
-    *s_cos_sin, *s_interleaved, *s_batch, *s_n_q_heads, *s_n_kv_heads, *s_page_tokens, *s_n_req, *s_n_prefix;
+    *s_cos_sin, *s_interleaved, *s_batch, *s_n_q_heads, *s_n_kv_heads, *s_page_tokens, *s_n_req, *s_n_prefix, *s_rows,
+    *s_state, *s_scratch, *s_cache;
 
 void *attr_ptr(PyObject *o, PyObject *name)          // data pointer of a tensor attribute, null for None
 {
@@ -688,6 +689,153 @@ PyObject *prefix_attention(PyObject *const *v, Py_ssize_t nargs)
                                   b.max_prefix_pages, (float)scale, pb, buf.numel(), room.get(), bytes, c.dtype, stream()));
 }
 
+// ---------------------------------------------------------------- microscaled operands
+struct Packed {     // an MX4Tensor
+    const at::Tensor t;
+    int rows, k;
+    explicit Packed(PyObject *o) : t(Attr(o, s_packed).t()), rows((int)attr_int(o, s_rows)), k((int)attr_int(o, s_k))
+    {
+        need_here(t);
+        if (t.scalar_type() != at::kByte || !t.is_contiguous() || t.numel() < mlora_mx4_bytes(rows, k))
+            raise(PyExc_ValueError, "the packed operand is not what its sizes need");
+    }
+};
+
+// Rows of `k` elements next to each other, and the elements from row to row.
+void *rows_of(const char *name, const at::Tensor &t, int64_t k, int64_t &stride)
+{
+    need_device(t);
+    if (t.dim() != 2 || (k >= 0 && t.size(1) != k)) raise(PyExc_ValueError, "%s must be [rows, k]", name);
+    if (t.size(0) > 0x7fffffffLL || t.size(1) > 0x7fffffffLL) raise(PyExc_ValueError, "%s is too large", name);
+    if (t.stride(1) != 1 && t.size(1) > 1) raise(PyExc_ValueError, "the elements of a row of %s must lie one behind the other", name);
+    need_here(t);
+    stride = t.size(0) > 1 ? t.stride(0) : t.size(1);
+    return t.data_ptr();
+}
+
+// mx4_quantize(x, packed): the packed buffer has the room that x needs, or an error
+PyObject *mx4_quantize(PyObject *const *v, Py_ssize_t nargs)
+{
+    if (nargs != 2) raise(PyExc_TypeError, "mx4_quantize takes 2 arguments");
+    const at::Tensor &x = tensor(v[0]), &b = tensor(v[1]);
+    const int dtype = dtype_of(x);
+    int64_t stride;
+    const void *rows = rows_of("x", x, -1, stride);
+    need_here(b);
+    if (b.scalar_type() != at::kByte || !b.is_contiguous()) raise(PyExc_ValueError, "packed must be a contiguous uint8 buffer");
+    return PyLong_FromLong(launch(mlora_mx4_quantize, rows, stride, (int)x.size(0), (int)x.size(1), dtype, b.data_ptr(), b.numel(), stream()));
+}
+
+// mx4_values(packed operand, out)
+PyObject *mx4_values(PyObject *const *v, Py_ssize_t nargs)
+{
+    if (nargs != 2) raise(PyExc_TypeError, "mx4_values takes 2 arguments");
+    const Packed p(v[0]);
+    const at::Tensor &out = tensor(v[1]);
+    const int dtype = dtype_of(out);
+    int64_t stride;
+    void *rows = rows_of("out", out, p.k, stride);
+    if (out.size(0) != p.rows) raise(PyExc_ValueError, "out must have %d rows", p.rows);
+    return PyLong_FromLong(launch(mlora_mx4_values, p.t.data_ptr(), p.t.numel(), p.rows, p.k, rows, stride, dtype, stream()));
+}
+
+// mx4_gemm(ys, xs, weights, accumulate)
+PyObject *mx4_gemm(PyObject *const *v, Py_ssize_t nargs)
+{
+    if (nargs != 4) raise(PyExc_TypeError, "mx4_gemm takes 4 arguments");
+    const List ys(v[0]);
+    const Ref xs(PySequence_Fast(v[1], "expected a sequence of MX4Tensor")), ws(PySequence_Fast(v[2], "expected a sequence of MX4Tensor"));
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(ws.o);
+    if (n < 1 || n > MLORA_MAX_PROJ || ys.size() != n || PySequence_Fast_GET_SIZE(xs.o) != n)
+        raise(PyExc_ValueError, "need 1..%d projections with one y, one x and one weight each", MLORA_MAX_PROJ);
+    const at::ScalarType type = ys[0].scalar_type();
+    const int dtype = dtype_of(ys[0]);
+    void *y[MLORA_MAX_PROJ];
+    const void *x[MLORA_MAX_PROJ], *w[MLORA_MAX_PROJ];
+    int32_t hin[MLORA_MAX_PROJ], hout[MLORA_MAX_PROJ];
+    int T = 0;
+    for (Py_ssize_t i = 0; i < n; i++) {
+        const Packed px(PySequence_Fast_GET_ITEM(xs.o, i)), pw(PySequence_Fast_GET_ITEM(ws.o, i));
+        const at::Tensor &yt = ys[i];
+        need_here(yt);
+        need_contiguous(yt);
+        if (i == 0) T = px.rows;
+        if (yt.scalar_type() != type) raise(PyExc_TypeError, "all y must share one 16-bit dtype");
+        if (px.rows != T || px.k != pw.k || yt.dim() != 2 || yt.size(0) != T || yt.size(1) != pw.rows)
+            raise(PyExc_ValueError, "projection %d: expected x [%d, %d] and y [%d, %d]", (int)i, T, pw.k, T, pw.rows);
+        y[i] = yt.data_ptr(); x[i] = px.t.data_ptr(); w[i] = pw.t.data_ptr();
+        hin[i] = pw.k; hout[i] = pw.rows;
+    }
+    // this call's own, as in bgmv_ref
+    const int64_t bytes = mlora_mx4_workspace_bytes((int)n, hin, hout, T);
+    at::DataPtr room;
+    if (bytes > 0) {
+        const c10::DeviceGuard device(ys[0].device());
+        room = c10::GetAllocator(at::kCUDA)->allocate((size_t)bytes);
+    }
+    return PyLong_FromLong(launch(mlora_mx4_gemm_multi, (int)n, y, x, w, hin, hout, T, dtype, (int)is_true(v[3]), room.get(), bytes > 0 ? bytes : 0, stream()));
+}
+
+// ---------------------------------------------------------------- page tables
+struct Pages {      // a KVPages
+    const at::Tensor state, scratch;
+    const Cache c;
+    int64_t n_layers;
+    int n_req, max_pages;
+    Pages(PyObject *o, PyObject *cache, PyObject *k) : state(Attr(o, s_state).t()), scratch(Attr(o, s_scratch).t()), c(cache_of(cache, 0)),
+        n_layers(tensor(k).size(0)), n_req((int)attr_int(o, s_n_req)), max_pages((int)attr_int(o, s_max_pages))
+    {
+        for (const at::Tensor &t : {state, scratch}) {
+            need_here(t);
+            if (t.scalar_type() != at::kInt || !t.is_contiguous()) raise(PyExc_ValueError, "the tables' state and scratch must be contiguous int32 buffers");
+        }
+    }
+};
+
+template <typename F>
+PyObject *with_pages(PyObject *const *v, Py_ssize_t nargs, bool wants, F call)
+{
+    if (nargs != (wants ? 2 : 1)) raise(PyExc_TypeError, "pages calls take the tables and, but for compact, the rows' values");
+    const Ref cache(PyObject_GetAttr(v[0], s_cache)), k(PyObject_GetAttr(cache.o, s_k));
+    const Pages p(v[0], cache.o, k.o);
+    const int32_t *want = nullptr;
+    if (wants) {
+        const at::Tensor &t = tensor(v[1]);
+        need_here(t);
+        if (t.scalar_type() != at::kInt) raise(PyExc_TypeError, "the rows' values must be int32");
+        if (t.dim() != 1 || t.size(0) != p.n_req || !t.is_contiguous()) raise(PyExc_ValueError, "expected one contiguous value for each of the %d rows", p.n_req);
+        want = static_cast<const int32_t *>(t.data_ptr());
+    }
+    return PyLong_FromLong(call(p, want));
+}
+
+// pages_resize(pages, want)
+PyObject *pages_resize(PyObject *const *v, Py_ssize_t nargs)
+{
+    return with_pages(v, nargs, true, [](const Pages &p, const int32_t *want) {
+        return launch(mlora_pages_resize, p.state.data_ptr(), p.state.numel(), p.scratch.data_ptr(), p.scratch.numel(), want, p.n_req, p.max_pages, p.c.k,
+                      p.c.v, (int)p.n_layers, p.c.n_pages, p.c.n_kv_heads, p.c.page_tokens, p.c.head_dim, stream());
+    });
+}
+
+// pages_fork(pages, parent)
+PyObject *pages_fork(PyObject *const *v, Py_ssize_t nargs)
+{
+    return with_pages(v, nargs, true, [](const Pages &p, const int32_t *parent) {
+        return launch(mlora_pages_fork, p.state.data_ptr(), p.state.numel(), p.scratch.data_ptr(), p.scratch.numel(), parent, p.n_req, p.max_pages,
+                      p.c.n_pages, p.c.page_tokens, stream());
+    });
+}
+
+// pages_compact(pages)
+PyObject *pages_compact(PyObject *const *v, Py_ssize_t nargs)
+{
+    return with_pages(v, nargs, false, [](const Pages &p, const int32_t *) {
+        return launch(mlora_pages_compact, p.state.data_ptr(), p.state.numel(), p.scratch.data_ptr(), p.scratch.numel(), p.n_req, p.max_pages, p.c.k,
+                      p.c.v, (int)p.n_layers, p.c.n_pages, p.c.n_kv_heads, p.c.page_tokens, p.c.head_dim, stream());
+    });
+}
+
 // ---------------------------------------------------------------- module
 template <PyObject *(*F)(PyObject *const *, Py_ssize_t)>
 PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t nargs)
@@ -704,7 +852,8 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 
 #define MLORA_FN(name) {#name, (PyCFunction)(void (*)())entry<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MLORA_FN(gather), MLORA_FN(bgmv), MLORA_FN(bgmv_ref), MLORA_FN(deltas_ref), MLORA_FN(order), MLORA_FN(state), MLORA_FN(prefill_plan),
-                         MLORA_FN(sgmv_multi), MLORA_FN(w4_gemv), MLORA_FN(kv_append), MLORA_FN(attn_plan), MLORA_FN(prefix_attention), {nullptr, nullptr, 0, nullptr}};
+                         MLORA_FN(sgmv_multi), MLORA_FN(w4_gemv), MLORA_FN(kv_append), MLORA_FN(attn_plan), MLORA_FN(prefix_attention),
+                         MLORA_FN(mx4_quantize), MLORA_FN(mx4_values), MLORA_FN(mx4_gemm), MLORA_FN(pages_resize), MLORA_FN(pages_fork), MLORA_FN(pages_compact), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native launch path of mlora's eager calls.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -723,7 +872,7 @@ PyMODINIT_FUNC PyInit__host()
         {&s_tok_pos, "tok_pos"}, {&s_pages, "pages"}, {&s_req_prefix, "req_prefix"}, {&s_prefix_pages, "prefix_pages"},
         {&s_prefix_len, "prefix_len"}, {&s_k, "k"}, {&s_v, "v"}, {&s_cos_sin, "cos_sin"}, {&s_interleaved, "interleaved"},
         {&s_batch, "batch"}, {&s_n_q_heads, "n_q_heads"}, {&s_n_kv_heads, "n_kv_heads"}, {&s_page_tokens, "page_tokens"},
-        {&s_n_req, "n_req"}, {&s_n_prefix, "n_prefix"}};
+        {&s_n_req, "n_req"}, {&s_n_prefix, "n_prefix"}, {&s_rows, "rows"}, {&s_state, "state"}, {&s_scratch, "scratch"}, {&s_cache, "cache"}};
     for (const auto &p : names)
         if (!(*p.first = PyUnicode_InternFromString(p.second))) return nullptr;
     return PyModule_Create(&module);

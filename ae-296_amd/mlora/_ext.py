@@ -26,6 +26,7 @@ CNT_NSEG, CNT_NVALID, CNT_NCHUNK, CNT_BAD, CNT_WORDS = 0, 1, 2, 3, 8
 WORK_WORDS = 80
 SCATTER_MAX_JOBS = 16
 ATTN_MAX_T = 8192                   # MLORA_ATTN_MAX_T
+PAGES_LAYOUT_WORDS = 8              # MLORA_PAGES_LAYOUT_WORDS
 NOALLOC_SCRATCH_BYTES = 16 << 20    # MLORA_NOALLOC_SCRATCH_BYTES
 
 
@@ -89,6 +90,16 @@ SIGNATURES = {
     "mlora_attn_plan": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
     "mlora_prefix_attention": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp,
                                       _vp, _vp, _i32, _i32, _f32, _vp, _i64, _vp, _i64, _i32, _vp]),
+    "mlora_mx4_bytes": (_i64, [_i32, _i32]),
+    "mlora_mx4_quantize": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "mlora_mx4_pack": (_i32, [_vp, _vp, _i32, _i32, _vp, _i64, _vp]),
+    "mlora_mx4_values": (_i32, [_vp, _i64, _i32, _i32, _vp, _i64, _i32, _vp]),
+    "mlora_mx4_workspace_bytes": (_i64, [_i32, _vp, _vp, _i32]),
+    "mlora_mx4_gemm_multi": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "mlora_pages_layout": (_i32, [_i32, _i32, _i64, _vp]),
+    "mlora_pages_resize": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _vp]),
+    "mlora_pages_fork": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i32, _i64, _i32, _vp]),
+    "mlora_pages_compact": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _vp]),
     "mlora_prefill_reflayout": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
 }
 

@@ -506,6 +506,62 @@ int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t
                            int max_prefix_pages, float scale, const void *plan, int64_t plan_bytes, void *workspace,
                            int64_t workspace_bytes, int dtype, void *stream);
 
+/*
+ * Microscaled 4-bit operands (MXFP4: elements 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign; a power of two, held as a byte 127 + X, for every 32
+ * columns of a row; byte 255: the block is NaN) and their products, for base projections whose weights and inputs are both kept so:
+ *     y_p[t][n] = (accumulate ? y_p[t][n] : 0) + sum_b 2^(X_x[t][b] + X_w[n][b]) sum_{k in block b} cx[t][k] * cw[n][k]
+ * A packed operand [rows, k] (rows: tokens, or the output columns of a weight; k the input width) takes mlora_mx4_bytes(rows, k) bytes, 16-byte
+ * aligned.  k and the output widths are multiples of 8; the last block of a row may be shorter.
+ *   mlora_mx4_quantize: from 16-bit rows x (x_stride elements from row to row, a multiple of 8).  X = floor(log2(largest magnitude)) - 2, -127 at
+ *     least; every element becomes the nearest value of the grid times 2^X, of two equally near ones that of the even code, and 6 * 2^X
+ *     at most.  A block with an infinity or a NaN is NaN.
+ *   mlora_mx4_pack: from codes uint8 [rows, k / 2] (an even column in the low half of a byte; sign in bit 3) and scales uint8 [rows, ceil(k / 32)].
+ *   mlora_mx4_values: the values a packed operand stands for, rounded to the 16-bit type (exact for what was quantised from that type).
+ *   mlora_mx4_gemm_multi takes y (16-bit [T, hout]), x and w (packed), hin and hout as HOST arrays of n_proj entries; no y may overlap another y, an x
+ *     or a w.  Products exact, sums in fp32, the result rounded once; a block with a NaN makes its results NaN, and where a sum leaves fp32's range
+ *     the result is infinite or NaN.  `workspace`: mlora_mx4_workspace_bytes(...) bytes (0: NULL will do); calls that share it must be ordered on
+ *     one stream.
+ * rows <= 2^20 where they are tokens (T), 2^24 otherwise; k <= 2^24.  The counterpart of the reference's quantised base GEMMs with quantised
+ * activations (quantize_gemm_int8.py:18,109), in the format of the 4-bit matrix instructions.
+ */
+int64_t mlora_mx4_bytes(int rows, int k);
+int mlora_mx4_quantize(const void *x, int64_t x_stride, int rows, int k, int dtype, void *packed, int64_t packed_bytes, void *stream);
+int mlora_mx4_pack(const uint8_t *codes, const uint8_t *scales, int rows, int k, void *packed, int64_t packed_bytes, void *stream);
+int mlora_mx4_values(const void *packed, int64_t packed_bytes, int rows, int k, void *out, int64_t out_stride, int dtype, void *stream);
+int64_t mlora_mx4_workspace_bytes(int n_proj, const int32_t *hin, const int32_t *hout, int T);
+int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const void *const *w, const int32_t *hin, const int32_t *hout,
+                         int T, int dtype, int accumulate, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Page tables that live on the device: n_req rows of max_pages page ids each (what page_tbl of the calls above takes), the tokens of every row and
+ * the number of table entries that name each page, so that rows may share pages.  A state of one row: lens[r] tokens on the pages table[r][0 ..
+ * ceil(lens[r] / page_tokens)), -1 behind them.  Pages outside the managed ones are never handed out, copied or moved.
+ *   mlora_pages_layout writes the offsets of the state's parts, in int32 words: at[0] free bits (one bit a page, in two words for every 64: managed
+ *     and named by no entry), [1] table, [2] lens, [3] refs [n_pages], [4] failed, [5] live, [6] the state's length; and [7] the scratch's
+ *     length, whose first words are the managed bits.  The rest of the scratch starts as zeros; both buffers belong to these calls, which must be
+ *     ordered on one stream.
+ *   mlora_pages_resize gives rows new lengths want[r] (device int32; negative: the row is left as it is).  First every shorter row's pages
+ *     behind its new end are given back.  Then every longer row gets the pages it lacks; where its last page is only partly filled and other
+ *     entries name it too, it gets a copy of the page's filled part, in keys and values of all layers, and names that instead - but
+ *     for the last such row, if all that name the page are such rows.  Free pages are handed out in ascending order, to the rows in their order, a copy
+ *     before the rest.  A longer row is served if the pages asked for by it and the rows before it are there, or if it asks for none and shares
+ *     nothing that it writes on; otherwise it keeps its length and pages, and is counted in `failed`, as is a row of more than max_pages pages.
+ *   mlora_pages_fork: row r goes on from row parent[r]'s tokens (negative or r: from its own), all rows at once: it gives its own pages back
+ *     and names the parent's.  A parent of n_req or more leaves the row as it is and is counted in `failed`.
+ *   mlora_pages_compact: with n managed pages in use (left in `live`), those that are not among the n lowest managed ids move, in their order,
+ *     to the free ids among these: keys and values of all layers, tables and refs.
+ * k_pages and v_pages: all layers' slabs, [n_layers, n_pages, n_kv_heads, page_tokens, head_dim].  n_req * max_pages <= 2^30, n_pages <= 2^24.
+ * The counterpart of the reference's MemoryManager (lightllm/common/mem_manager.py:4-111) and its request table (req_manager.py:3-36).
+ */
+#define MLORA_PAGES_LAYOUT_WORDS 8
+int mlora_pages_layout(int n_req, int max_pages, int64_t n_pages, int64_t *at);
+int mlora_pages_resize(void *state, int64_t state_words, void *scratch, int64_t scratch_words, const int32_t *want, int n_req, int max_pages,
+                       void *k_pages, void *v_pages, int n_layers, int64_t n_pages, int n_kv_heads, int page_tokens, int head_dim, void *stream);
+int mlora_pages_fork(void *state, int64_t state_words, void *scratch, int64_t scratch_words, const int32_t *parent, int n_req, int max_pages,
+                     int64_t n_pages, int page_tokens, void *stream);
+int mlora_pages_compact(void *state, int64_t state_words, void *scratch, int64_t scratch_words, int n_req, int max_pages,
+                        void *k_pages, void *v_pages, int n_layers, int64_t n_pages, int n_kv_heads, int page_tokens, int head_dim, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
