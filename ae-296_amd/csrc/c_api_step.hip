@@ -393,15 +393,18 @@ int mlora_mx4_values(const void *packed, int64_t packed_bytes, int rows, int k, 
     return launched(mlora::launch_mx4_values(a, dtype, static_cast<hipStream_t>(stream)), "values");
 }
 
-int64_t mlora_mx4_workspace_bytes(int n_proj, const int32_t *hin, const int32_t *hout, int T)
+int mlora_mx4_form(int n_proj, const int32_t *hin, const int32_t *hout, int T, int32_t *shape)
 {
     mlora::Mx4Args a;
     const int rc = mx4_sizes(a, n_proj, hin, hout, T);
-    return rc ? rc : T == 0 ? 0 : mlora::mx4_workspace_bytes(a);
+    if (rc) return rc;
+    if (T == 0 || !shape) return fail(MLORA_EINVAL, "T must be positive and shape not NULL");
+    mlora::mx4_form(a, shape, shape + 1);
+    return MLORA_OK;
 }
 
 int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const void *const *w, const int32_t *hin, const int32_t *hout,
-                         int T, int dtype, int accumulate, void *workspace, int64_t workspace_bytes, void *stream)
+                         int T, int dtype, int accumulate, void *stream)
 {
     if (dtype != MLORA_F16 && dtype != MLORA_BF16) return fail(MLORA_EDTYPE, "dtype must be MLORA_F16 or MLORA_BF16 (got %d)", dtype);
     mlora::Mx4Args a;
@@ -422,10 +425,7 @@ int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const
                 (o < p && overlap(y[p], yp, y[o], (size_t)T * hout[o] * 2)))
                 return fail(MLORA_EINVAL, "projection %d: y overlaps y, x or the weight of projection %d", p, o);
         }
-    const int64_t need = mlora::mx4_workspace_bytes(a);
-    if (need > 0 && (!workspace || workspace_bytes < need)) return fail(MLORA_ENOSPACE, "workspace has %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
-    if (!aligned16(workspace)) return fail(MLORA_EALIGN, "workspace must be 16-byte aligned");
-    return launched(mlora::launch_mx4_gemm(a, dtype, workspace, static_cast<hipStream_t>(stream)), "product");
+    return launched(mlora::launch_mx4_gemm(a, dtype, static_cast<hipStream_t>(stream)), "product");
 }
 
 int mlora_pages_layout(int n_req, int max_pages, int64_t n_pages, int64_t *at)

@@ -713,30 +713,54 @@ void *rows_of(const char *name, const at::Tensor &t, int64_t k, int64_t &stride)
     return t.data_ptr();
 }
 
-// mx4_quantize(x, packed): the packed buffer has the room that x needs, or an error
+at::Tensor new_bytes(int64_t n, const at::Tensor &like)
+{
+    const c10::DeviceGuard device(like.device());
+    return at::empty({n}, like.options().dtype(at::kByte));
+}
+
+// mx4_quantize(x, packed or None) -> (packed, rows, k): the caller's buffer, which must have the room that x needs, or a new one
 PyObject *mx4_quantize(PyObject *const *v, Py_ssize_t nargs)
 {
     if (nargs != 2) raise(PyExc_TypeError, "mx4_quantize takes 2 arguments");
-    const at::Tensor &x = tensor(v[0]), &b = tensor(v[1]);
+    const at::Tensor &x = tensor(v[0]);
     const int dtype = dtype_of(x);
     int64_t stride;
     const void *rows = rows_of("x", x, -1, stride);
+    const int64_t need = mlora_mx4_bytes((int)x.size(0), (int)x.size(1));
+    if (need < 0) return PyLong_FromLong((long)need);
+    at::Tensor b = v[1] == Py_None ? new_bytes(need, x) : tensor(v[1]);
     need_here(b);
     if (b.scalar_type() != at::kByte || !b.is_contiguous()) raise(PyExc_ValueError, "packed must be a contiguous uint8 buffer");
-    return PyLong_FromLong(launch(mlora_mx4_quantize, rows, stride, (int)x.size(0), (int)x.size(1), dtype, b.data_ptr(), b.numel(), stream()));
+    const int rc = launch(mlora_mx4_quantize, rows, stride, (int)x.size(0), (int)x.size(1), dtype, b.data_ptr(), b.numel(), stream());
+    if (rc) return PyLong_FromLong(rc);
+    PyObject *packed = v[1] == Py_None ? THPVariable_Wrap(std::move(b)) : Py_NewRef(v[1]);
+    if (!packed) throw PyFail();
+    return Py_BuildValue("(Nii)", packed, (int)x.size(0), (int)x.size(1));
 }
 
-// mx4_values(packed operand, out)
+// mx4_values(packed operand, out or None, dtype code for a new one) -> out
 PyObject *mx4_values(PyObject *const *v, Py_ssize_t nargs)
 {
-    if (nargs != 2) raise(PyExc_TypeError, "mx4_values takes 2 arguments");
+    if (nargs != 3) raise(PyExc_TypeError, "mx4_values takes 3 arguments");
     const Packed p(v[0]);
-    const at::Tensor &out = tensor(v[1]);
+    at::Tensor out;
+    if (v[1] == Py_None) {
+        const c10::DeviceGuard device(p.t.device());
+        out = at::empty({p.rows, p.k}, p.t.options().dtype(as_int(v[2]) == MLORA_F16 ? at::kHalf : at::kBFloat16));
+    } else {
+        out = tensor(v[1]);
+    }
     const int dtype = dtype_of(out);
     int64_t stride;
     void *rows = rows_of("out", out, p.k, stride);
     if (out.size(0) != p.rows) raise(PyExc_ValueError, "out must have %d rows", p.rows);
-    return PyLong_FromLong(launch(mlora_mx4_values, p.t.data_ptr(), p.t.numel(), p.rows, p.k, rows, stride, dtype, stream()));
+    const int rc = launch(mlora_mx4_values, p.t.data_ptr(), p.t.numel(), p.rows, p.k, rows, stride, dtype, stream());
+    if (rc) return PyLong_FromLong(rc);
+    if (v[1] != Py_None) return Py_NewRef(v[1]);
+    PyObject *o = THPVariable_Wrap(std::move(out));
+    if (!o) throw PyFail();
+    return o;
 }
 
 // mx4_gemm(ys, xs, weights, accumulate)
@@ -766,14 +790,7 @@ PyObject *mx4_gemm(PyObject *const *v, Py_ssize_t nargs)
         y[i] = yt.data_ptr(); x[i] = px.t.data_ptr(); w[i] = pw.t.data_ptr();
         hin[i] = pw.k; hout[i] = pw.rows;
     }
-    // this call's own, as in bgmv_ref
-    const int64_t bytes = mlora_mx4_workspace_bytes((int)n, hin, hout, T);
-    at::DataPtr room;
-    if (bytes > 0) {
-        const c10::DeviceGuard device(ys[0].device());
-        room = c10::GetAllocator(at::kCUDA)->allocate((size_t)bytes);
-    }
-    return PyLong_FromLong(launch(mlora_mx4_gemm_multi, (int)n, y, x, w, hin, hout, T, dtype, (int)is_true(v[3]), room.get(), bytes > 0 ? bytes : 0, stream()));
+    return PyLong_FromLong(launch(mlora_mx4_gemm_multi, (int)n, y, x, w, hin, hout, T, dtype, (int)is_true(v[3]), stream()));
 }
 
 // ---------------------------------------------------------------- page tables

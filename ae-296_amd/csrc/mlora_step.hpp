@@ -187,8 +187,8 @@ int launch_w4_gemv(const W4Args &a, int dtype, hipStream_t s);
 int launch_mx4_quantize(const Mx4QuantArgs &a, int dtype, hipStream_t s);
 int launch_mx4_pack(const Mx4PackArgs &a, hipStream_t s);
 int launch_mx4_values(const Mx4ValuesArgs &a, int dtype, hipStream_t s);
-int64_t mx4_workspace_bytes(const Mx4Args &a);
-int launch_mx4_gemm(const Mx4Args &a, int dtype, void *workspace, hipStream_t s);
+void mx4_form(const Mx4Args &a, int *columns, int *tokens);
+int launch_mx4_gemm(const Mx4Args &a, int dtype, hipStream_t s);
 int launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s);
 int launch_pages_resize(const PagesArgs &a, hipStream_t s);
 int launch_pages_fork(const PagesArgs &a, hipStream_t s);

@@ -94,8 +94,8 @@ SIGNATURES = {
     "mlora_mx4_quantize": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _i64, _vp]),
     "mlora_mx4_pack": (_i32, [_vp, _vp, _i32, _i32, _vp, _i64, _vp]),
     "mlora_mx4_values": (_i32, [_vp, _i64, _i32, _i32, _vp, _i64, _i32, _vp]),
-    "mlora_mx4_workspace_bytes": (_i64, [_i32, _vp, _vp, _i32]),
-    "mlora_mx4_gemm_multi": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "mlora_mx4_form": (_i32, [_i32, _vp, _vp, _i32, _vp]),
+    "mlora_mx4_gemm_multi": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
     "mlora_pages_layout": (_i32, [_i32, _i32, _i64, _vp]),
     "mlora_pages_resize": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _vp]),
     "mlora_pages_fork": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i32, _i64, _i32, _vp]),

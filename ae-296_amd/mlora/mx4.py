@@ -53,30 +53,20 @@ class MX4Tensor:
 
     def values(self, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """What the operand stands for, [rows, k] in a 16-bit type (into `out`, whose rows may be apart): exact for what was quantised from it."""
-        if out is None:
-            _ext.dtype_code(dtype)
-            out = torch.empty((self.rows, self.k), dtype=dtype, device=self.packed.device)
-        rc = _ext.host().mx4_values(self, out)
-        if rc:
-            _ext.check(rc)
-        return out
+        got = _ext.host().mx4_values(self, out, _ext.dtype_code(dtype) if out is None else 0)
+        if type(got) is int:
+            _ext.check(got)
+        return got
 
 
 def mx4_quantize(x: torch.Tensor, out: Optional[MX4Tensor] = None) -> MX4Tensor:
     """A 16-bit tensor [rows, k] (its rows may be apart) in the form above, one launch.  Pass `out` to reuse an operand's buffer, for a batch it was made
     for or a smaller one (no allocation; it is then what is returned)."""
-    if x.dim() != 2:
-        raise ValueError("x must be [rows, k]")
-    rows, k = x.shape
-    if out is None:
-        made = MX4Tensor.__new__(MX4Tensor)
-        made.packed = torch.empty(_packed_bytes(rows, k), dtype=torch.uint8, device=x.device)
-    else:
-        made = out
-    rc = _ext.host().mx4_quantize(x, made.packed)
-    if rc:
-        _ext.check(rc)
-    made.rows, made.k = rows, k           # only now: a refused call leaves `out` what it was
+    got = _ext.host().mx4_quantize(x, None if out is None else out.packed)
+    if type(got) is int:
+        _ext.check(got)
+    made = MX4Tensor.__new__(MX4Tensor) if out is None else out
+    made.packed, made.rows, made.k = got           # only now: a refused call leaves `out` what it was
     return made
 
 
@@ -99,10 +89,8 @@ class MX4Weight(MX4Tensor):
         if w.dim() != 2:
             raise ValueError("expected a weight [hin, hout]")
         made = cls.__new__(cls)
-        made.packed, made.rows, made.k = None, 0, 0
-        t = w.t().contiguous()
-        made.packed = torch.empty(_packed_bytes(*t.shape), dtype=torch.uint8, device=w.device)
-        return mx4_quantize(t, out=made)
+        made.packed = None
+        return mx4_quantize(w.t().contiguous(), out=made)
 
 
 def mx4_gemm(ys: Sequence[torch.Tensor], xs: Sequence[MX4Tensor], ws: Sequence[MX4Tensor], accumulate: bool = False) -> None:

@@ -519,8 +519,8 @@ int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t
  *   mlora_mx4_values: the values a packed operand stands for, rounded to the 16-bit type (exact for what was quantised from that type).
  *   mlora_mx4_gemm_multi takes y (16-bit [T, hout]), x and w (packed), hin and hout as HOST arrays of n_proj entries; no y may overlap another y, an x
  *     or a w.  Products exact, sums in fp32, the result rounded once; a block with a NaN makes its results NaN, and where a sum leaves fp32's range
- *     the result is infinite or NaN.  `workspace`: mlora_mx4_workspace_bytes(...) bytes (0: NULL will do); calls that share it must be ordered on
- *     one stream.
+ *     the result is infinite or NaN.
+ *   mlora_mx4_form: the output columns (shape[0]) and tokens (shape[1]) of a workgroup of such a call.  Informational.
  * rows <= 2^20 where they are tokens (T), 2^24 otherwise; k <= 2^24.  The counterpart of the reference's quantised base GEMMs with quantised
  * activations (quantize_gemm_int8.py:18,109), in the format of the 4-bit matrix instructions.
  */
@@ -528,9 +528,9 @@ int64_t mlora_mx4_bytes(int rows, int k);
 int mlora_mx4_quantize(const void *x, int64_t x_stride, int rows, int k, int dtype, void *packed, int64_t packed_bytes, void *stream);
 int mlora_mx4_pack(const uint8_t *codes, const uint8_t *scales, int rows, int k, void *packed, int64_t packed_bytes, void *stream);
 int mlora_mx4_values(const void *packed, int64_t packed_bytes, int rows, int k, void *out, int64_t out_stride, int dtype, void *stream);
-int64_t mlora_mx4_workspace_bytes(int n_proj, const int32_t *hin, const int32_t *hout, int T);
+int mlora_mx4_form(int n_proj, const int32_t *hin, const int32_t *hout, int T, int32_t *shape);
 int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const void *const *w, const int32_t *hin, const int32_t *hout,
-                         int T, int dtype, int accumulate, void *workspace, int64_t workspace_bytes, void *stream);
+                         int T, int dtype, int accumulate, void *stream);
 
 /*
  * Page tables that live on the device: n_req rows of max_pages page ids each (what page_tbl of the calls above takes), the tokens of every row and

@@ -117,6 +117,37 @@ def test_a_weight_is_quantised_along_its_input():
     same(ref.f64(m.values(BF16)), ref.values(*ref.quantize(ref.f64(w.t()))))
 
 
+def test_refusals_on_the_device():
+    say("mx4 refusals")
+    x = torch.zeros((4, 64), dtype=F16, device="cuda")
+    q = mlora.mx4_quantize(x)
+    for bad in (x[:, :12], x[:, 4:]):                              # a width, and an address
+        with pytest.raises(mlora.MloraError):
+            mlora.mx4_quantize(bad)
+    for bad in (x.t(), x[0], x.unsqueeze(0)):
+        with pytest.raises(ValueError):
+            mlora.mx4_quantize(bad)
+    with pytest.raises(TypeError):
+        mlora.mx4_quantize(x.float())
+    with pytest.raises(mlora.MloraError):
+        mlora.mx4_quantize(torch.zeros((40, 64), dtype=F16, device="cuda"), out=q)
+    assert (q.rows, q.k) == (4, 64)                                # what it was
+    with pytest.raises(TypeError):
+        q.values(torch.float32)
+    with pytest.raises(ValueError):
+        q.values(out=x[:3])
+    w, y = mlora.MX4Weight.quantize(torch.zeros((64, 16), dtype=F16, device="cuda")), torch.zeros((4, 16), dtype=F16, device="cuda")
+    for ys, xs, ws in (([y, y], [q], [w]), ([y[:3]], [q], [w]), ([y[:, :8]], [q], [w]), ([y], [mlora.mx4_quantize(x[:, :32])], [w]), ([y] * 9, [q] * 9, [w] * 9)):
+        with pytest.raises(ValueError):
+            mlora.mx4_gemm(ys, xs, ws)
+    with pytest.raises(TypeError):
+        mlora.mx4_gemm([y.float()], [q], [w])
+    with pytest.raises(TypeError):
+        mlora.mx4_gemm([y, y.bfloat16()], [q, q], [w, w])
+    with pytest.raises(mlora.MloraError):
+        mlora.mx4_gemm([y, y], [q, q], [w, w])                     # one y twice
+
+
 def test_no_rows():
     say("mx4 no rows")
     q = mlora.mx4_quantize(torch.empty((0, 64), dtype=F16, device="cuda"))

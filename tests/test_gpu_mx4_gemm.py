@@ -1,4 +1,6 @@
 """Products of microscaled 4-bit operands against the 64-bit product of the values they stand for."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -6,6 +8,7 @@ import torch
 import mlora
 import mx4_ref as ref
 from gpu_common import say
+from mlora import _ext
 from step_ref import check, store_bound
 
 pytestmark = pytest.mark.gpu
@@ -60,6 +63,29 @@ def test_output_widths(n):
     run(2, 256, n, F16, seed=n)
     run(40, 256, n, F16, seed=n)
     run(260, 256, n, BF16, seed=n)
+
+
+FORMS = {(16, 16): (17, 136, 72), (32, 16): (17, 136, 2056), (16, 32): (50, 2184, 1032), (32, 32): (50, 1032, 2056), (32, 64): (257, 1032, 1032), (64, 64): (201, 2184, 2056),
+         (128, 64): (300, 136, 2056), (128, 128): (1030, 136, 2056), (128, 256): (1030, 1160, 4104), (256, 256): (1030, 2184, 8200)}
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("form", FORMS)
+def test_every_form(form, dtype, accumulate):
+    """Sizes that end inside a block, a tile, a quad of tiles and a workgroup's columns and tokens."""
+    T, k, n = FORMS[form]
+    shape = (C.c_int32 * 2)()
+    assert _ext.lib().mlora_mx4_form(1, (C.c_int32 * 1)(k), (C.c_int32 * 1)(n), T, shape) == 0 and tuple(shape) == form
+    run(T, k, n, dtype, accumulate=accumulate)
+
+
+@pytest.mark.parametrize("k", [8, 128, 256, 384, 512, 640, 768, 896, 1024, 1152, 2176])
+def test_steps_of_the_large_tiles(k):
+    """Every number of steps on either side of a ring's four stages."""
+    say(f"large tiles k={k}")
+    for T, n in ((1100, 8200), (1030, 4104), (1030, 2056), (300, 2056)):
+        run(T, k, n, BF16, seed=k)
 
 
 @pytest.mark.parametrize("T", [1, 20, 100, 300])

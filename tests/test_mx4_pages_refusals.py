@@ -55,7 +55,7 @@ def test_pack_arguments(kw, code):
 def gemm(**kw):
     a = dict(n=2, y=ptrs(1 << 20, 2 << 20, *[16] * 6), x=ptrs(3 << 20, 3 << 20, *[16] * 6), w=ptrs(4 << 20, 5 << 20, *[16] * 6), hin=ints(64), hout=ints(64), T=3, dtype=0)
     a.update(kw)
-    return _ext.lib().mlora_mx4_gemm_multi(a["n"], a["y"], a["x"], a["w"], a["hin"], a["hout"], a["T"], a["dtype"], 0, None, 0, None)
+    return _ext.lib().mlora_mx4_gemm_multi(a["n"], a["y"], a["x"], a["w"], a["hin"], a["hout"], a["T"], a["dtype"], 0, None)
 
 
 @pytest.mark.parametrize("kw, code", [
@@ -68,20 +68,13 @@ def test_gemm_arguments(kw, code):
     assert gemm(**kw) == code
 
 
-def test_workspace_size_arguments():
-    size = _ext.lib().mlora_mx4_workspace_bytes
-    assert size(1, ints(64), ints(64), 0) == 0 and size(1, ints(64), ints(64), 1) >= 0
-    assert size(0, ints(64), ints(64), 1) == ERANGE and size(1, ints(60), ints(64), 1) == EALIGN and size(1, ints(64), None, 1) == EINVAL
-
-
-def test_a_workspace_too_small_is_refused():
-    lib, T = _ext.lib(), 200
-    hin, hout = ints(16384), ints(64)
-    need = lib.mlora_mx4_workspace_bytes(1, hin, hout, T)
-    args = lambda ws, n: (1, ptrs(1 << 30), ptrs(1 << 31), ptrs(1 << 32), hin, hout, T, 0, 0, ws, n, None)          # noqa: E731
-    if need:
-        assert lib.mlora_mx4_gemm_multi(*args(None, need)) == ENOSPACE and lib.mlora_mx4_gemm_multi(*args(one, need - 1)) == ENOSPACE
-        assert lib.mlora_mx4_gemm_multi(*args(off, need)) == EALIGN
+def test_form_arguments():
+    form, shape = _ext.lib().mlora_mx4_form, (C.c_int32 * 2)()
+    assert form(1, ints(4096), ints(4096), 1, shape) == OK and list(shape) == [16, 16]
+    assert form(2, ints(5120), ints(13824), 8000, shape) == OK and list(shape) == [256, 256]
+    assert form(1, ints(64), ints(64), 1 << 20, shape) == OK and form(8, ints(1 << 24), ints(1 << 24), 1 << 20, shape) == OK
+    assert form(0, ints(64), ints(64), 1, shape) == ERANGE and form(1, ints(60), ints(64), 1, shape) == EALIGN
+    assert form(1, ints(64), ints(64), 0, shape) == EINVAL and form(1, ints(64), ints(64), 1, None) == EINVAL
 
 
 def test_operands_from_python():
@@ -95,8 +88,6 @@ def test_operands_from_python():
             bad()
     with pytest.raises(TypeError):
         mlora.mx4_quantize(torch.zeros((2, 8)))
-    with pytest.raises(_ext.MloraError):
-        mlora.mx4_quantize(torch.zeros((2, 12)).half())
     with pytest.raises(_ext.MloraError):
         mlora.MX4Tensor(c[:, :31], s)
     with pytest.raises(ValueError):
