@@ -150,7 +150,7 @@ int pages_args(mlora::PagesArgs &a, void *state, int64_t state_words, void *scra
     a.free_bits = s; a.table = s + l.table; a.lens = s + l.lens; a.refs = s + l.refs; a.failed = s + l.failed; a.live = s + l.live;
     a.managed = c; a.head = c + l.head; a.writers = c + l.writers; a.last_writer = c + l.last_writer; a.picked = c + l.picked;
     a.move_from = c + l.move_from; a.word_movers = c + l.word_movers; a.word_rank = c + l.word_rank; a.row_page = c + l.row_page;
-    a.row_new = c + l.row_new; a.copies = c + l.copies; a.rows = c + l.rows;
+    a.row_new = c + l.row_new; a.copies = c + l.copies; a.rows = c + l.rows; a.pieces = c + l.pieces;
     a.want = want; a.n_pages = n_pages; a.n_req = n_req; a.max_pages = max_pages; a.page_shift = log2_exact(page_tokens);
     return MLORA_OK;
 }
@@ -431,8 +431,8 @@ int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const
 int mlora_pages_layout(int n_req, int max_pages, int64_t n_pages, int64_t *at)
 {
     if (n_req <= 0 || max_pages <= 0 || n_pages <= 0) return fail(MLORA_EINVAL, "n_req, max_pages and n_pages must be positive (got %d, %d, %lld)", n_req, max_pages, (long long)n_pages);
-    if ((int64_t)n_req * max_pages > (1 << 30) || n_req > (1 << 24) || n_pages > (1 << 24))
-        return fail(MLORA_ERANGE, "at most 2^24 rows and pages and 2^30 table entries (got %d, %lld, %lld)", n_req, (long long)n_pages, (long long)n_req * max_pages);
+    if ((int64_t)n_req * max_pages > (1 << 30) || n_req > (1 << 20) || n_pages > (1 << 24))
+        return fail(MLORA_ERANGE, "at most 2^20 rows, 2^24 pages and 2^30 table entries (got %d, %lld, %lld)", n_req, (long long)n_pages, (long long)n_req * max_pages);
     if (!at) return fail(MLORA_EINVAL, "at must not be NULL");
     const mlora::PagesLayout l = mlora::pages_layout(n_req, max_pages, n_pages);
     const int64_t words[MLORA_PAGES_LAYOUT_WORDS] = {0, l.table, l.lens, l.refs, l.failed, l.live, l.state_words, l.scratch_words};

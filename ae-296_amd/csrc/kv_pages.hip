@@ -14,8 +14,10 @@
 namespace mlora {
 
 constexpr int ASSIGN_NT = 1024;
+constexpr long long RELEASE_ENTRIES = 1 << 17;
 
 __device__ __forceinline__ int read_now(const int32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ unsigned long long read_now(const unsigned long long *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ int pages_of(int tokens, int shift, int most)
 {
     if (tokens <= 0) return 0;
@@ -31,22 +33,31 @@ __device__ __forceinline__ void drop_page(const PagesArgs &p, int page)
     if (page >= 0 && page < p.n_pages && atomicSub(p.refs + page, 1) == 1) set_free(p, page);
 }
 
-// Exclusive sum over the workgroup's ASSIGN_NT threads; `total` is everyone's.  Two barriers.
-__device__ __forceinline__ unsigned block_scan(unsigned v, unsigned *lds, unsigned &total)
+// A barrier behind which the workgroup's atomics and stores have been made.
+__device__ __forceinline__ void settled_barrier()
+{
+    __builtin_amdgcn_s_waitcnt(0x0f70);                  // vector memory
+    __syncthreads();
+}
+
+struct Sums { unsigned a, b; };
+// Exclusive sums of two values over the workgroup's ASSIGN_NT threads; `total` is everyone's.  Two barriers.
+__device__ __forceinline__ Sums block_scan(Sums v, Sums *lds, Sums &total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const unsigned upto = wave_scan(v);
+    const Sums upto = {wave_scan(v.a), wave_scan(v.b)};
     if (lane == 63) lds[wave] = upto;
     __syncthreads();
-    unsigned before = 0;
-    total = 0;
+    Sums before = {0, 0};
+    total = {0, 0};
+#pragma unroll
     for (int i = 0; i < ASSIGN_NT / 64; i++) {
-        const unsigned s = lds[i];
-        if (i < wave) before += s;
-        total += s;
+        const Sums s = lds[i];
+        if (i < wave) { before.a += s.a; before.b += s.b; }
+        total.a += s.a; total.b += s.b;
     }
     __syncthreads();
-    return before + upto - v;
+    return {before.a + upto.a - v.a, before.b + upto.b - v.b};
 }
 
 // ------------------------------------------------------------------ resize
@@ -67,111 +78,210 @@ __global__ __launch_bounds__(256) void pages_release_kernel(const PagesArgs p)
     if (lane == 0) p.lens[r] = want;
 }
 
-struct GrowRow { bool longer, fits; int old, want, had, gets, part, at; };
+struct GrowRow { bool shorter, longer, fits; int old, want, had, gets, part, at; };
 __device__ __forceinline__ GrowRow grow_row(const PagesArgs &p, int r)
 {
-    GrowRow g;
+    GrowRow g = {};
+    if (r >= p.n_req) return g;
     g.old = p.lens[r]; g.want = p.want[r];
     if (g.old < 0) g.old = 0;
+    g.shorter = g.want >= 0 && g.want < g.old;
     g.longer = g.want > g.old;
     g.fits = g.longer && (long long)g.want <= (long long)p.max_pages << p.page_shift;
     g.had = pages_of(g.old, p.page_shift, p.max_pages);
-    g.gets = g.fits ? pages_of(g.want, p.page_shift, p.max_pages) : g.had;
+    g.gets = g.fits || g.shorter ? pages_of(g.want, p.page_shift, p.max_pages) : g.had;
     g.part = g.old & ((1 << p.page_shift) - 1);
     g.at = g.old >> p.page_shift;
     return g;
 }
 
-// Everything that depends on the order of the rows, in one workgroup.
+// Calls f(rank, page) for every set bit of the wavefront's words, a word at a time, a lane a bit: rank counts the bits from the word's own on, and
+// `word` of lane l is the bits of the 64 pages from 64 (first + l) on.  (A thread for each word takes its up to 64 bits one after the other: 3 us.)
+template <typename F>
+__device__ __forceinline__ void each_bit(unsigned long long word, unsigned rank, int first, F f)
+{
+    const int lane = threadIdx.x & 63;
+    for (uint64_t left = __ballot(word != 0); left; left &= left - 1) {
+        const int from = __builtin_ctzll(left);
+        const unsigned long long w = (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(word >> 32), from) << 32 | (unsigned)__builtin_amdgcn_readlane((int)word, from);
+        const unsigned r = (unsigned)__builtin_amdgcn_readlane((int)rank, from);
+        if (w >> lane & 1) f(r + (unsigned)__builtin_popcountll(w & ((1ull << lane) - 1)), (first + from) * 64 + lane);
+    }
+}
+
+// Everything that depends on the order of the rows, in one workgroup, a thread a row at a time.  ONE: no more rows than threads, which then keep theirs
+// in registers.  RELEASE: pages are given back here as well, and there is no launch before this one.
+// Bound by chains of dependent loads, each a way to the last-level cache (the tables were written on other XCDs): lengths -> the row's last page -> its count, the bits
+// beside them, and where pages are given back or shared the same again behind that.
+constexpr unsigned HELD_PICKS = 2048;
+template <bool ONE, bool RELEASE>
 __global__ __launch_bounds__(ASSIGN_NT) void pages_assign_kernel(const PagesArgs p)
 {
-    __shared__ unsigned lds[ASSIGN_NT / 64];
-    __shared__ unsigned granted, failed, copies;
-    const int tid = threadIdx.x;
+    __shared__ Sums lds[ASSIGN_NT / 64];
+    __shared__ unsigned drops_upto[ASSIGN_NT];
+    __shared__ int drops_end[ASSIGN_NT];
+    __shared__ int picks[HELD_PICKS];                       // the first of the picked ids
+    __shared__ unsigned granted, failed, copies, widest;
+    const int tid = threadIdx.x, wave = tid >> 6;
     const int words = (int)((p.n_pages + 63) >> 6);
     unsigned long long *bits = reinterpret_cast<unsigned long long *>(p.free_bits);
-    if (tid == 0) { granted = 0; failed = 0; copies = 0; }
-    // which rows write on pages that others name, and how many rows do so on each
-    for (int r = tid; r < p.n_req; r += ASSIGN_NT) {
-        const GrowRow g = grow_row(p, r);
-        int page = -1;
-        if (g.fits && g.part) {
-            page = p.table[(size_t)r * p.max_pages + g.at];
-            if (page < 0 || page >= p.n_pages || p.refs[page] <= 1) page = -1;
+    if (tid == 0) { granted = 0; failed = 0; copies = 0; widest = 0; }
+    unsigned long long word = tid < words ? bits[tid] : 0ull;
+    const GrowRow mine = grow_row(p, tid);
+    // the page a row will write on, if it has tokens of the row already, and the entries that name it
+    auto written = [&](const GrowRow &g, int r) {
+        const int page = g.fits && g.part ? p.table[(size_t)r * p.max_pages + g.at] : -1;
+        return page >= 0 && page < p.n_pages ? page : -1;
+    };
+    const int my_page = written(mine, tid);
+    int my_refs = my_page >= 0 ? p.refs[my_page] : 0;
+    Sums total;
+    bool dropped = false;
+    if constexpr (RELEASE) {
+        for (int r0 = 0; r0 < p.n_req; r0 += ASSIGN_NT) {
+            const GrowRow g = ONE || r0 == 0 ? mine : grow_row(p, r0 + tid);
+            const unsigned n = g.shorter ? (unsigned)(g.had - g.gets) : 0u;
+            if (__syncthreads_or(n > 0)) {
+                dropped = true;
+                const unsigned first = block_scan({n, 0}, lds, total).a;
+                drops_upto[tid] = first + n;
+                drops_end[tid] = g.had - (int)(first + n);
+                __syncthreads();
+                for (unsigned i = tid; i < total.a; i += ASSIGN_NT) {
+                    int row = 0;                            // the first whose drops go beyond i
+#pragma unroll
+                    for (int s = ASSIGN_NT / 2; s; s >>= 1)
+                        if (drops_upto[row + s - 1] <= i) row += s;
+                    int32_t *entry = p.table + (size_t)(r0 + row) * p.max_pages + (drops_end[row] + (int)i);
+                    const int page = *entry;
+                    *entry = -1;
+                    drop_page(p, page);
+                }
+                settled_barrier();
+            }
+            if (g.shorter) p.lens[r0 + tid] = g.want;
         }
-        p.row_page[r] = page;
+        if (dropped) {                                      // counts and bits are others now
+            if (my_page >= 0) my_refs = read_now(p.refs + my_page);
+            if (tid < words) word = read_now(bits + tid);
+        }
+    }
+    // which rows write on pages that others name, and how many rows do so on each
+    int page = my_refs > 1 ? my_page : -1;
+    bool sharing = false;
+    for (int r0 = 0; r0 < p.n_req; r0 += ASSIGN_NT) {
+        const int r = r0 + tid;
+        if (!ONE) {
+            page = written(grow_row(p, r), r);
+            if (page >= 0 && read_now(p.refs + page) <= 1) page = -1;
+            if (r < p.n_req) p.row_page[r] = page;
+        }
         if (page >= 0) {
             atomicAdd(p.writers + page, 1);
             atomicMax(p.last_writer + page, r + 1);
+            sharing = true;
         }
     }
-    unsigned mine = 0, n_free;
-    for (int w = tid; w < words; w += ASSIGN_NT) mine += __builtin_popcountll(bits[w]);
-    block_scan(mine, lds, n_free);
+    __builtin_amdgcn_s_waitcnt(0x0f70);                  // behind the barrier the writers' counts can be read
+    const bool any_sharing = __syncthreads_or(sharing);
+    unsigned count = (unsigned)__builtin_popcountll(word), n_free = 0, word_rank = 0;
+    for (int w = tid + ASSIGN_NT; w < words; w += ASSIGN_NT) count += (unsigned)__builtin_popcountll(read_now(bits + w));
     // the rows' needs in their order
     unsigned before = 0;
+    GrowRow g = mine;
+    unsigned gets = 0, new_at = 0;
     for (int r0 = 0; r0 < p.n_req; r0 += ASSIGN_NT) {
         const int r = r0 + tid;
-        GrowRow g = {};
-        int page = -1;
-        bool copy = false;
-        if (r < p.n_req) {
+        if (!ONE) {
             g = grow_row(p, r);
-            page = p.row_page[r];
-            copy = page >= 0 && !(read_now(p.writers + page) == p.refs[page] && read_now(p.last_writer + page) == r + 1);
+            page = any_sharing && r < p.n_req ? p.row_page[r] : -1;
         }
-        const unsigned need = (unsigned)(g.gets - g.had) + (copy ? 1u : 0u);
-        unsigned sum;
-        const unsigned first = before + block_scan(need, lds, sum), upto = first + need;
-        before += sum;
+        bool copy = false;
+        if (any_sharing && page >= 0) copy = !(read_now(p.writers + page) == read_now(p.refs + page) && read_now(p.last_writer + page) == r + 1);
+        const unsigned need = g.fits ? (unsigned)(g.gets - g.had) + (copy ? 1u : 0u) : 0u;
+        const Sums s = block_scan({need, r0 == 0 ? count : 0u}, lds, total);
+        if (r0 == 0) { n_free = total.b; word_rank = s.b; }
+        const unsigned first = before + s.a, upto = first + need;
+        before += total.a;
         const bool served = g.fits && (upto <= n_free || (need == 0 && page < 0));
         if (g.longer && !served) atomicAdd(&failed, 1u);
-        if (served && upto <= n_free) atomicMax(&granted, upto);
-        if (r < p.n_req) {
-            p.row_new[3 * r] = served ? g.gets - g.had : 0;
+        gets = served ? (unsigned)(g.gets - g.had) : 0u;
+        new_at = first + (copy ? 1u : 0u);
+        if (served && need) atomicMax(&granted, upto);
+        if (gets > 4) atomicMax(&widest, gets);
+        if (served) p.lens[r] = g.want;
+        if (served && copy) {
+            int32_t *job = p.copies + 5 * atomicAdd(&copies, 1u);
+            job[0] = page; job[1] = (int)first; job[2] = g.part; job[3] = r; job[4] = g.at;
+        }
+        if (!ONE && r < p.n_req) {
+            p.row_new[3 * r] = (int)gets;
             p.row_new[3 * r + 1] = g.had;
-            p.row_new[3 * r + 2] = (int)(first + (copy ? 1u : 0u));
-            if (served) p.lens[r] = g.want;
-            if (served && copy) {
-                int32_t *job = p.copies + 5 * atomicAdd(&copies, 1u);
-                job[0] = page; job[1] = (int)first; job[2] = g.part; job[3] = r; job[4] = g.at;
-            }
+            p.row_new[3 * r + 2] = (int)new_at;
         }
     }
     __syncthreads();
     // the lowest free ids, as many as are granted
     const unsigned n = granted;
+    const bool wide = widest > 0;
     unsigned done = 0;
     for (int w0 = 0; w0 < words && done < n; w0 += ASSIGN_NT) {
         const int w = w0 + tid;
-        unsigned long long word = w < words ? bits[w] : 0ull;
-        unsigned sum;
-        unsigned rank = done + block_scan((unsigned)__builtin_popcountll(word), lds, sum);
-        done += sum;
-        if (word && rank < n) {
-            do {
-                p.picked[rank++] = w * 64 + __builtin_ctzll(word);
-                word &= word - 1;
-            } while (word && rank < n);
+        unsigned rank = word_rank;
+        if (words > ASSIGN_NT) {
+            if (w0 > 0) word = w < words ? read_now(bits + w) : 0ull;
+            rank = done + block_scan({(unsigned)__builtin_popcountll(word), 0}, lds, total).a;
+            done += total.a;
+        } else {
+            done = n;
+        }
+        if (rank >= n) word = 0;
+        each_bit(word, rank, w0 + wave * 64, [&](unsigned nth, int id) {
+            if (nth >= n) return;
+            if (nth < HELD_PICKS) picks[nth] = id;
+            if (wide || n > HELD_PICKS) p.picked[nth] = id;
+        });
+        if (word) {
+            const unsigned here = (unsigned)__builtin_popcountll(word);
+            if (here <= n - rank) word = 0;
+            else for (unsigned i = rank; i < n; i++) word &= word - 1;
             bits[w] = word;
         }
     }
-    __syncthreads();
-    for (int r = tid; r < p.n_req; r += ASSIGN_NT) {
-        const int page = p.row_page[r];
-        if (page >= 0) { p.writers[page] = 0; p.last_writer[page] = 0; }
+    settled_barrier();
+    auto pick = [&](unsigned nth) { return nth < HELD_PICKS ? picks[nth] : p.picked[nth]; };
+    if (any_sharing) {
+        for (int r = tid; r < p.n_req; r += ASSIGN_NT) {
+            if (!ONE) page = p.row_page[r];
+            if (page >= 0) { p.writers[page] = 0; p.last_writer[page] = 0; }
+        }
+        for (unsigned c = tid; c < copies; c += ASSIGN_NT) {
+            int32_t *job = p.copies + 5 * c;
+            const int to = pick((unsigned)job[1]);
+            job[1] = to;
+            p.table[(size_t)job[3] * p.max_pages + job[4]] = to;
+            p.refs[to] = 1;
+            atomicSub(p.refs + job[0], 1);
+        }
     }
-    for (unsigned c = tid; c < copies; c += ASSIGN_NT) {
-        int32_t *job = p.copies + 5 * c;
-        const int to = p.picked[job[1]];
-        job[1] = to;
-        p.table[(size_t)job[3] * p.max_pages + job[4]] = to;
-        p.refs[to] = 1;
-        atomicSub(p.refs + job[0], 1);
+    // a few new pages a row enter their tables here, more by the next launch
+    auto enter = [&](int r, int had, unsigned from, unsigned many) {
+        for (unsigned i = 0; i < many; i++) {
+            const int id = pick(from + i);
+            p.table[(size_t)r * p.max_pages + had + (int)i] = id;
+            p.refs[id] = 1;
+        }
+    };
+    if (ONE) {
+        if (!wide) enter(tid, g.had, new_at, gets);
+        else if (tid < p.n_req) { p.row_new[3 * tid] = (int)gets; p.row_new[3 * tid + 1] = g.had; p.row_new[3 * tid + 2] = (int)new_at; }
+    } else if (n && !wide) {
+        for (int r = tid; r < p.n_req; r += ASSIGN_NT) enter(r, p.row_new[3 * r + 1], (unsigned)p.row_new[3 * r + 2], (unsigned)p.row_new[3 * r]);
     }
     if (tid == 0) {
         p.head[0] = (int)copies;
-        *p.failed += (int)failed;
+        p.head[1] = wide;
+        if (failed) *p.failed += (int)failed;
     }
 }
 
@@ -188,18 +298,18 @@ __device__ __forceinline__ void copy_tokens(const PagesArgs &p, long long unit, 
     }
 }
 
-// The rows' new pages enter their tables, and shared pages are copied: all that is wide.
+// What is wide: many new pages a row enter their tables, and shared pages are copied.
 __global__ __launch_bounds__(256) void pages_fill_kernel(const PagesArgs p)
 {
-    const int lane = threadIdx.x & 63;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < p.n_req; r += gridDim.x * 4) {
-        const int n = p.row_new[3 * r], had = p.row_new[3 * r + 1], first = p.row_new[3 * r + 2];
-        for (int i = lane; i < n; i += 64) {
-            const int page = p.picked[first + i];
-            p.table[(size_t)r * p.max_pages + had + i] = page;
-            p.refs[page] = 1;
+    if (p.head[1])
+        for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < p.n_req; r += gridDim.x * 4) {
+            const int n = p.row_new[3 * r], had = p.row_new[3 * r + 1], first = p.row_new[3 * r + 2];
+            for (int i = threadIdx.x & 63; i < n; i += 64) {
+                const int page = p.picked[first + i];
+                p.table[(size_t)r * p.max_pages + had + i] = page;
+                p.refs[page] = 1;
+            }
         }
-    }
     const long long per = 2ll * p.n_layers, units = p.head[0] * per;
     for (long long u = blockIdx.x; u < units; u += gridDim.x) {
         const int32_t *job = p.copies + 5 * (u / per);
@@ -209,10 +319,15 @@ __global__ __launch_bounds__(256) void pages_fill_kernel(const PagesArgs p)
 
 int launch_pages_resize(const PagesArgs &a, hipStream_t s)
 {
-    const unsigned rows = (unsigned)(a.n_req + 3) / 4;
-    hipLaunchKernelGGL(pages_release_kernel, dim3(rows), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(pages_assign_kernel, dim3(1), dim3(ASSIGN_NT), 0, s, a);
-    hipLaunchKernelGGL(pages_fill_kernel, dim3(4u * device_compute_units()), dim3(256), 0, s, a);
+    // Pages are given back by the workgroup that hands them out, 1024 at a time, or by a launch of their own
+    const bool release = (long long)a.n_req * a.max_pages <= RELEASE_ENTRIES, one = a.n_req <= ASSIGN_NT;
+    if (!release) hipLaunchKernelGGL(pages_release_kernel, dim3((unsigned)(a.n_req + 3) / 4), dim3(256), 0, s, a);
+    if (one && release) hipLaunchKernelGGL((pages_assign_kernel<true, true>), dim3(1), dim3(ASSIGN_NT), 0, s, a);
+    else if (one) hipLaunchKernelGGL((pages_assign_kernel<true, false>), dim3(1), dim3(ASSIGN_NT), 0, s, a);
+    else if (release) hipLaunchKernelGGL((pages_assign_kernel<false, true>), dim3(1), dim3(ASSIGN_NT), 0, s, a);
+    else hipLaunchKernelGGL((pages_assign_kernel<false, false>), dim3(1), dim3(ASSIGN_NT), 0, s, a);
+    const long long units = 2ll * a.n_layers * a.n_req, most = 8ll * device_compute_units();
+    hipLaunchKernelGGL(pages_fill_kernel, dim3((unsigned)(units < most ? units : most)), dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }
 
@@ -224,47 +339,70 @@ __device__ __forceinline__ int parent_of(const PagesArgs &p, int r)
     return of >= 0 && of < p.n_req && of != r ? of : -1;
 }
 
-// What the rows will be, from what all rows are: kept aside, with the new holders counted, before any row changes.  -2: as it is.
+// What the rows will be, from what all rows are: kept aside, with the new holders counted, before any row changes.  A workgroup a piece of FORK_PIECE entries of a
+// row; a piece that is the parent's already, as most of beams are, is marked and not copied, and so are single entries (-2).
 __global__ __launch_bounds__(256) void pages_fork_kernel(const PagesArgs p)
 {
-    const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (r >= p.n_req) return;
-    if (p.want[r] >= p.n_req && lane == 0) atomicAdd(p.failed, 1);
+    const int pieces = (p.max_pages + FORK_PIECE - 1) / FORK_PIECE, r = blockIdx.x / pieces, i0 = (blockIdx.x - r * pieces) * FORK_PIECE;
+    if (p.want[r] >= p.n_req && i0 == 0 && threadIdx.x == 0) atomicAdd(p.failed, 1);
     const int of = parent_of(p, r);
     if (of < 0) return;
-    const int had = pages_of(p.lens[r], p.page_shift, p.max_pages), gets = pages_of(p.lens[of], p.page_shift, p.max_pages);
+    const int tokens = p.lens[of], had = pages_of(p.lens[r], p.page_shift, p.max_pages), gets = pages_of(tokens, p.page_shift, p.max_pages);
     const int32_t *mine = p.table + (size_t)r * p.max_pages, *its = p.table + (size_t)of * p.max_pages;
-    for (int i = lane; i < gets; i += 64) {
-        const int page = its[i];
-        const bool same = i < had && mine[i] == page;
-        p.rows[(size_t)r * p.max_pages + i] = same ? -2 : page;
-        if (!same && page >= 0 && page < p.n_pages) atomicAdd(p.refs + page, 1);
+    int page[FORK_PIECE / 256];
+    bool differs = false;
+#pragma unroll
+    for (int u = 0; u < FORK_PIECE / 256; u++) {
+        const int i = i0 + u * 256 + threadIdx.x;
+        page[u] = i < gets ? its[i] : -1;
+        if (i >= had ? i >= gets : page[u] == mine[i]) page[u] = -2;
+        differs |= page[u] != -2;
     }
-    if (lane == 0) p.row_page[r] = p.lens[of];
+    const int any = __syncthreads_or(differs);
+    if (any) {
+#pragma unroll
+        for (int u = 0; u < FORK_PIECE / 256; u++) {
+            const int i = i0 + u * 256 + threadIdx.x;
+            if (i < p.max_pages) p.rows[(size_t)r * p.max_pages + i] = page[u];
+            if (page[u] >= 0 && page[u] < p.n_pages) atomicAdd(p.refs + page[u], 1);
+        }
+    }
+    if (threadIdx.x == 0) {
+        p.pieces[blockIdx.x] = any;
+        if (i0 == 0) p.row_page[r] = tokens;
+    }
 }
 
 __global__ __launch_bounds__(256) void pages_forked_kernel(const PagesArgs p)
 {
-    const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (r >= p.n_req) return;
+    const int pieces = (p.max_pages + FORK_PIECE - 1) / FORK_PIECE, r = blockIdx.x / pieces, i0 = (blockIdx.x - r * pieces) * FORK_PIECE;
     if (parent_of(p, r) < 0) return;
     const int tokens = p.row_page[r];
-    const int had = pages_of(p.lens[r], p.page_shift, p.max_pages), gets = pages_of(tokens, p.page_shift, p.max_pages);
-    int32_t *mine = p.table + (size_t)r * p.max_pages;
-    for (int i = lane; i < (had > gets ? had : gets); i += 64) {
-        const int page = i < gets ? p.rows[(size_t)r * p.max_pages + i] : -1;
-        if (page == -2) continue;
-        if (i < had) drop_page(p, mine[i]);
-        mine[i] = page;
+    if (p.pieces[blockIdx.x]) {
+        int32_t *mine = p.table + (size_t)r * p.max_pages;
+        const int32_t *next = p.rows + (size_t)r * p.max_pages;
+        int page[FORK_PIECE / 256], old[FORK_PIECE / 256];
+#pragma unroll
+        for (int u = 0; u < FORK_PIECE / 256; u++) {
+            const int i = i0 + u * 256 + threadIdx.x;
+            page[u] = i < p.max_pages ? next[i] : -2;
+            old[u] = i < p.max_pages ? mine[i] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < FORK_PIECE / 256; u++) {
+            if (page[u] == -2) continue;
+            mine[i0 + u * 256 + threadIdx.x] = page[u];
+            drop_page(p, old[u]);
+        }
     }
-    if (lane == 0) p.lens[r] = tokens;
+    if (i0 == 0 && threadIdx.x == 0) p.lens[r] = tokens;
 }
 
 int launch_pages_fork(const PagesArgs &a, hipStream_t s)
 {
-    const unsigned rows = (unsigned)(a.n_req + 3) / 4;
-    hipLaunchKernelGGL(pages_fork_kernel, dim3(rows), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(pages_forked_kernel, dim3(rows), dim3(256), 0, s, a);
+    const dim3 grid((unsigned)a.n_req * (unsigned)((a.max_pages + FORK_PIECE - 1) / FORK_PIECE));
+    hipLaunchKernelGGL(pages_fork_kernel, grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL(pages_forked_kernel, grid, dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }
 
@@ -272,50 +410,52 @@ int launch_pages_fork(const PagesArgs &a, hipStream_t s)
 // Which pages move where: with n pages in use, those beyond the n-th of all managed ids go, in their order, to the free ones before it.
 __global__ __launch_bounds__(ASSIGN_NT) void pages_moves_kernel(const PagesArgs p)
 {
-    __shared__ unsigned lds[ASSIGN_NT / 64];
+    __shared__ Sums lds[ASSIGN_NT / 64];
     __shared__ int border;
     const int tid = threadIdx.x;
     const int words = (int)((p.n_pages + 63) >> 6);
     unsigned long long *bits = reinterpret_cast<unsigned long long *>(p.free_bits);
     const unsigned long long *managed = reinterpret_cast<const unsigned long long *>(p.managed);
-    unsigned mine = 0, n;
-    for (int w = tid; w < words; w += ASSIGN_NT) mine += __builtin_popcountll(managed[w] & ~bits[w]);
-    block_scan(mine, lds, n);
+    // a thread's word of the first round stays in registers
+    const unsigned long long m0 = tid < words ? managed[tid] : 0ull, f0 = tid < words ? bits[tid] : 0ull;
+    unsigned used = (unsigned)__builtin_popcountll(m0 & ~f0);
+    for (int w = tid + ASSIGN_NT; w < words; w += ASSIGN_NT) used += (unsigned)__builtin_popcountll(managed[w] & ~bits[w]);
     if (tid == 0) border = (int)p.n_pages;
-    __syncthreads();
+    Sums total, s = block_scan({used, (unsigned)__builtin_popcountll(m0)}, lds, total);
+    const unsigned n = total.a;
     unsigned done = 0;
-    for (int w0 = 0; w0 < words; w0 += ASSIGN_NT) {
-        const int w = w0 + tid;
-        unsigned long long m = w < words ? managed[w] : 0ull;
-        unsigned sum;
-        const unsigned rank = done + block_scan((unsigned)__builtin_popcountll(m), lds, sum);
-        done += sum;
+    for (int w0 = 0; w0 < words && done <= n; w0 += ASSIGN_NT) {
+        unsigned long long m = m0;
+        if (w0 > 0) {
+            m = w0 + tid < words ? managed[w0 + tid] : 0ull;
+            s = block_scan({0, (unsigned)__builtin_popcountll(m)}, lds, total);
+        }
+        const unsigned rank = done + s.b;
+        done += total.b;
         if (n >= rank && n - rank < (unsigned)__builtin_popcountll(m)) {
             for (unsigned i = rank; i < n; i++) m &= m - 1;
-            border = w * 64 + __builtin_ctzll(m);
+            border = (w0 + tid) * 64 + __builtin_ctzll(m);
         }
-        if (done > n) break;
     }
     __syncthreads();
     const int B = border;
     unsigned from = 0, to = 0;
     for (int w0 = 0; w0 < words; w0 += ASSIGN_NT) {
         const int w = w0 + tid;
-        const unsigned long long m = w < words ? managed[w] : 0ull, f = w < words ? bits[w] : 0ull;
+        const unsigned long long m = w0 == 0 ? m0 : w < words ? managed[w] : 0ull, f = w0 == 0 ? f0 : w < words ? bits[w] : 0ull;
         const unsigned long long below = B >= w * 64 + 64 ? ~0ull : B <= w * 64 ? 0ull : (1ull << (B - w * 64)) - 1;
-        unsigned long long holes = f & below, movers = m & ~f & ~below;
-        unsigned sum_f, sum_t;
-        unsigned rf = from + block_scan((unsigned)__builtin_popcountll(movers), lds, sum_f);
-        unsigned rt = to + block_scan((unsigned)__builtin_popcountll(holes), lds, sum_t);
-        from += sum_f;
-        to += sum_t;
+        const unsigned long long holes = f & below, movers = m & ~f & ~below;
+        s = block_scan({(unsigned)__builtin_popcountll(movers), (unsigned)__builtin_popcountll(holes)}, lds, total);
+        const unsigned rf = from + s.a, rt = to + s.b;
+        from += total.a;
+        to += total.b;
         if (w < words) {
             p.word_rank[w] = (int)rf;
             reinterpret_cast<unsigned long long *>(p.word_movers)[w] = movers;
             bits[w] = m & ~below;
         }
-        for (; movers; movers &= movers - 1) p.move_from[rf++] = w * 64 + __builtin_ctzll(movers);
-        for (; holes; holes &= holes - 1) p.picked[rt++] = w * 64 + __builtin_ctzll(holes);
+        each_bit(movers, rf, w0 + (tid & ~63), [&](unsigned nth, int id) { p.move_from[nth] = id; });
+        each_bit(holes, rt, w0 + (tid & ~63), [&](unsigned nth, int id) { p.picked[nth] = id; });
     }
     if (tid == 0) {
         p.head[0] = (int)from;
@@ -352,7 +492,8 @@ __global__ __launch_bounds__(256) void pages_move_kernel(const PagesArgs p)
 int launch_pages_compact(const PagesArgs &a, hipStream_t s)
 {
     hipLaunchKernelGGL(pages_moves_kernel, dim3(1), dim3(ASSIGN_NT), 0, s, a);
-    hipLaunchKernelGGL(pages_move_kernel, dim3(8u * device_compute_units()), dim3(256), 0, s, a);
+    const long long units = 2ll * a.n_layers * a.n_pages, most = 8ll * device_compute_units();
+    hipLaunchKernelGGL(pages_move_kernel, dim3((unsigned)(units < most ? units : most)), dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }
 

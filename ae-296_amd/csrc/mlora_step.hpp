@@ -134,10 +134,11 @@ struct KvAppendArgs {
 // ---- the cache's page tables.  State, one buffer of int32 words: [free bits, two words for 64 pages][table n_req * max_pages][lens n_req]
 // [refs n_pages][failed][live].  Scratch, likewise: [managed bits][words of head][writers n_pages][last_writer n_pages] - these three are set once,
 // and the counts are zeros again after every call - then [picked n_pages][move_from n_pages][word_rank][word_movers][row_page n_req]
-// [row_new 3 n_req][copies 5 n_req][rows n_req * max_pages].
+// [row_new 3 n_req][copies 5 n_req][rows n_req * max_pages][pieces: a word for every FORK_PIECE entries of a row].
+constexpr int FORK_PIECE = 1024;               // entries of a row that a workgroup forks
 struct PagesLayout {
     int64_t table, lens, refs, failed, live, state_words;
-    int64_t head, writers, last_writer, picked, move_from, word_rank, word_movers, row_page, row_new, copies, rows, scratch_words;
+    int64_t head, writers, last_writer, picked, move_from, word_rank, word_movers, row_page, row_new, copies, rows, pieces, scratch_words;
 };
 inline PagesLayout pages_layout(int64_t n_req, int64_t max_pages, int64_t n_pages)
 {
@@ -160,12 +161,13 @@ inline PagesLayout pages_layout(int64_t n_req, int64_t max_pages, int64_t n_page
     l.row_new = l.row_page + n_req;
     l.copies = l.row_new + 3 * n_req;
     l.rows = l.copies + 5 * n_req;
-    l.scratch_words = l.rows + n_req * max_pages;
+    l.pieces = l.rows + n_req * max_pages;
+    l.scratch_words = l.pieces + n_req * ((max_pages + FORK_PIECE - 1) / FORK_PIECE);
     return l;
 }
 struct PagesArgs {
     int32_t *free_bits, *table, *lens, *refs, *failed, *live;
-    int32_t *head, *writers, *last_writer, *picked, *move_from, *word_rank, *word_movers, *row_page, *row_new, *copies, *rows;
+    int32_t *head, *writers, *last_writer, *picked, *move_from, *word_rank, *word_movers, *row_page, *row_new, *copies, *rows, *pieces;
     const int32_t *managed, *want;             // want: the rows' new lengths, or their parents
     uint16_t *k, *v;
     int64_t n_pages;

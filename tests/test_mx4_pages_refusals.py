@@ -104,7 +104,7 @@ def test_layout():
     rc, at = layout()
     assert rc == OK and at[:7] == [0, 4, 24, 28, 98, 99, 100] and at[7] >= 4 + 2 + 4 * 70
     for kw, code in ((dict(n_req=0), EINVAL), (dict(max_pages=0), EINVAL), (dict(n_pages=0), EINVAL), (dict(n_pages=(1 << 24) + 1), ERANGE),
-                     (dict(n_req=1 << 16, max_pages=(1 << 14) + 1), ERANGE), (dict(n_req=(1 << 24) + 1), ERANGE)):
+                     (dict(n_req=1 << 16, max_pages=(1 << 14) + 1), ERANGE), (dict(n_req=(1 << 20) + 1), ERANGE)):
         assert layout(**kw)[0] == code
     assert _ext.lib().mlora_pages_layout(1, 1, 1, None) == EINVAL
 
