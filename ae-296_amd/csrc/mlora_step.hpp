@@ -131,26 +131,26 @@ struct KvAppendArgs {
     int n_pos, rot, interleaved;
     int32_t *bad;
 };
-// ---- the cache's page tables.  State, one buffer of int32 words: [free bits, two words for 64 pages][table n_req * max_pages][lens n_req]
-// [refs n_pages][failed][live].  Scratch, likewise: [managed bits][words of head][writers n_pages][last_writer n_pages] - these three are set once,
+// ---- the cache's page tables.  State, one buffer of int32 words: [free: a byte a page, 0 or 1, to a multiple of 64][table n_req * max_pages]
+// [lens n_req][refs n_pages][failed][live].  Scratch, likewise: [managed: bytes as free][words of head][writers n_pages][last_writer n_pages] - these three are set once,
 // and the counts are zeros again after every call - then [picked n_pages][move_from n_pages][word_rank][word_movers][row_page n_req]
-// [row_new 3 n_req][copies 5 n_req][rows n_req * max_pages][pieces: a word for every FORK_PIECE entries of a row].
-constexpr int FORK_PIECE = 1024;               // entries of a row that a workgroup forks
+// [row_new 3 n_req][row_copy 2 n_req][copies 3 n_req][rows n_req * max_pages][pieces: a word for every ROW_PIECE entries of a row].
+constexpr int ROW_PIECE = 1024;                // entries of a row that a workgroup takes
 struct PagesLayout {
     int64_t table, lens, refs, failed, live, state_words;
-    int64_t head, writers, last_writer, picked, move_from, word_rank, word_movers, row_page, row_new, copies, rows, pieces, scratch_words;
+    int64_t head, writers, last_writer, picked, move_from, word_rank, word_movers, row_page, row_new, row_copy, copies, rows, pieces, scratch_words;
 };
 inline PagesLayout pages_layout(int64_t n_req, int64_t max_pages, int64_t n_pages)
 {
     const int64_t words = (n_pages + 63) / 64;
     PagesLayout l;
-    l.table = 2 * words;
+    l.table = 16 * words;
     l.lens = l.table + n_req * max_pages;
     l.refs = l.lens + n_req;
     l.failed = l.refs + n_pages;
     l.live = l.failed + 1;
     l.state_words = l.live + 1;
-    l.head = 2 * words;
+    l.head = 16 * words;
     l.writers = l.head + 2;
     l.last_writer = l.writers + n_pages;
     l.picked = l.last_writer + n_pages;
@@ -159,16 +159,19 @@ inline PagesLayout pages_layout(int64_t n_req, int64_t max_pages, int64_t n_page
     l.word_rank = l.word_movers + 2 * words;
     l.row_page = l.word_rank + words;
     l.row_new = l.row_page + n_req;
-    l.copies = l.row_new + 3 * n_req;
-    l.rows = l.copies + 5 * n_req;
+    l.row_copy = l.row_new + 3 * n_req;
+    l.copies = l.row_copy + 2 * n_req;
+    l.rows = l.copies + 3 * n_req;
     l.pieces = l.rows + n_req * max_pages;
-    l.scratch_words = l.pieces + n_req * ((max_pages + FORK_PIECE - 1) / FORK_PIECE);
+    l.scratch_words = l.pieces + n_req * ((max_pages + ROW_PIECE - 1) / ROW_PIECE);
     return l;
 }
 struct PagesArgs {
-    int32_t *free_bits, *table, *lens, *refs, *failed, *live;
-    int32_t *head, *writers, *last_writer, *picked, *move_from, *word_rank, *word_movers, *row_page, *row_new, *copies, *rows, *pieces;
-    const int32_t *managed, *want;             // want: the rows' new lengths, or their parents
+    uint8_t *free_pages;
+    int32_t *table, *lens, *refs, *failed, *live;
+    int32_t *head, *writers, *last_writer, *picked, *move_from, *word_rank, *word_movers, *row_page, *row_new, *row_copy, *copies, *rows, *pieces;
+    const uint8_t *managed;
+    const int32_t *want;                       // want: the rows' new lengths, or their parents
     uint16_t *k, *v;
     int64_t n_pages;
     int n_req, max_pages, page_shift, n_layers, n_kv_heads, head_elems;      // head_elems: elements of one head of a page

@@ -36,7 +36,8 @@ class KVPages:
         self.cache, self.n_req, self.max_pages = cache, n_req, max_pages
         self.state = torch.zeros(words, dtype=torch.int32, device=cache.device)
         self.scratch = torch.zeros(scratch, dtype=torch.int32, device=cache.device)
-        self._free, self._managed = self.state[:table], self.scratch[:table]         # a bit a page
+        # a byte a page
+        self._free, self._managed = (x[:table].view(torch.uint8)[:cache.n_pages] for x in (self.state, self.scratch))
         self.table = self.state[table:lens].view(n_req, max_pages)
         self.lens, self.refs = self.state[lens:refs], self.state[refs:failed]
         self.failed = self.state[failed:live]          # rows that resize or fork could not serve, added up until it is cleared
@@ -44,32 +45,21 @@ class KVPages:
         self.table.fill_(-1)
         self.take(cache.free_pages if n_pages is None else n_pages)
 
-    def _bits(self, words: torch.Tensor) -> np.ndarray:
-        """One truth value a page."""
-        return np.unpackbits(words.cpu().numpy().view(np.uint8), bitorder="little")[:self.cache.n_pages].astype(bool)
-
-    def _set_bits(self, words: torch.Tensor, on: np.ndarray) -> None:
-        full = np.zeros(words.numel() * 32, bool)
-        full[:len(on)] = on
-        words.copy_(torch.from_numpy(np.packbits(full, bitorder="little").view(np.int32)))
-
     def take(self, n: int) -> None:
-        """n more pages of the cache.  Waits for the device."""
-        ids = self.cache.allocate(n)
-        for words in (self._managed, self._free):
-            on = self._bits(words)
-            on[ids] = True
-            self._set_bits(words, on)
+        """n more pages of the cache."""
+        ids = torch.tensor(self.cache.allocate(n), dtype=torch.long, device=self.state.device)
+        self._managed[ids] = 1
+        self._free[ids] = 1
 
     def give_back(self) -> int:
         """Gives the cache the pages behind the last one in use (all that are free, after ``compact``) and returns how many.  Waits for the device."""
-        managed, free = self._bits(self._managed), self._bits(self._free)
+        managed, free = self._managed.cpu().numpy().astype(bool), self._free.cpu().numpy().astype(bool)
         used = np.flatnonzero(managed & ~free)
         ids = np.flatnonzero(free)
         ids = ids[ids > (used[-1] if len(used) else -1)]
-        managed[ids] = free[ids] = False
-        self._set_bits(self._managed, managed)
-        self._set_bits(self._free, free)
+        gone = torch.from_numpy(ids).to(self.state.device)
+        self._managed[gone] = 0
+        self._free[gone] = 0
         self.cache.release(ids[::-1].tolist())
         return len(ids)
 
@@ -83,8 +73,7 @@ class KVPages:
             raise ValueError(f"lengths must be in 0..{self.max_pages * self.cache.page_tokens}")
         held = torch.arange(self.max_pages, device=table.device) < torch.from_numpy(-(-n // self.cache.page_tokens)).to(table.device)[:, None]
         ids = table[held].long()
-        managed = self._bits(self._managed)
-        if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= self.cache.n_pages or not bool(torch.from_numpy(managed).to(ids.device)[ids].all())):
+        if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= self.cache.n_pages or not bool(self._managed.to(ids.device)[ids].all())):
             raise ValueError("a row names a page that is not among the managed ones")
         pairs = torch.sort(held.nonzero()[:, 0] * self.cache.n_pages + ids)[0]
         if bool((pairs[1:] == pairs[:-1]).any()):
@@ -93,8 +82,7 @@ class KVPages:
         self.table.copy_(table.masked_fill(~held, -1))
         self.lens.copy_(lens)
         self.refs.copy_(refs)
-        refs = refs.cpu().numpy()
-        self._set_bits(self._free, managed & (refs == 0))
+        self._free.copy_(self._managed.bool() & (self.refs == 0))
 
     def resize(self, want: torch.Tensor) -> None:
         """Rows' new lengths, int32 [n_req] on the device (negative: as it is; 0 gives all pages back).  Shorter rows give pages back first; then longer rows, in

@@ -25,7 +25,7 @@ class Pair:
         self.pages = mlora.KVPages(self.cache, n_req, max_pages, taken)
         managed = [p for p in range(n_pages) if p not in held_back]
         if taken is not None:
-            managed = np.flatnonzero(self.pages._bits(self.pages._managed)).tolist()
+            managed = self.pages._managed.nonzero().flatten().tolist()
         self.model = Tables([[] for _ in range(n_req)], [0] * n_req, managed, n_pages, P, max_pages)
         self.k, self.v = self.cache.k.clone(), self.cache.v.clone()
 
@@ -39,7 +39,7 @@ class Pair:
         assert p.refs.tolist() == m.refs(), what
         assert p.failed.tolist() == [m.failed], what
         refs = m.refs()
-        assert np.flatnonzero(p._bits(p._free)).tolist() == [i for i in m.managed if refs[i] == 0], what
+        assert p._free.nonzero().flatten().tolist() == [i for i in m.managed if refs[i] == 0], what
         assert torch.equal(self.cache.k, self.k) and torch.equal(self.cache.v, self.v), what
 
     def resize(self, want, check=True):
@@ -166,7 +166,7 @@ def test_pages_are_taken_and_given_back():
     p.resize([64, 33])
     assert p.model.failed == 1
     p.pages.take(4)
-    p.model.managed = sorted(np.flatnonzero(p.pages._bits(p.pages._managed)).tolist())
+    p.model.managed = p.pages._managed.nonzero().flatten().tolist()
     p.resize([64, 33])
     p.resize([0, -1])
     p.compact()

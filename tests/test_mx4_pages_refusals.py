@@ -102,7 +102,7 @@ def layout(n_req=4, max_pages=5, n_pages=70):
 
 def test_layout():
     rc, at = layout()
-    assert rc == OK and at[:7] == [0, 4, 24, 28, 98, 99, 100] and at[7] >= 4 + 2 + 4 * 70
+    assert rc == OK and at[:7] == [0, 32, 52, 56, 126, 127, 128] and at[7] >= 32 + 2 + 4 * 70
     for kw, code in ((dict(n_req=0), EINVAL), (dict(max_pages=0), EINVAL), (dict(n_pages=0), EINVAL), (dict(n_pages=(1 << 24) + 1), ERANGE),
                      (dict(n_req=1 << 16, max_pages=(1 << 14) + 1), ERANGE), (dict(n_req=(1 << 20) + 1), ERANGE)):
         assert layout(**kw)[0] == code
@@ -111,7 +111,7 @@ def test_layout():
 
 @pytest.mark.parametrize("kw, code", [
     (dict(state=None), EINVAL), (dict(scratch=None), EINVAL), (dict(want=None), EINVAL), (dict(state=off), EALIGN), (dict(scratch=off), EALIGN),
-    (dict(words=99), ENOSPACE), (dict(scratch_words=200), ENOSPACE), (dict(n_req=0), EINVAL), (dict(max_pages=-1), EINVAL), (dict(n_pages=0), EINVAL),
+    (dict(words=127), ENOSPACE), (dict(scratch_words=200), ENOSPACE), (dict(n_req=0), EINVAL), (dict(max_pages=-1), EINVAL), (dict(n_pages=0), EINVAL),
     (dict(P=8), EINVAL), (dict(P=48), EINVAL), (dict(P=512), EINVAL), (dict(max_pages=1 << 27, n_req=1), ERANGE),
     (dict(k=None), EINVAL), (dict(v=None), EINVAL), (dict(k=off), EALIGN), (dict(layers=0), EINVAL), (dict(heads=0), EINVAL), (dict(D=96), ERANGE),
     (dict(heads=(1 << 14) + 1), ERANGE)])
