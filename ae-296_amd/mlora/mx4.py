@@ -51,6 +51,13 @@ class MX4Tensor:
         _ext.check(_ext.lib().mlora_mx4_pack(codes.data_ptr(), scales.data_ptr(), self.rows, self.k, self.packed.data_ptr(), need,
                                              _ext.current_stream_ptr()))
 
+    @classmethod
+    def empty(cls, rows: int, k: int, device: str | torch.device = "cuda") -> "MX4Tensor":
+        """Room for an operand of up to so many rows, for ``mx4_quantize(..., out=)``; until then it holds anything."""
+        made = cls.__new__(cls)
+        made.packed, made.rows, made.k = torch.empty(_packed_bytes(rows, k), dtype=torch.uint8, device=device), rows, k
+        return made
+
     def values(self, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """What the operand stands for, [rows, k] in a 16-bit type (into `out`, whose rows may be apart): exact for what was quantised from it."""
         got = _ext.host().mx4_values(self, out, _ext.dtype_code(dtype) if out is None else 0)

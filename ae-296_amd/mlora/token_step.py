@@ -1,4 +1,4 @@
-"""One decode step of the attention blocks: 4-bit base projections, every token's adapter, rotation and append, attention.
+"""One decode step of the attention blocks: 4-bit base projections (16-bit inputs on ``W4Weight``, or 4-bit ones on ``MX4Weight``), every token's adapter, rotation and append, attention.
 
     step = TokenStep(pool, cache, weights, n_q_heads, rope)
     step.begin(batch, tok_adapter)                  # once per step: both plans
@@ -12,21 +12,23 @@ replay and other work of the same step object are ordered on one stream.
 """
 from __future__ import annotations
 
-from typing import Dict, Optional, Sequence
+from typing import Dict, Optional, Sequence, Union
 
 import torch
 
 from . import ops
 from .attention import KVBatch, KVCache, RopeTable, kv_append, plan_attention, prefix_attention
+from .mx4 import MX4Tensor, MX4Weight, mx4_gemm, mx4_quantize
 from .pool import AdapterPool
 from .w4 import W4Weight, w4_gemv
 
 
 class TokenStep:
-    """`weights[layer][name]` are the base projections of q, k and v (`names`, in that order) as ``W4Weight``; None leaves them
+    """`weights[layer][name]` are the base projections of q, k and v (`names`, in that order), a layer's all as ``W4Weight`` or all as
+    ``MX4Weight`` (the layer's input is then rounded to 4 bits for them, and the adapters take it as it is); None leaves them
     to the caller, whose base products ``layer`` then takes as `qkv`, or without any the deltas alone are q, k and v."""
 
-    def __init__(self, pool: AdapterPool, cache: KVCache, weights: Optional[Sequence[Dict[str, W4Weight]]], n_q_heads: int,
+    def __init__(self, pool: AdapterPool, cache: KVCache, weights: Optional[Sequence[Dict[str, Union[W4Weight, MX4Weight]]]], n_q_heads: int,
                  rope: Optional[RopeTable] = None, names: Sequence[str] = ("q", "k", "v")):
         if len(names) != 3:
             raise ValueError("names must be the projections of q, k and v")
@@ -44,6 +46,10 @@ class TokenStep:
             for name, width in zip(names, self.widths):
                 if (layer[name].hin, layer[name].hout) != (hin, width):
                     raise ValueError(f"the 4-bit weight of {name} must be {hin} -> {width}")
+            if len({isinstance(layer[name], MX4Weight) for name in names}) > 1:
+                raise ValueError("the weights of a layer must all be W4Weight or all MX4Weight")
+        self.hin = hin
+        self._mx4 = [isinstance(layer[names[0]], MX4Weight) for layer in weights or ()]
         self.pool, self.cache, self.weights, self.n_q_heads, self.rope, self.names = pool, cache, weights, n_q_heads, rope, list(names)
         self.batch: Optional[KVBatch] = None
         self.tok_adapter = None
@@ -65,9 +71,11 @@ class TokenStep:
             room = max(1, 1 << (T - 1).bit_length()) if T else 1
             if room not in self._buffers:
                 new = dict(dtype=self.cache.dtype, device=self.cache.device)
-                self._buffers[room] = [torch.empty((room, w), **new) for w in self.widths] + [torch.empty((room, self.n_q_heads, self.cache.head_dim), **new)]
-            *qkv, out = (b[:T] for b in self._buffers[room])
-            kept = self._kept[T] = [None, None, qkv, out, -1]
+                self._buffers[room] = ([torch.empty((room, w), **new) for w in self.widths] + [torch.empty((room, self.n_q_heads, self.cache.head_dim), **new)],
+                                       MX4Tensor.empty(room, self.hin, self.cache.device) if any(self._mx4) else None)
+            rows, x4 = self._buffers[room]
+            *qkv, out = (b[:T] for b in rows)
+            kept = self._kept[T] = [None, None, qkv, out, -1, x4]
         if n_prefix > kept[4]:            # room for twice as many, so that a growing number of prompts moves the plan a few times only
             holds = n_prefix if kept[1] is None else min(2 * n_prefix, 4096)
             plan = plan_attention(batch, self.cache, self.n_q_heads, room=holds)
@@ -83,6 +91,7 @@ class TokenStep:
         self.bad.zero_()
         kept[3].zero_()              # rows without a request: the attention leaves them alone, and other batches share the buffer
         self.decode_plan, self.attn_plan, self.qkv, self.out = kept[:4]
+        self._x4 = kept[5]
         self.batch, self.tok_adapter = batch, tok_adapter
 
     def layer(self, layer: int, x: torch.Tensor, qkv: Optional[Sequence[torch.Tensor]] = None, scale: Optional[float] = None) -> torch.Tensor:
@@ -95,7 +104,11 @@ class TokenStep:
             raise ValueError("qkv is for a step without weights of its own")
         ys = list(qkv) if qkv is not None else self.qkv
         if self.weights is not None:
-            w4_gemv(ys, [x] * 3, [self.weights[layer][n] for n in self.names])
+            ws = [self.weights[layer][n] for n in self.names]
+            if self._mx4[layer]:
+                mx4_gemm(ys, [mx4_quantize(x, out=self._x4)] * 3, ws)
+            else:
+                w4_gemv(ys, [x] * 3, ws)
         ops.bgmv(ys, [x] * 3, self.pool, layer, self.names, self.tok_adapter, plan=self.decode_plan,
                  accumulate=qkv is not None or self.weights is not None)
         D, T = self.cache.head_dim, self.batch.T
