@@ -105,11 +105,13 @@ struct Mx4Proj {
     const unsigned char *x, *w;
     int64_t x_scales_at, w_scales_at;
     int hin, hout, k_tiles, quads;
-    unsigned end;              // workgroups of the projections up to this one (set by the launcher)
+    unsigned end;              // tiles of the projections up to this one (set by the launcher)
 };
 struct Mx4Args {
     Mx4Proj pr[STEP_MAX_PROJ];
     int n_proj, T, accumulate;
+    unsigned whole;            // tiles that a workgroup takes whole (these two set by the launcher)
+    int first;                 // row of workgroups that a launch begins with
 };
 
 // ---- keys and values

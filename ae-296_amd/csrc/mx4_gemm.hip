@@ -29,7 +29,7 @@ __global__ __launch_bounds__(64 * MX_WAVES) void mx4_slim_kernel(const Mx4Args p
     int proj = 0;
     while (proj + 1 < p.n_proj && blockIdx.x >= p.pr[proj].end) proj++;
     const Mx4Proj &w = p.pr[proj];
-    const int nt = (int)(blockIdx.x - (proj ? p.pr[proj - 1].end : 0u)) * NT, tt = blockIdx.y * MT;
+    const int nt = (int)(blockIdx.x - (proj ? p.pr[proj - 1].end : 0u)) * NT, tt = ((int)blockIdx.y + p.first) * MT;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int n_tiles = (w.hout + 15) / 16, t_tiles = (p.T + 15) / 16, k_tiles = w.k_tiles, quads = w.quads;
     const bool row_in = tt * 16 + (lane & 15) < p.T;
@@ -137,28 +137,13 @@ __device__ __forceinline__ float16_t mx4_mfma32(const uint4 &a, const uint4 &b, 
 template <int WI, int XI> constexpr int mx4_stage_bytes() { return 4 * (WI + XI) * MX4_TILE_BYTES; }
 template <int WI, int XI> constexpr int mx4_ring_bytes() { return MX_RING * mx4_stage_bytes<WI, XI>() + 2 * 4 * (WI + XI) * MX4_QUAD_BYTES; }
 
+// Columns 64 WI nt .. and tokens 64 XI tt .. of one product.
 template <int DT, int WI, int XI, int KS, bool ACC>
-__global__ __launch_bounds__(MX_NT * KS) void mx4_tile_kernel(const Mx4Args p)
+__device__ __forceinline__ void mx4_tile(const Mx4Args &p, const Mx4Proj &w, int nt, int tt, unsigned char *const all_rings)
 {
     constexpr int STAGE = mx4_stage_bytes<WI, XI>(), SSTAGE = 4 * (WI + XI) * MX4_QUAD_BYTES, NL = WI + XI;
     constexpr int RINGS = mx4_ring_bytes<WI, XI>();
     static_assert(KS * RINGS <= 160 * 1024, "the rings must fit the LDS of a compute unit");
-    __shared__ __attribute__((aligned(16))) unsigned char all_rings[KS * RINGS];
-
-    // Workgroups go to the 8 XCDs round-robin by id; every XCD works through one contiguous range of the tiles, in which GROUP token tiles sweep the
-    // column tiles together, so that what is in flight on one XCD shares its panels in that L2.
-    int proj = 0;
-    while (proj + 1 < p.n_proj && blockIdx.x >= p.pr[proj].end) proj++;
-    const Mx4Proj &w = p.pr[proj];
-    const int at = (int)(blockIdx.x - (proj ? p.pr[proj - 1].end : 0u));
-    constexpr int GROUP = 4;
-    const int ntn = (w.hout + 64 * WI - 1) / (64 * WI), ntt = (p.T + 64 * XI - 1) / (64 * XI), tiles = ntn * ntt;
-    const int base = tiles >> 3, more = tiles & 7, xcd = at & 7;
-    const int L = xcd * base + (xcd < more ? xcd : more) + (at >> 3);
-    const int grp = L / (GROUP * ntn), within = L - grp * (GROUP * ntn);
-    const int in_grp = ntt - grp * GROUP < GROUP ? ntt - grp * GROUP : GROUP;
-    const int tt = grp * GROUP + within % in_grp, nt = within / in_grp;
-
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3);
     const int part = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / MX_NT);
     const int wm = wave >> 1, wn = wave & 1, l32 = lane & 31, lh = lane >> 5;
@@ -340,7 +325,8 @@ __global__ __launch_bounds__(MX_NT * KS) void mx4_tile_kernel(const Mx4Args p)
     constexpr int PITCH = 64 * WI + 16, CHUNKS = 4 * WI;
     static_assert(4 * 32 * PITCH <= MX_RING * STAGE, "the staging tiles reuse the ring");
     unsigned char *const out = lds + wave * 32 * PITCH;
-    int ol = threadIdx.x & 63;                           // the lane once more, not kept in registers through the loop
+    // the lane once more, from the hardware: not kept in a register through the loop
+    int ol = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
     asm volatile("" : "+v"(ol));
     const int o32 = ol & 31, oh = ol >> 5;
     const int n0 = nt * 64 * WI + wm * 32 * WI, t0 = tt * 64 * XI + wn * 32 * XI;
@@ -376,6 +362,59 @@ __global__ __launch_bounds__(MX_NT * KS) void mx4_tile_kernel(const Mx4Args p)
     }
 }
 
+// Workgroups go to the 8 XCDs round-robin by id: the id-th of n workgroups takes tile number L of n, so that every XCD works through one contiguous range of them.
+__device__ __forceinline__ int mx4_spread(int id, int n)
+{
+    const int base = n >> 3, more = n & 7, xcd = id & 7;
+    return xcd * base + (xcd < more ? xcd : more) + (id >> 3);
+}
+
+// Tile number L of a call: GROUP token tiles sweep a product's column tiles together, so that what is in flight on one XCD shares its panels in that L2.
+struct Mx4Place { int proj, nt, tt; };
+template <int WI, int XI>
+__device__ __forceinline__ Mx4Place mx4_place(const Mx4Args &p, int L)
+{
+    constexpr int GROUP = 4;
+    int proj = 0;
+    while (proj + 1 < p.n_proj && (unsigned)L >= p.pr[proj].end) proj++;
+    if (proj) L -= (int)p.pr[proj - 1].end;
+    const int ntn = (p.pr[proj].hout + 64 * WI - 1) / (64 * WI), ntt = (p.T + 64 * XI - 1) / (64 * XI);
+    const int grp = L / (GROUP * ntn), within = L - grp * (GROUP * ntn);
+    const int in_grp = ntt - grp * GROUP < GROUP ? ntt - grp * GROUP : GROUP;
+    return {proj, within / in_grp, grp * GROUP + within % in_grp};
+}
+
+template <int DT, int WI, int XI, int KS, bool ACC>
+__global__ __launch_bounds__(MX_NT * KS) void mx4_tile_kernel(const Mx4Args p)
+{
+    __shared__ __attribute__((aligned(16))) unsigned char rings[KS * mx4_ring_bytes<WI, XI>()];
+    const Mx4Place at = mx4_place<WI, XI>(p, mx4_spread((int)blockIdx.x, (int)gridDim.x));
+    mx4_tile<DT, WI, XI, KS, ACC>(p, p.pr[at.proj], at.nt, at.tt, rings);
+}
+
+// Tiles of 256 x 256, the first `whole` of them whole, and the others, which would be half a round of workgroups or less, as halves of 128 tokens (8000 tokens,
+// 13824 -> 5120, 2.5 rounds: 264 -> 240 us; 5120 -> 2 x 13824, 13.5 rounds: 552 -> 530).
+//
+// What bounds it: power.  A step of a whole tile is 128 matrix instructions, 1024 cycles of each pipe.  On one unit alone it takes 500 ns, 0.86 of the pipes' rate
+// at 2.4 GHz (a barrier a step and one wavefront a pipe); with all units at work 795 ns, where the instructions alone, from registers and on
+// random numbers, take 700 (6.1 PFLOP/s; on zeros 9.4): the card lowers its clock to 1.7 GHz.  64 rows of either operand in LDS for every 32 read feed the pipes at half of
+// the LDS' rate; 128 x 128 tiles need all of it and run at 1.5 GHz.
+template <int DT, bool ACC>
+__global__ __launch_bounds__(MX_NT) void mx4_halves_kernel(const Mx4Args p)
+{
+    __shared__ __attribute__((aligned(16))) unsigned char rings[mx4_ring_bytes<4, 4>()];
+    const int id = (int)blockIdx.x, whole = (int)p.whole;
+    if (id < whole) {
+        const Mx4Place at = mx4_place<4, 4>(p, mx4_spread(id, whole));
+        mx4_tile<DT, 4, 4, 1, ACC>(p, p.pr[at.proj], at.nt, at.tt, rings);
+    } else {
+        const int half = mx4_spread(id - whole, (int)gridDim.x - whole);
+        const Mx4Place at = mx4_place<4, 4>(p, whole + half / 2);
+        const int tt = 2 * at.tt + (half & 1);
+        if (tt * 128 < p.T) mx4_tile<DT, 4, 2, 1, ACC>(p, p.pr[at.proj], at.nt, tt, rings);
+    }
+}
+
 template <int DT, int WI, int XI, int KS>
 static int launch_tiles(Mx4Args &a, hipStream_t s)
 {
@@ -387,26 +426,43 @@ static int launch_tiles(Mx4Args &a, hipStream_t s)
     return (int)hipGetLastError();
 }
 
+template <int DT>
+static int launch_halves(Mx4Args &a, hipStream_t s)
+{
+    unsigned end = 0;
+    for (int p = 0; p < a.n_proj; p++) a.pr[p].end = end += (unsigned)((a.pr[p].hout + 255) / 256) * (unsigned)((a.T + 255) / 256);
+    const unsigned units = (unsigned)device_compute_units(), rest = end % units;
+    a.whole = 2 * rest <= units ? end - rest : end;
+    const dim3 grid(a.whole + 2 * (end - a.whole));
+    if (a.accumulate) hipLaunchKernelGGL((mx4_halves_kernel<DT, true>), grid, dim3(MX_NT), 0, s, a);
+    else hipLaunchKernelGGL((mx4_halves_kernel<DT, false>), grid, dim3(MX_NT), 0, s, a);
+    return (int)hipGetLastError();
+}
+
 template <int DT, int MT, int NT>
 static int launch_slim(Mx4Args &a, hipStream_t s)
 {
     unsigned end = 0;
     for (int p = 0; p < a.n_proj; p++) a.pr[p].end = end += (unsigned)(a.pr[p].hout + 16 * NT - 1) / (16 * NT);
-    hipLaunchKernelGGL((mx4_slim_kernel<DT, MT, NT>), dim3(end, (unsigned)(a.T + 16 * MT - 1) / (16 * MT)), dim3(64 * MX_WAVES), 0, s, a);
-    return (int)hipGetLastError();
+    const int rows = (a.T + 16 * MT - 1) / (16 * MT), most = 65535;              // of a grid's second dimension
+    int rc = 0;
+    for (a.first = 0; a.first < rows && !rc; a.first += most) {
+        hipLaunchKernelGGL((mx4_slim_kernel<DT, MT, NT>), dim3(end, (unsigned)(rows - a.first < most ? rows - a.first : most)), dim3(64 * MX_WAVES), 0, s, a);
+        rc = (int)hipGetLastError();
+    }
+    return rc;
 }
 
 // ------------------------------------------------------------------ which form
-// A form's time: start + round * m + max(step, m * step_full) * K tiles, with m the workgroups of the busiest compute unit - a workgroup alone is bound by the
-// way of its operands from memory, several share the unit - but not less than the call's bytes take, where forms are alike and the one for the fewest tokens is
-// taken.  The constants (us) are fitted to 1500 times of sixteen calls (one to three products of a whole,
-// half or quarter layer of Llama-7B and 13B) at 1 to 8000 tokens, each form over the range in which it comes near the fastest; fitted and measured times
-// differ by 5 % (few tokens) to 12 % (tiles) on average.  The form with the least is 0.4 % behind the fastest of all on average; the worst were
-// 24 to 64 tokens, 5120 -> 2 x 13824 (64 columns x 64 tokens, 16 to 23 % behind 128 columns) and then 1.5 rounds of 256 x 256 tiles (8 % behind
-// 128 x 128).  Examples, with the second best:
-//      1 token, 4096 -> 4096: 16 columns x 16 tokens 4.1 us, 32 columns 4.8;     64 tokens: 32 x 32 5.7, 64 columns x 32 tokens 6.9
+// A form's time: start + round * m + max(step, m * step_full) * K tiles, with m the workgroups of the busiest compute unit (a workgroup alone is bound by the
+// way of its operands from memory, several share the unit), but not less than the call's bytes take: where forms are alike then, the one for the fewest tokens
+// is taken.  The constants (us) are fitted to 2064 times of sixteen calls (one to three products of a whole, half or quarter layer of Llama-7B and 13B) at 1 to 8000
+// tokens, each form over the range in which it comes near the fastest; fitted and measured times differ by 5 % (few tokens) to 12 % (tiles) on average.  The
+// form with the least time is 0.5 % behind the fastest on average; the worst were 24 to 64 tokens, 5120 -> 2 x 13824 (64 columns x 64 tokens, 16 to 23 % behind
+// 128 columns) and then 1.5 rounds of 256 x 256 tiles (8 % behind 128 x 128).  Examples, with another one:
+//      1 token, 4096 -> 4096: 16 columns x 16 tokens 4.1 us, 32 columns 4.8;     64 tokens: 32 x 32 5.7, 32 columns x 64 tokens 6.9
 //      64 tokens, 4096 -> 2 x 11008: 128 columns x 64 tokens 13.1, 64 x 64 15.5;  512 tokens: 256 x 256 29.8, 128 x 128 32.4
-//      512 tokens, 11008 -> 4096: 128 columns x 64 tokens 23.7, 64 x 64 28.0;    8000 tokens, 13824 -> 5120: 256 x 256 272, 128 columns x 256 tokens 275
+//      512 tokens, 11008 -> 4096: 128 columns x 64 tokens 23.7, 64 x 64 28.0;     1536 tokens: 128 columns x 256 tokens 39.7, 128 x 128 41.0
 namespace {
 struct Mx4Form {
     int columns, tokens;
@@ -424,7 +480,7 @@ const Mx4Form mx4_forms[] = {
     {128, 64, 2.1f, 1.0f, 0.216f, 0.179f, MX_FORM(launch_tiles, 2, 1, 1)},
     {128, 128, 2.4f, 1.2f, 0.0f, 0.25f, MX_FORM(launch_tiles, 2, 2, 1)},
     {128, 256, 0.0f, 4.8f, 0.0f, 0.389f, MX_FORM(launch_tiles, 2, 4, 1)},
-    {256, 256, 0.0f, 7.3f, 0.0f, 0.62f, MX_FORM(launch_tiles, 4, 4, 1)},
+    {256, 256, 0.0f, 7.3f, 0.0f, 0.62f, {launch_halves<DT_F16>, launch_halves<DT_BF16>}},
 };
 
 const Mx4Form &mx4_form(const Mx4Args &a)
@@ -442,7 +498,9 @@ const Mx4Form &mx4_form(const Mx4Args &a)
     for (const Mx4Form &f : mx4_forms) {
         int64_t groups = 0;
         for (int p = 0; p < a.n_proj; p++) groups += (int64_t)((a.pr[p].hout + f.columns - 1) / f.columns) * ((a.T + f.tokens - 1) / f.tokens);
-        const float m = (float)((groups + units - 1) / units), each = m * f.step_full > f.step ? m * f.step_full : f.step;
+        float m = (float)((groups + units - 1) / units);
+        if (f.columns == 256 && groups % units && 2 * (groups % units) <= units) m -= 0.37f;         // a round of halves
+        const float each = m * f.step_full > f.step ? m * f.step_full : f.step;
         float time = f.start + f.round * m + each * (float)steps;
         if (time < memory) time = memory;
         if (!best || time < least) { best = &f; least = time; }

@@ -94,6 +94,22 @@ def test_accumulate(T):
     run(T, 640, 200, BF16, accumulate=True)
 
 
+def test_the_most_tokens():
+    """2^20 tokens of one narrow product: more rows of workgroups than a launch's second dimension takes, compared at both ends and in the middle."""
+    say("mx4_gemm 2^20 tokens")
+    T = 1 << 20
+    base, xv = operand(64, 40, 1)
+    row = base.values(BF16)
+    x = mlora.mx4_quantize(row.repeat(T // 64, 1))
+    w, wv = operand(8, 40, 2, 3, mlora.MX4Weight)
+    y = torch.empty((T, 8), dtype=BF16, device="cuda")
+    mlora.mx4_gemm([y], [x], [w])
+    again = ref.values(*ref.quantize(xv))
+    for at in (0, T // 2, T - 64):
+        compare(y[at:at + 64], again, wv, BF16, what=f"rows from {at}")
+    assert torch.equal(y.view(-1, 64, 8), y[:64].expand(T // 64, 64, 8))
+
+
 def test_powers_of_two_far_apart():
     """Blocks whose scales differ by up to 2^40: the small ones fall below what fp32 holds beside the large ones."""
     run(20, 1024, 64, BF16, spread=40)
