@@ -462,7 +462,7 @@ static int launch_slim(Mx4Args &a, hipStream_t s)
 // 128 columns) and then 1.5 rounds of 256 x 256 tiles (8 % behind 128 x 128).  Examples, with another one:
 //      1 token, 4096 -> 4096: 16 columns x 16 tokens 4.1 us, 32 columns 4.8;     64 tokens: 32 x 32 5.7, 32 columns x 64 tokens 6.9
 //      64 tokens, 4096 -> 2 x 11008: 128 columns x 64 tokens 13.1, 64 x 64 15.5;  512 tokens: 256 x 256 29.8, 128 x 128 32.4
-//      512 tokens, 11008 -> 4096: 128 columns x 64 tokens 23.7, 64 x 64 28.0;     1536 tokens: 128 columns x 256 tokens 39.7, 128 x 128 41.0
+//      512 tokens, 11008 -> 4096: 128 columns x 64 tokens 23.7, 64 x 64 28.0;     1536 tokens: 256 x 256 in halves 41.4, 128 x 128 41.0
 namespace {
 struct Mx4Form {
     int columns, tokens;
@@ -479,7 +479,6 @@ const Mx4Form mx4_forms[] = {
     {64, 64, 3.0f, 0.84f, 0.136f, 0.12f, MX_FORM(launch_tiles, 1, 1, 2)},
     {128, 64, 2.1f, 1.0f, 0.216f, 0.179f, MX_FORM(launch_tiles, 2, 1, 1)},
     {128, 128, 2.4f, 1.2f, 0.0f, 0.25f, MX_FORM(launch_tiles, 2, 2, 1)},
-    {128, 256, 0.0f, 4.8f, 0.0f, 0.389f, MX_FORM(launch_tiles, 2, 4, 1)},
     {256, 256, 0.0f, 7.3f, 0.0f, 0.62f, {launch_halves<DT_F16>, launch_halves<DT_BF16>}},
 };
 

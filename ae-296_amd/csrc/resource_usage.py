@@ -17,7 +17,9 @@ the limits below.  The limits say what the kernels were designed around:
 * four workgroups of the reference layout's prefill expand fit a compute unit, by their registers and by their LDS;
 * two workgroups of `w4_gemv_kernel` and of the forms of `w4_wide_kernel` that the choice of forms counts two of fit a compute unit, by their
   registers and by their LDS; so do two of the attention kernel;
-* M0 in `gemm_lora_kernel`, `gemm_lora_short_kernel`, `sgmv_shrink_kernel` and `w4_wide_kernel` is written only by the kernel's own LDS-bound loads: one
+* `mx4_halves_kernel` keeps its 256 accumulators in AGPRs on one workgroup a compute unit; two workgroups of the smaller tiles of `mx4_tile_kernel`, and four of
+  `mx4_slim_kernel` for one tile, fit it;
+* M0 in `gemm_lora_kernel`, `gemm_lora_short_kernel`, `sgmv_shrink_kernel`, `w4_wide_kernel`, `mx4_tile_kernel` and `mx4_halves_kernel` is written only by the kernel's own LDS-bound loads: one
   `s_mov_b32 m0` per such load and no other instruction that names M0.
 """
 from __future__ import annotations
@@ -55,6 +57,12 @@ LIMITS = [
     ("prefix_attn.hip", r"prefix_attention_kernel<", {"occupancy": (2, 8), "lds": (0, 80 * 1024)}),
     ("kv_append.hip", r".", {"scratch": (0, 0), "vgpr_spill": (0, 0)}),
     ("prefix_attn.hip", r".", {"scratch": (0, 0), "vgpr_spill": (0, 0)}),
+    ("mx4.hip", r".", {"scratch": (0, 0), "vgpr_spill": (0, 0)}),
+    ("mx4_gemm.hip", r".", {"scratch": (0, 0), "vgpr_spill": (0, 0)}),
+    ("mx4_gemm.hip", r"mx4_halves_kernel<", {"agprs": (256, 256), "occupancy": (1, 1), "lds": (0, 160 * 1024)}),
+    ("mx4_gemm.hip", r"mx4_tile_kernel<", {"occupancy": (2, 8), "lds": (0, 80 * 1024)}),
+    ("mx4_gemm.hip", r"mx4_slim_kernel<\d, 1, 1>", {"occupancy": (8, 8), "lds": (0, 40 * 1024)}),
+    ("kv_pages.hip", r".", {"scratch": (0, 0), "vgpr_spill": (0, 0)}),
     ("sgmv_prefill.hip", r"sgmv_expand_kernel<\d, \d+, true>", {"occupancy": (4, 8), "lds": (0, 40 * 1024)}),
 ]
 
@@ -143,7 +151,7 @@ def violations(source: str, report):
                     if not lo <= rec.get(field, -1) <= hi:
                         bad.append(f"{source}: {name}: {field} = {rec.get(field)}, allowed {lo}..{hi}")
     for name, rec in report.items():
-        if re.search(r"gemm_lora_(short_)?kernel<|sgmv_shrink_kernel<|w4_wide_kernel<", name):
+        if re.search(r"gemm_lora_(short_)?kernel<|sgmv_shrink_kernel<|w4_wide_kernel<|mx4_(tile|halves)_kernel<", name):
             if rec.get("m0_other", 1) != 0 or rec.get("m0_writes", 0) != rec.get("lds_loads", -1):
                 bad.append(f"{source}: {name}: M0 is named by {rec.get('m0_other')} instructions besides its "
                            f"{rec.get('m0_writes')} writes, for {rec.get('lds_loads')} LDS-bound loads")

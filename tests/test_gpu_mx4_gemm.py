@@ -65,16 +65,16 @@ def test_output_widths(n):
     run(260, 256, n, BF16, seed=n)
 
 
-FORMS = {(16, 16): (17, 136, 72), (32, 16): (17, 136, 2056), (16, 32): (50, 2184, 1032), (32, 32): (50, 1032, 2056), (32, 64): (257, 1032, 1032), (64, 64): (201, 2184, 2056),
-         (128, 64): (300, 136, 2056), (128, 128): (1030, 136, 2056), (128, 256): (1030, 1160, 4104), (256, 256): (1030, 2184, 8200)}
+# the last three: tiles of 256 tokens alone, halves alone, both
+FORMS = [((16, 16), 17, 136, 72), ((32, 16), 17, 136, 2056), ((16, 32), 50, 2184, 1032), ((32, 32), 50, 1032, 2056), ((32, 64), 257, 1032, 1032), ((64, 64), 201, 2184, 2056),
+         ((128, 64), 300, 136, 2056), ((128, 128), 1030, 136, 2056), ((256, 256), 1030, 2184, 8200), ((256, 256), 1030, 2184, 4104), ((256, 256), 2570, 1160, 8200)]
 
 
 @pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("form", FORMS)
-def test_every_form(form, dtype, accumulate):
+@pytest.mark.parametrize("form, T, k, n", FORMS)
+def test_every_form(form, T, k, n, dtype, accumulate):
     """Sizes that end inside a block, a tile, a quad of tiles and a workgroup's columns and tokens."""
-    T, k, n = FORMS[form]
     shape = (C.c_int32 * 2)()
     assert _ext.lib().mlora_mx4_form(1, (C.c_int32 * 1)(k), (C.c_int32 * 1)(n), T, shape) == 0 and tuple(shape) == form
     run(T, k, n, dtype, accumulate=accumulate)
@@ -84,7 +84,7 @@ def test_every_form(form, dtype, accumulate):
 def test_steps_of_the_large_tiles(k):
     """Every number of steps on either side of a ring's four stages."""
     say(f"large tiles k={k}")
-    for T, n in ((1100, 8200), (1030, 4104), (1030, 2056), (300, 2056)):
+    for T, n in ((2570, 8200), (1030, 4104), (1030, 2056), (300, 2056)):
         run(T, k, n, BF16, seed=k)
 
 
