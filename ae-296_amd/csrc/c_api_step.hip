@@ -144,6 +144,8 @@ int pages_args(mlora::PagesArgs &a, void *state, int64_t state_words, void *scra
     if (state_words < at[6] || scratch_words < at[7])
         return fail(MLORA_ENOSPACE, "state and scratch have %lld and %lld words, %lld and %lld needed", (long long)state_words, (long long)scratch_words,
                     (long long)at[6], (long long)at[7]);
+    if (wants && (overlap(want, (size_t)n_req * 4, state, (size_t)state_words * 4) || overlap(want, (size_t)n_req * 4, scratch, (size_t)scratch_words * 4)))
+        return fail(MLORA_EINVAL, "the rows' values must not lie in state or scratch");
     const mlora::PagesLayout l = mlora::pages_layout(n_req, max_pages, n_pages);
     int32_t *s = static_cast<int32_t *>(state), *c = static_cast<int32_t *>(scratch);
     memset(&a, 0, sizeof(a));

@@ -43,7 +43,9 @@ class KVCache:
         """n free page ids."""
         if n < 0 or n > len(self._free):
             raise MemoryError(f"cache full: {n} pages needed, {len(self._free)} free")
-        got = [self._free.pop() for _ in range(n)]
+        rest = len(self._free) - n
+        got = self._free[rest:][::-1]
+        del self._free[rest:]
         self._used.update(got)
         return got
 

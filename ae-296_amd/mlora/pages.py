@@ -24,8 +24,9 @@ from .attention import KVCache
 
 
 class KVPages:
-    """Tables for `n_req` requests of up to `max_pages` pages each, over `n_pages` pages taken from the cache (by default all it has free).  `state` holds all of
-    it (int32): a copy of it is a snapshot, and copying that back restores it, but not what was written to the cache meanwhile."""
+    """Tables for `n_req` requests of up to `max_pages` pages each, over `n_pages` pages taken from the cache (by default all it has
+    free).  `state` holds all of it (int32): a copy of it is a snapshot, which may be copied back until the next ``take``, ``give_back`` or
+    ``compact``; what was written to the cache meanwhile stays written."""
 
     def __init__(self, cache: KVCache, n_req: int, max_pages: int, n_pages: Optional[int] = None):
         at = (C.c_int64 * _ext.PAGES_LAYOUT_WORDS)()
@@ -47,12 +48,13 @@ class KVPages:
 
     def take(self, n: int) -> None:
         """n more pages of the cache."""
-        ids = torch.tensor(self.cache.allocate(n), dtype=torch.long, device=self.state.device)
+        ids = torch.from_numpy(np.array(self.cache.allocate(n), np.int64)).to(self.state.device)
         self._managed[ids] = 1
         self._free[ids] = 1
 
     def give_back(self) -> int:
-        """Gives the cache the pages behind the last one in use (all that are free, after ``compact``) and returns how many.  Waits for the device."""
+        """Gives the cache the pages behind the last one in use (all that are free, after ``compact``) and returns how many.
+        Waits for the device."""
         managed, free = self._managed.cpu().numpy().astype(bool), self._free.cpu().numpy().astype(bool)
         used = np.flatnonzero(managed & ~free)
         ids = np.flatnonzero(free)
@@ -60,49 +62,59 @@ class KVPages:
         gone = torch.from_numpy(ids).to(self.state.device)
         self._managed[gone] = 0
         self._free[gone] = 0
-        self.cache.release(ids[::-1].tolist())
+        self.cache.release(ids.tolist())
         return len(ids)
 
     def adopt(self, table: torch.Tensor, lens: torch.Tensor) -> None:
-        """Tables and lengths from elsewhere (int32 [n_req, max_pages] and [n_req]) in place of the present ones; pages that several rows name are shared, and what
-        lies behind a row's last page does not count.  Waits for the device."""
+        """Tables and lengths from elsewhere (int32 [n_req, max_pages] and [n_req]) in place of the present ones; pages that several rows
+        name are shared, and what lies behind a row's last page does not count.  Waits for the device."""
         if tuple(table.shape) != (self.n_req, self.max_pages) or tuple(lens.shape) != (self.n_req,):
             raise ValueError(f"expected a table [{self.n_req}, {self.max_pages}] and {self.n_req} lengths")
-        n = lens.cpu().numpy().astype(np.int64)
-        if (n < 0).any() or (n > self.max_pages * self.cache.page_tokens).any():
-            raise ValueError(f"lengths must be in 0..{self.max_pages * self.cache.page_tokens}")
-        held = torch.arange(self.max_pages, device=table.device) < torch.from_numpy(-(-n // self.cache.page_tokens)).to(table.device)[:, None]
-        ids = table[held].long()
-        if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= self.cache.n_pages or not bool(self._managed.to(ids.device)[ids].all())):
+        M, N, device = self.max_pages, self.cache.n_pages, self.state.device
+        table, lens = table.to(device), lens.to(device)
+        n, column = lens.long(), torch.arange(M, device=device)
+        held = column < ((n + self.cache.page_tokens - 1) // self.cache.page_tokens)[:, None]
+        # entries that do not count: places of their own behind the last page, a column each
+        at = torch.where(held, table, N + column)
+        exists = (at >= 0) & (at < N + M)
+        at = torch.where(exists, at, N + column)
+        known = torch.cat((self._managed.bool(), torch.ones(M, dtype=torch.bool, device=device)))
+        in_order = torch.sort(at, 1)[0]
+        fine = torch.stack((((n >= 0) & (n <= M * self.cache.page_tokens)).all(), exists.all() & (known[at] | ~held).all() & ((at < N) == held).all(),
+                            (in_order[:, 1:] != in_order[:, :-1]).all())).tolist()
+        if not fine[0]:
+            raise ValueError(f"lengths must be in 0..{M * self.cache.page_tokens}")
+        if not fine[1]:
             raise ValueError("a row names a page that is not among the managed ones")
-        pairs = torch.sort(held.nonzero()[:, 0] * self.cache.n_pages + ids)[0]
-        if bool((pairs[1:] == pairs[:-1]).any()):
+        if not fine[2]:
             raise ValueError("a row names a page twice")
-        refs = torch.bincount(ids, minlength=self.cache.n_pages).to(torch.int32)
-        self.table.copy_(table.masked_fill(~held, -1))
-        self.lens.copy_(lens)
-        self.refs.copy_(refs)
+        refs = torch.zeros(N + M, dtype=torch.int32, device=device)
+        refs.index_add_(0, at.view(-1), torch.ones_like(at, dtype=torch.int32).view(-1))
+        self.table.copy_(torch.where(held, at, -1))
+        self.lens.copy_(n)
+        self.refs.copy_(refs[:N])
         self._free.copy_(self._managed.bool() & (self.refs == 0))
 
     def resize(self, want: torch.Tensor) -> None:
-        """Rows' new lengths, int32 [n_req] on the device (negative: as it is; 0 gives all pages back).  Shorter rows give pages back first; then longer rows, in
-        their order, get the lowest free ids.  A longer row that will write on a page other rows name as well gets its own copy of what that
-        holds, in all layers - the last of them keeps the page if all of them do.  A row that does not fit keeps its length and pages and counts in
-        `failed`; so does every later one that needs a page."""
+        """Rows' new lengths, int32 [n_req] on the device and not `lens` itself (negative: as it is; 0 gives all pages back).  Shorter
+        rows give pages back first; then longer rows, in their order, get the lowest free ids.  A longer row that will write on a page other
+        rows name as well gets its own copy of what that holds, in all layers - the last of them keeps the page if all of them do.  A row
+        that does not fit keeps its length and pages and counts in `failed`; so does every later one that needs a page."""
         rc = _ext.host().pages_resize(self, want)
         if rc:
             _ext.check(rc)
 
     def fork(self, parent: torch.Tensor) -> None:
-        """Row r goes on from row parent[r]'s tokens (int32 [n_req] on the device; negative or r itself: from its own), all rows at once, so a permutation is one
-        too.  Pages are shared until one of the rows writes on them (``resize``).  A parent of n_req or more counts in `failed`."""
+        """Row r goes on from row parent[r]'s tokens (int32 [n_req] on the device; negative or r itself: from its own), all rows at once,
+        so a permutation is one too.  Pages are shared, the last one too: ``resize`` comes before the next token is appended, and
+        copies what would be written on.  A parent of n_req or more leaves the row as it is and counts in `failed`."""
         rc = _ext.host().pages_fork(self, parent)
         if rc:
             _ext.check(rc)
 
     def compact(self) -> None:
-        """Moves the pages in use to the lowest ids, with their keys and values; `live` says how many there are.  Tables made before (plans, copies of `table`) are
-        void afterwards."""
+        """Moves the pages in use to the lowest ids, with their keys and values; `live` says how many there are.  Copies of `table` made
+        before are void afterwards."""
         rc = _ext.host().pages_compact(self)
         if rc:
             _ext.check(rc)

@@ -1042,7 +1042,7 @@ def main():
                          "reference's arrival trace; swap = adapter swap-in from pinned host memory; assist = CPU-assist transport; "
                          "f1 = base projection + LoRA in one pass on the config-4 batch; reflayout = the reference's pool layout and call; "
                          "coldstart = prefill latency with the adapter cached, loading (CPU-assisted) and loaded on demand")
-    ap.add_argument("--case", help="run ten passes of this case of perf/cases.py or perf/operators.py and end, for a kernel trace (nothing is timed)")
+    ap.add_argument("--case", help="run ten passes of this case of perf/cases.py, perf/operators.py or perf/more_operators.py and end, for a kernel trace (nothing is timed)")
     args = ap.parse_args()
     if args.gpus != 1:
         print("bench.py measures one GPU: this build has no multi-GPU path (run with --gpus 1)", file=sys.stderr)
@@ -1059,9 +1059,9 @@ def main():
     dev = torch.device("cuda:0")
     torch.cuda.set_device(dev)
     if args.case:
-        from perf import cases, operators
-        operators.own = True
-        cases, case = next((m, c) for m in (cases, operators) for c in m.listed() if c["name"] == args.case)
+        from perf import cases, more_operators, operators
+        operators.own = more_operators.own = True
+        cases, case = next((m, c) for m in (cases, operators, more_operators) for c in m.listed() if c["name"] == args.case)
         state = cases.prepare(case, 1)
         for _ in range(10):
             cases.run(state)

@@ -550,7 +550,7 @@ int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const
  *     and names the parent's.  A parent of n_req or more leaves the row as it is and is counted in `failed`.
  *   mlora_pages_compact: with n managed pages in use (left in `live`), those that are not among the n lowest managed ids move, in their order,
  *     to the free ids among these: keys and values of all layers, tables and refs.
- * k_pages and v_pages: all layers' slabs, [n_layers, n_pages, n_kv_heads, page_tokens, head_dim].  n_req <= 2^20, n_req * max_pages <= 2^30, n_pages <= 2^24.
+ * want and parent must not lie in state or scratch.  k_pages and v_pages: all layers' slabs, [n_layers, n_pages, n_kv_heads, page_tokens, head_dim].  n_req <= 2^20, n_req * max_pages <= 2^30, n_pages <= 2^24.
  * The counterpart of the reference's MemoryManager (lightllm/common/mem_manager.py:4-111) and its request table (req_manager.py:3-36).
  */
 #define MLORA_PAGES_LAYOUT_WORDS 8

@@ -176,6 +176,7 @@ def test_pages_are_taken_and_given_back():
     assert p.model.failed == 2 and p.pages.give_back() == 0
     p.resize([0, 0])
     assert p.pages.give_back() == 3 and p.cache.free_pages == 30
+    assert p.cache.allocate(3) == [0, 1, 2]
 
 
 def test_adopted_tables():

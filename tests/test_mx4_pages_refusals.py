@@ -14,7 +14,6 @@ one = C.c_void_p(16)          # never dereferenced: every call below fails valid
 off = C.c_void_p(8)
 OK, EINVAL, ERANGE, EALIGN, EDTYPE, ENOSPACE = (_ext.MLORA_OK, _ext.MLORA_EINVAL, _ext.MLORA_ERANGE, _ext.MLORA_EALIGN,
                                                 _ext.MLORA_EDTYPE, _ext.MLORA_ENOSPACE)
-BIG = 1 << 40
 
 
 def ptrs(*v):
@@ -117,7 +116,7 @@ def test_layout():
     (dict(heads=(1 << 14) + 1), ERANGE)])
 def test_page_calls(kw, code):
     lib = _ext.lib()
-    a = dict(state=one, words=BIG, scratch=one, scratch_words=BIG, want=one, n_req=4, max_pages=5, n_pages=70, P=16, k=one, v=one, layers=2, heads=2, D=64)
+    a = dict(state=one, words=1 << 20, scratch=one, scratch_words=1 << 20, want=C.c_void_p(1 << 30), n_req=4, max_pages=5, n_pages=70, P=16, k=one, v=one, layers=2, heads=2, D=64)
     a.update(kw)
     slabs = (a["k"], a["v"], a["layers"], a["n_pages"], a["heads"], a["P"], a["D"])
     assert lib.mlora_pages_resize(a["state"], a["words"], a["scratch"], a["scratch_words"], a["want"], a["n_req"], a["max_pages"], *slabs, None) == code
@@ -125,6 +124,15 @@ def test_page_calls(kw, code):
         assert lib.mlora_pages_compact(a["state"], a["words"], a["scratch"], a["scratch_words"], a["n_req"], a["max_pages"], *slabs, None) == code
     if not {"k", "v", "layers", "heads", "D"} & set(kw):
         assert lib.mlora_pages_fork(a["state"], a["words"], a["scratch"], a["scratch_words"], a["want"], a["n_req"], a["max_pages"], a["n_pages"], a["P"], None) == code
+
+
+def test_rows_values_inside_the_tables():
+    """Lengths given as the tables' own would never differ from them, and parents there would change under the call."""
+    lib, state, scratch = _ext.lib(), 1 << 20, 1 << 24
+    for want in (state, state + 56 * 4, state - 12, scratch + 4 * 127):
+        assert lib.mlora_pages_resize(C.c_void_p(state), 128, C.c_void_p(scratch), 1 << 16, C.c_void_p(want), 4, 5, one, one, 2, 70, 2, 16, 64, None) == EINVAL
+        assert lib.mlora_pages_fork(C.c_void_p(state), 128, C.c_void_p(scratch), 1 << 16, C.c_void_p(want), 4, 5, 70, 16, None) == EINVAL
+        assert b"must not lie" in lib.mlora_last_error()
 
 
 def host_pages(n_req=3, max_pages=4, n_pages=20, taken=None):
