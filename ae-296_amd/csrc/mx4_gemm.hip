@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64 * MX_WAVES) void mx4_slim_kernel(const Mx4Args p
 #pragma unroll
         for (int j = 0; j < MT; j++) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
     // Where a wavefront holds more than one tile of each, the next quad's are asked for before this one's are multiplied (64 tokens, 4096 -> 4096: 6.2 -> 5.7 us);
-    // with one, twice the registers cost resident workgroups (16 tokens, 4096 -> 2 x 13824: 15.5 -> 18.6 us).  Lanes of rows that x does not have load nothing.
+    // with one, twice the registers cost resident workgroups (16 tokens, 5120 -> 2 x 13824: 15.5 -> 18.6 us).  Lanes of rows that x does not have load nothing.
     struct Ops { uint4 a[4][NT], b[4][MT]; uint32_t sa[NT], sb[MT]; } ops[2];
     auto load = [&](Ops &o, int quad) {
 #pragma unroll
@@ -397,8 +397,8 @@ __global__ __launch_bounds__(MX_NT * KS) void mx4_tile_kernel(const Mx4Args p)
 //
 // What bounds it: power.  A step of a whole tile is 128 matrix instructions, 1024 cycles of each pipe.  On one unit alone it takes 500 ns, 0.86 of the pipes' rate
 // at 2.4 GHz (a barrier a step and one wavefront a pipe); with all units at work 795 ns, where the instructions alone, from registers and on
-// random numbers, take 700 (6.1 PFLOP/s; on zeros 9.4): the card lowers its clock to 1.7 GHz.  64 rows of either operand in LDS for every 32 read feed the pipes at half of
-// the LDS' rate; 128 x 128 tiles need all of it and run at 1.5 GHz.
+// random numbers, take 700 (5.9 to 6.4 PFLOP/s; on ones up to 9.4): the card lowers its clock to 1.7 GHz.  64 rows of either operand in LDS for every 32 read
+// feed the pipes at half of the LDS' rate; 128 x 128 tiles need all of it and run at 1.5 GHz.
 template <int DT, bool ACC>
 __global__ __launch_bounds__(MX_NT) void mx4_halves_kernel(const Mx4Args p)
 {
