@@ -57,6 +57,13 @@ int check_mx4_packed(const void *packed, int64_t bytes, const mlora::Mx4Shape &s
     return MLORA_OK;
 }
 
+// Rows of 16-bit elements beside a packed operand: workgroups read one and write the other in no order.
+int check_mx4_apart(const void *x, int64_t stride, const void *packed, const mlora::Mx4Shape &sh)
+{
+    if (overlap(x, ((size_t)(sh.rows - 1) * stride + sh.k) * 2, packed, sh.bytes)) return fail(MLORA_EINVAL, "packed overlaps the rows");
+    return MLORA_OK;
+}
+
 // The sizes of a call's products; the pointers follow.
 int mx4_sizes(mlora::Mx4Args &a, int n_proj, const int32_t *hin, const int32_t *hout, int T)
 {
@@ -361,7 +368,7 @@ int mlora_mx4_quantize(const void *x, int64_t x_stride, int rows, int k, int dty
     if (!x) return fail(MLORA_EINVAL, "x must not be NULL");
     if (!aligned16(x) || (x_stride & 7)) return fail(MLORA_EALIGN, "x must be 16-byte aligned and x_stride a multiple of 8 (got %lld)", (long long)x_stride);
     if (x_stride < k && rows > 1) return fail(MLORA_EINVAL, "x_stride must be at least k (got %lld)", (long long)x_stride);
-    if ((rc = check_mx4_packed(packed, packed_bytes, a.sh))) return rc;
+    if ((rc = check_mx4_packed(packed, packed_bytes, a.sh)) || (rc = check_mx4_apart(x, x_stride, packed, a.sh))) return rc;
     a.x = static_cast<const uint16_t *>(x); a.x_stride = x_stride; a.packed = static_cast<unsigned char *>(packed);
     return launched(mlora::launch_mx4_quantize(a, dtype, static_cast<hipStream_t>(stream)), "quantize");
 }
@@ -375,6 +382,8 @@ int mlora_mx4_pack(const uint8_t *codes, const uint8_t *scales, int rows, int k,
     a.sh = mlora::mx4_shape(rows, k);
     if (!codes || !scales) return fail(MLORA_EINVAL, "codes and scales must not be NULL");
     if ((rc = check_mx4_packed(packed, packed_bytes, a.sh))) return rc;
+    if (overlap(codes, (size_t)rows * (k / 2), packed, a.sh.bytes) || overlap(scales, (size_t)rows * a.sh.blocks, packed, a.sh.bytes))
+        return fail(MLORA_EINVAL, "packed overlaps codes or scales");
     a.codes = codes; a.scales = scales; a.packed = static_cast<unsigned char *>(packed);
     return launched(mlora::launch_mx4_pack(a, static_cast<hipStream_t>(stream)), "pack");
 }
@@ -390,7 +399,7 @@ int mlora_mx4_values(const void *packed, int64_t packed_bytes, int rows, int k, 
     if (!out) return fail(MLORA_EINVAL, "out must not be NULL");
     if (!aligned16(out) || (out_stride & 7)) return fail(MLORA_EALIGN, "out must be 16-byte aligned and out_stride a multiple of 8 (got %lld)", (long long)out_stride);
     if (out_stride < k && rows > 1) return fail(MLORA_EINVAL, "out_stride must be at least k (got %lld)", (long long)out_stride);
-    if ((rc = check_mx4_packed(packed, packed_bytes, a.sh))) return rc;
+    if ((rc = check_mx4_packed(packed, packed_bytes, a.sh)) || (rc = check_mx4_apart(out, out_stride, packed, a.sh))) return rc;
     a.packed = static_cast<const unsigned char *>(packed); a.out = static_cast<uint16_t *>(out); a.out_stride = out_stride;
     return launched(mlora::launch_mx4_values(a, dtype, static_cast<hipStream_t>(stream)), "values");
 }

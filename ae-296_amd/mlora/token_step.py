@@ -1,4 +1,5 @@
-"""One decode step of the attention blocks: 4-bit base projections (16-bit inputs on ``W4Weight``, or 4-bit ones on ``MX4Weight``), every token's adapter, rotation and append, attention.
+"""One decode step of the attention blocks: 4-bit base projections (16-bit inputs on ``W4Weight``, or 4-bit ones on ``MX4Weight``), every
+token's adapter, rotation and append, attention.
 
     step = TokenStep(pool, cache, weights, n_q_heads, rope)
     step.begin(batch, tok_adapter)                  # once per step: both plans

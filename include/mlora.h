@@ -517,6 +517,7 @@ int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t
  *     at most.  A block with an infinity or a NaN is NaN.
  *   mlora_mx4_pack: from codes uint8 [rows, k / 2] (an even column in the low half of a byte; sign in bit 3) and scales uint8 [rows, ceil(k / 32)].
  *   mlora_mx4_values: the values a packed operand stands for, rounded to the 16-bit type (exact for what was quantised from that type).
+ *     In these three, packed may not overlap what it is made from or what is made from it.
  *   mlora_mx4_gemm_multi takes y (16-bit [T, hout]), x and w (packed), hin and hout as HOST arrays of n_proj entries; no y may overlap another y, an x
  *     or a w.  Products exact, sums in fp32, the result rounded once; a block with a NaN makes its results NaN, and where a sum leaves fp32's range
  *     the result is infinite or NaN.
@@ -550,7 +551,8 @@ int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const
  *     and names the parent's.  A parent of n_req or more leaves the row as it is and is counted in `failed`.
  *   mlora_pages_compact: with n managed pages in use (left in `live`), those that are not among the n lowest managed ids move, in their order,
  *     to the free ids among these: keys and values of all layers, tables and refs.
- * want and parent must not lie in state or scratch.  k_pages and v_pages: all layers' slabs, [n_layers, n_pages, n_kv_heads, page_tokens, head_dim].  n_req <= 2^20, n_req * max_pages <= 2^30, n_pages <= 2^24.
+ * want and parent must not lie in state or scratch.  k_pages and v_pages: all layers' slabs, [n_layers, n_pages, n_kv_heads, page_tokens,
+ * head_dim].  n_req <= 2^20, n_req * max_pages <= 2^30, n_pages <= 2^24.
  * The counterpart of the reference's MemoryManager (lightllm/common/mem_manager.py:4-111) and its request table (req_manager.py:3-36).
  */
 #define MLORA_PAGES_LAYOUT_WORDS 8

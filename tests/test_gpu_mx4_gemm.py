@@ -157,6 +157,27 @@ def test_quantised_input_and_weight_end_to_end():
     compare(y, ref.values(*ref.quantize(ref.f64(x))), ref.values(*ref.quantize(ref.f64(w.t()))), F16)
 
 
+def test_calls_on_two_streams_at_once():
+    say("mx4_gemm two streams")
+    ws = [operand(n, 2048, 60 + n, 3, mlora.MX4Weight)[0] for n in (264, 4096)]
+    xs = [torch.randn((T, 2048), generator=torch.Generator().manual_seed(T)).to(BF16).cuda() for T in (700, 33)]
+    want = []
+    for x, w in zip(xs, ws):
+        y = torch.empty((x.shape[0], w.hout), dtype=BF16, device="cuda")
+        mlora.mx4_gemm([y], [mlora.mx4_quantize(x)], [w])
+        want.append(y)
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[torch.empty_like(y) for _ in range(8)] for y in want]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for s, x, w, ys in zip(streams, xs, ws, got):
+            with torch.cuda.stream(s):
+                mlora.mx4_gemm([ys[i]], [mlora.mx4_quantize(x)], [w])
+    torch.cuda.synchronize()
+    for ys, y in zip(got, want):
+        assert all(torch.equal(a, y) for a in ys)
+
+
 def test_runs_are_alike_on_a_stream_of_ones_own_and_in_a_graph():
     say("mx4_gemm stream and graph")
     T, k, n = 130, 4096, 512

@@ -255,6 +255,44 @@ def test_steps_captured_in_a_graph():
             p.compact()
 
 
+def test_two_graphs_and_eager_calls_share_the_tables():
+    say("pages two graphs")
+    p = Pair(6, 5, 24)
+    want, parent = p.ints([-1] * 6), p.ints([-1] * 6)
+    grow, spread = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(grow):
+        p.pages.resize(want)
+    with torch.cuda.graph(spread):
+        p.pages.fork(parent)
+        p.pages.resize(want)
+        p.pages.compact()
+    rng = np.random.default_rng(11)
+    for i in range(5):
+        w = np.minimum(np.array(p.model.lens) + rng.integers(0, 20, 6), 80).tolist()
+        for a, b, n in p.model.resize(w):
+            for t in (p.k, p.v):
+                t[:, b, :, :n] = t[:, a, :, :n]
+        want.copy_(p.ints(w))
+        grow.replay()
+        p.check(f"grow {i}")
+        f = np.where(rng.random(6) < 0.4, rng.integers(0, 6, 6), -1).tolist()
+        p.model.fork(f)
+        w = [max(n - int(rng.integers(0, 5)), 0) if rng.random() < 0.5 else min(n + 1, 80) for n in p.model.lens]
+        for a, b, n in p.model.resize(w):
+            for t in (p.k, p.v):
+                t[:, b, :, :n] = t[:, a, :, :n]
+        moves = p.model.compact()
+        for t in (p.k, p.v):
+            old = t.clone()
+            for a, b in moves:
+                t[:, b] = old[:, a]
+        parent.copy_(p.ints(f))
+        want.copy_(p.ints(w))
+        spread.replay()
+        p.check(f"spread {i}")
+        p.resize([0 if r == i else n for r, n in enumerate(p.model.lens)])
+
+
 def test_keys_follow_their_request():
     """Tables as a decode step uses them: two answers forked from one prompt write different tokens and each attends to its own."""
     say("pages and attention")

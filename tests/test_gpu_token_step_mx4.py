@@ -136,6 +136,23 @@ def test_a_captured_step_replays():
         assert torch.equal(once(), got) and torch.equal(pages.state, state) and torch.equal(cache.k, k), i
 
 
+def test_batches_of_no_and_of_few_tokens_in_turn():
+    """One step object over batches whose operands share a buffer, one of them empty."""
+    print("[gpu-case] mx4 token step batches in turn", flush=True)
+    pool, _, cache, g = build(1, 136, 4, 2, 64, 3, torch.float16, 40, 1)
+    _, packed = weights_of(1, pool.projections, torch.float16, 2)
+    step = mlora.TokenStep(pool, cache, packed, 4, mlora.RopeTable(64, 64))
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")          # noqa: E731
+    for T in (5, 0, 8, 0, 6, 1, 33):
+        batch = mlora.KVBatch(i32(range(T)), i32([0] * T), i32([[t] for t in range(max(T, 1))]))
+        x = torch.randn((T, 136), device="cuda", generator=g).half()
+        step.begin(batch, i32([-1] * T))
+        assert step.layer(0, x).shape[0] == T
+        v = torch.empty((T, step.widths[2]), dtype=torch.float16, device="cuda")
+        mlora.mx4_gemm([v], [mlora.mx4_quantize(x)], [packed[0]["v"]])
+        assert torch.equal(step.qkv[2], v), T
+
+
 def test_kinds_of_weights():
     pool, _, cache, g = build(1, 128, 4, 2, 64, 3, torch.float16, 8, 1)
     plain, packed = weights_of(1, pool.projections, torch.float16, 2)

@@ -51,6 +51,18 @@ def test_pack_arguments(kw, code):
     assert _ext.lib().mlora_mx4_pack(a["c"], a["s"], a["rows"], a["k"], a["p"], a["n"], None) == code
 
 
+# 3 rows of 64 columns, 80 elements apart: 448 bytes; packed 1280, codes 96, scales 6
+@pytest.mark.parametrize("at", [1 << 20, (1 << 20) + 432, (1 << 20) - 1264])
+def test_operands_that_overlap_their_source(at):
+    lib, rows, packed = _ext.lib(), C.c_void_p(1 << 20), C.c_void_p(at)
+    assert lib.mlora_mx4_quantize(rows, 80, 3, 64, 0, packed, 1280, None) == EINVAL
+    assert lib.mlora_mx4_values(packed, 1280, 3, 64, rows, 80, 1, None) == EINVAL
+    near = C.c_void_p(at if at != (1 << 20) + 432 else (1 << 20) + 80)
+    assert lib.mlora_mx4_pack(rows, one, 3, 64, near, 1280, None) == EINVAL
+    near = C.c_void_p(at if at != (1 << 20) + 432 else 1 << 20)
+    assert lib.mlora_mx4_pack(one, rows, 3, 64, near, 1280, None) == EINVAL
+
+
 def gemm(**kw):
     a = dict(n=2, y=ptrs(1 << 20, 2 << 20, *[16] * 6), x=ptrs(3 << 20, 3 << 20, *[16] * 6), w=ptrs(4 << 20, 5 << 20, *[16] * 6), hin=ints(64), hout=ints(64), T=3, dtype=0)
     a.update(kw)
