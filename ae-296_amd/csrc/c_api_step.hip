@@ -157,7 +157,7 @@ int pages_args(mlora::PagesArgs &a, void *state, int64_t state_words, void *scra
     int32_t *s = static_cast<int32_t *>(state), *c = static_cast<int32_t *>(scratch);
     memset(&a, 0, sizeof(a));
     a.free_pages = reinterpret_cast<uint8_t *>(s); a.table = s + l.table; a.lens = s + l.lens; a.refs = s + l.refs; a.failed = s + l.failed; a.live = s + l.live;
-    a.managed = reinterpret_cast<const uint8_t *>(c); a.head = c + l.head; a.writers = c + l.writers; a.last_writer = c + l.last_writer; a.picked = c + l.picked;
+    a.managed = reinterpret_cast<const uint8_t *>(c); a.grown = c + l.grown; a.head = c + l.head; a.writers = c + l.writers; a.last_writer = c + l.last_writer; a.picked = c + l.picked;
     a.move_from = c + l.move_from; a.word_movers = c + l.word_movers; a.word_rank = c + l.word_rank; a.row_page = c + l.row_page;
     a.row_new = c + l.row_new; a.row_copy = c + l.row_copy; a.copies = c + l.copies; a.rows = c + l.rows; a.pieces = c + l.pieces;
     a.want = want; a.n_pages = n_pages; a.n_req = n_req; a.max_pages = max_pages; a.page_shift = log2_exact(page_tokens);

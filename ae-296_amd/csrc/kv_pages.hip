@@ -3,7 +3,8 @@
 // neighbouring ids, which rows mostly have, meet in one word (2048 pages of a row given back by a workgroup: 28 us in bits).
 //
 // resize gives every row its new length: pages behind a shorter end go back, a longer one gets the lowest free ids, row by row, and a row that
-// will write on a page others name as well gets a copy of what it holds there.  fork lets rows go on from other rows' tokens, sharing their
+// will write on a page others name as well gets a copy of what it holds there.  Which rows got longer is left in grown: no other row may be written
+// on, as the pages behind its end may be shared.  fork lets rows go on from other rows' tokens, sharing their
 // pages.  compact moves the pages in use to the lowest ids.  Which id a page gets depends on the tables alone: ids are dealt out by sums over rows
 // and bits, and counts are changed by atomics whose order no result shows.
 //
@@ -262,6 +263,7 @@ __global__ __launch_bounds__(ASSIGN_NT) void pages_assign_kernel(const PagesArgs
         if (served && need) atomicMax(&granted, upto);
         if (gets > 4) atomicMax(&widest, gets);
         if (served || g.shorter) p.lens[r] = g.want;
+        if (r < p.n_req) p.grown[r] = served ? r : -1;
         copies_page = served && copy;
         if (!ONE && r < p.n_req) {
             p.row_new[3 * r] = (int)gets;
@@ -402,7 +404,10 @@ __device__ __forceinline__ int parent_of(const PagesArgs &p, int r)
 __global__ __launch_bounds__(256) void pages_fork_kernel(const PagesArgs p)
 {
     const int pieces = (p.max_pages + ROW_PIECE - 1) / ROW_PIECE, r = blockIdx.x / pieces, i0 = (blockIdx.x - r * pieces) * ROW_PIECE;
-    if (p.want[r] >= p.n_req && i0 == 0 && threadIdx.x == 0) atomicAdd(p.failed, 1);
+    if (i0 == 0 && threadIdx.x == 0) {
+        if (p.want[r] >= p.n_req) atomicAdd(p.failed, 1);
+        p.grown[r] = -1;                                    // last pages may be shared from now on
+    }
     const int of = parent_of(p, r);
     if (of < 0) return;
     const int tokens = p.lens[of], had = pages_of(p.lens[r], p.page_shift, p.max_pages), gets = pages_of(tokens, p.page_shift, p.max_pages);

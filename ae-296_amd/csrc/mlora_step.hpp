@@ -134,13 +134,13 @@ struct KvAppendArgs {
     int32_t *bad;
 };
 // ---- the cache's page tables.  State, one buffer of int32 words: [free: a byte a page, 0 or 1, to a multiple of 64][table n_req * max_pages]
-// [lens n_req][refs n_pages][failed][live].  Scratch, likewise: [managed: bytes as free][words of head][writers n_pages][last_writer n_pages] - these three are set once,
-// and the counts are zeros again after every call - then [picked n_pages][move_from n_pages][word_rank][word_movers][row_page n_req]
+// [lens n_req][refs n_pages][failed][live].  Scratch, likewise: [managed: bytes as free][grown n_req][words of head][writers n_pages][last_writer n_pages] - all but grown are
+// set once, and the counts are zeros again after every call - then [picked n_pages][move_from n_pages][word_rank][word_movers][row_page n_req]
 // [row_new 3 n_req][row_copy 2 n_req][copies 3 n_req][rows n_req * max_pages][pieces: a word for every ROW_PIECE entries of a row].
 constexpr int ROW_PIECE = 1024;                // entries of a row that a workgroup takes
 struct PagesLayout {
     int64_t table, lens, refs, failed, live, state_words;
-    int64_t head, writers, last_writer, picked, move_from, word_rank, word_movers, row_page, row_new, row_copy, copies, rows, pieces, scratch_words;
+    int64_t grown, head, writers, last_writer, picked, move_from, word_rank, word_movers, row_page, row_new, row_copy, copies, rows, pieces, scratch_words;
 };
 inline PagesLayout pages_layout(int64_t n_req, int64_t max_pages, int64_t n_pages)
 {
@@ -152,7 +152,8 @@ inline PagesLayout pages_layout(int64_t n_req, int64_t max_pages, int64_t n_page
     l.failed = l.refs + n_pages;
     l.live = l.failed + 1;
     l.state_words = l.live + 1;
-    l.head = 16 * words;
+    l.grown = 16 * words;
+    l.head = l.grown + n_req;
     l.writers = l.head + 2;
     l.last_writer = l.writers + n_pages;
     l.picked = l.last_writer + n_pages;
@@ -171,7 +172,7 @@ inline PagesLayout pages_layout(int64_t n_req, int64_t max_pages, int64_t n_page
 struct PagesArgs {
     uint8_t *free_pages;
     int32_t *table, *lens, *refs, *failed, *live;
-    int32_t *head, *writers, *last_writer, *picked, *move_from, *word_rank, *word_movers, *row_page, *row_new, *row_copy, *copies, *rows, *pieces;
+    int32_t *grown, *head, *writers, *last_writer, *picked, *move_from, *word_rank, *word_movers, *row_page, *row_new, *row_copy, *copies, *rows, *pieces;
     const uint8_t *managed;
     const int32_t *want;                       // want: the rows' new lengths, or their parents
     uint16_t *k, *v;

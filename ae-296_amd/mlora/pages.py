@@ -2,7 +2,7 @@
 
     pages = KVPages(cache, n_req, max_pages)
     pages.resize(want)                              # new lengths: pages handed out, given back, copied where they are shared
-    batch = KVBatch(tok_req, tok_pos, pages.table, ...)
+    batch = KVBatch(pages.grown, pages.lens - 1, pages.table, ...)      # one new token a row, for the rows that could be served
     ...
     pages.fork(parent)                              # beams, or more answers to one prompt
 
@@ -43,6 +43,9 @@ class KVPages:
         self.lens, self.refs = self.state[lens:refs], self.state[refs:failed]
         self.failed = self.state[failed:live]          # rows that resize or fork could not serve, added up until it is cleared
         self.live = self.state[live:words]             # pages in use, as of the last compact
+        # r where the last resize made row r longer, else -1 (all of them after fork and adopt); not part of a snapshot
+        self.grown = self.scratch[table:table + n_req]
+        self.grown.fill_(-1)
         self.table.fill_(-1)
         self.take(cache.free_pages if n_pages is None else n_pages)
 
@@ -94,12 +97,17 @@ class KVPages:
         self.lens.copy_(n)
         self.refs.copy_(refs[:N])
         self._free.copy_(self._managed.bool() & (self.refs == 0))
+        self.grown.fill_(-1)
 
     def resize(self, want: torch.Tensor) -> None:
         """Rows' new lengths, int32 [n_req] on the device and not `lens` itself (negative: as it is; 0 gives all pages back).  Shorter
         rows give pages back first; then longer rows, in their order, get the lowest free ids.  A longer row that will write on a page other
         rows name as well gets its own copy of what that holds, in all layers - the last of them keeps the page if all of them do.  A row
-        that does not fit keeps its length and pages and counts in `failed`; so does every later one that needs a page."""
+        that does not fit keeps its length and pages and counts in `failed`; so does every later one that needs a page.
+
+        A step appends to rows that got longer and to no others, from their old length on: a row that was not served still names the page that it was
+        refused a copy of, and what is appended there replaces other rows' tokens.  `grown` says which rows these are, on the device: as the ``tok_req`` of
+        a batch of one token a row (the others are then left alone, their outputs zeros), or by ``grown[row]`` for several tokens a row."""
         rc = _ext.host().pages_resize(self, want)
         if rc:
             _ext.check(rc)

@@ -539,16 +539,20 @@ int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const
  * ceil(lens[r] / page_tokens)), -1 behind them.  Pages outside the managed ones are never handed out, copied or moved.
  *   mlora_pages_layout writes the offsets of the state's parts, in int32 words: at[0] free (a byte a page, padded with zeros to 64 of them: 1
  *     where it is managed and named by no entry), [1] table, [2] lens, [3] refs [n_pages], [4] failed, [5] live, [6] the state's length; and [7] the scratch's
- *     length, whose first words are the managed pages' bytes, likewise.  The rest of the scratch starts as zeros; both buffers belong to these calls, which must be
- *     ordered on one stream.
+ *     length, whose first words are the managed pages' bytes, likewise, and behind them, from word at[1] on, grown[n_req].  The rest of the scratch starts as zeros; both
+ *     buffers belong to these calls, which must be ordered on one stream.
  *   mlora_pages_resize gives rows new lengths want[r] (device int32; negative: the row is left as it is).  First every shorter row's pages
  *     behind its new end are given back.  Then every longer row gets the pages it lacks; where its last page is only partly filled and other
  *     entries name it too, it gets a copy of the page's filled part, in keys and values of all layers, and names that instead - but
  *     for the last such row, if all that name the page are such rows.  Free pages are handed out in ascending order, to the rows in their order, a copy
  *     before the rest.  A longer row is served if the pages asked for by it and the rows before it are there, or if it asks for none and shares
  *     nothing that it writes on; otherwise it keeps its length and pages, and is counted in `failed`, as is a row of more than max_pages pages.
+ *     grown[r] is r where the call made row r longer and -1 for every other row.  Only tokens from a row's old length on, of a row that got longer, may
+ *     be written: the last page of another may be shared, and a token appended to it would replace one of whoever shares it.  With one new token a row,
+ *     grown serves as tok_req of the calls above as it is.
  *   mlora_pages_fork: row r goes on from row parent[r]'s tokens (negative or r: from its own), all rows at once: it gives its own pages back
- *     and names the parent's.  A parent of n_req or more leaves the row as it is and is counted in `failed`.
+ *     and names the parent's.  A parent of n_req or more leaves the row as it is and is counted in `failed`.  grown is -1
+ *     for all rows until the next resize.
  *   mlora_pages_compact: with n managed pages in use (left in `live`), those that are not among the n lowest managed ids move, in their order,
  *     to the free ids among these: keys and values of all layers, tables and refs.
  * want and parent must not lie in state or scratch.  k_pages and v_pages: all layers' slabs, [n_layers, n_pages, n_kv_heads, page_tokens,
