@@ -25,16 +25,21 @@ __device__ __forceinline__ int pages_of(int tokens, int shift, int most)
     const int n = (int)(((unsigned)tokens + (1u << shift) - 1u) >> shift);
     return n < most ? n : most;
 }
-// Of N pages at once, so that their counts are asked for together.
+// Of N pages at once, so that their counts are asked for together.  A page that is not managed is counted, but never free.
 template <int N>
 __device__ __forceinline__ void drop_pages(const PagesArgs &p, const int (&page)[N])
 {
     int before[N];
+    uint8_t own[N];
 #pragma unroll
-    for (int u = 0; u < N; u++) before[u] = page[u] >= 0 && page[u] < p.n_pages ? atomicSub(p.refs + page[u], 1) : 0;
+    for (int u = 0; u < N; u++) {
+        const bool exists = page[u] >= 0 && page[u] < p.n_pages;
+        before[u] = exists ? atomicSub(p.refs + page[u], 1) : 0;
+        own[u] = exists ? p.managed[page[u]] : 0;
+    }
 #pragma unroll
     for (int u = 0; u < N; u++)
-        if (before[u] == 1) p.free_pages[page[u]] = 1;
+        if (before[u] == 1 && own[u]) p.free_pages[page[u]] = 1;
 }
 
 // The bytes of 64 pages, 0 or 1, as a word, and back.

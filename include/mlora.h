@@ -536,7 +536,8 @@ int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const
 /*
  * Page tables that live on the device: n_req rows of max_pages page ids each (what page_tbl of the calls above takes), the tokens of every row and
  * the number of table entries that name each page, so that rows may share pages.  A state of one row: lens[r] tokens on the pages table[r][0 ..
- * ceil(lens[r] / page_tokens)), -1 behind them.  Pages outside the managed ones are never handed out, copied or moved.
+ * ceil(lens[r] / page_tokens)), -1 behind them.  Pages outside the managed ones may stand in a table: they are counted and
+ * copied from, but never handed out and never moved.
  *   mlora_pages_layout writes the offsets of the state's parts, in int32 words: at[0] free (a byte a page, padded with zeros to 64 of them: 1
  *     where it is managed and named by no entry), [1] table, [2] lens, [3] refs [n_pages], [4] failed, [5] live, [6] the state's length; and [7] the scratch's
  *     length, whose first words are the managed pages' bytes, likewise, and behind them, from word at[1] on, grown[n_req].  The rest of the scratch starts as zeros; both
