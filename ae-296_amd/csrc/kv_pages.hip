@@ -25,16 +25,21 @@ __device__ __forceinline__ int pages_of(int tokens, int shift, int most)
     const int n = (int)(((unsigned)tokens + (1u << shift) - 1u) >> shift);
     return n < most ? n : most;
 }
-// Of N pages at once, so that their counts are asked for together.
+// Of N pages at once, so that their counts are asked for together.  A page that is not managed is counted, but never free: looked up where the count
+// has come to zero (a fork of 512 rows of up to 4096 pages 13.5 -> 13.8 us, 65536 pages given back by one workgroup 63 -> 72).  Masking free pages where
+// they are read costs a step without any instead: 64 K pages 9.7 -> 10.5 us, 2 M pages 47 -> 70.
 template <int N>
 __device__ __forceinline__ void drop_pages(const PagesArgs &p, const int (&page)[N])
 {
     int before[N];
 #pragma unroll
     for (int u = 0; u < N; u++) before[u] = page[u] >= 0 && page[u] < p.n_pages ? atomicSub(p.refs + page[u], 1) : 0;
+    uint8_t own[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) own[u] = before[u] == 1 ? p.managed[page[u]] : 0;
 #pragma unroll
     for (int u = 0; u < N; u++)
-        if (before[u] == 1) p.free_pages[page[u]] = 1;
+        if (own[u]) p.free_pages[page[u]] = 1;
 }
 
 // The bytes of 64 pages, 0 or 1, as a word, and back.
@@ -59,10 +64,6 @@ __device__ __forceinline__ void store_word(uint8_t *bytes, int word, unsigned lo
         stg16(bytes + (size_t)word * 64 + i * 16, make_uint4(four(b), four(b >> 4), four(b >> 8), four(b >> 12)));
     }
 }
-
-// Which of 64 pages can be handed out.  The byte of a page that is not managed says nothing: what gives pages back marks it like any other, as a look at managed
-// there is one more way to memory behind the count's (512 rows of up to 4096 pages forked: 14.4 us, here 13.8; 256 rows that grow by a token: 9.4 and 9.7).
-__device__ __forceinline__ unsigned long long free_word(const PagesArgs &p, int word) { return load_word(p.free_pages, word) & load_word(p.managed, word); }
 
 // A barrier behind which the workgroup's atomics and stores have been made.
 __device__ __forceinline__ void settled_barrier()
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(ASSIGN_NT) void pages_assign_kernel(const PagesArgs
     const int tid = threadIdx.x;
     const int words = (int)((p.n_pages + 63) >> 6);
     if (tid == 0) { granted = 0; failed = 0; copies = 0; widest = 0; }
-    unsigned long long word = tid < words ? free_word(p, tid) : 0ull;
+    unsigned long long word = tid < words ? load_word(p.free_pages, tid) : 0ull;
     const GrowRow mine = grow_row(p, tid);
     // the page a row will write on, if it has tokens of the row already, and the entries that name it
     auto written = [&](const GrowRow &g, int r) {
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(ASSIGN_NT) void pages_assign_kernel(const PagesArgs
         }
         if (dropped) {                                      // counts and free pages are others now
             if (my_page >= 0) my_refs = read_now(p.refs + my_page);
-            if (tid < words) word = free_word(p, tid);
+            if (tid < words) word = load_word(p.free_pages, tid);
         }
     }
     // which rows write on pages that others name, and how many rows do so on each
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(ASSIGN_NT) void pages_assign_kernel(const PagesArgs
     __builtin_amdgcn_s_waitcnt(0x0f70);                  // behind the barrier the writers' counts can be read
     const bool any_sharing = __syncthreads_or(sharing);
     unsigned count = (unsigned)__builtin_popcountll(word), n_free = 0, word_rank = 0;
-    for (int w = tid + ASSIGN_NT; w < words; w += ASSIGN_NT) count += (unsigned)__builtin_popcountll(free_word(p, w));
+    for (int w = tid + ASSIGN_NT; w < words; w += ASSIGN_NT) count += (unsigned)__builtin_popcountll(load_word(p.free_pages, w));
     // the rows' needs in their order
     unsigned before = 0;
     GrowRow g = mine;
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(ASSIGN_NT) void pages_assign_kernel(const PagesArgs
         const int w = w0 + tid;
         unsigned rank = word_rank;
         if (words > ASSIGN_NT) {
-            if (w0 > 0) word = w < words ? free_word(p, w) : 0ull;
+            if (w0 > 0) word = w < words ? load_word(p.free_pages, w) : 0ull;
             rank = done + block_scan({(unsigned)__builtin_popcountll(word), 0}, lds, total).a;
             done += total.a;
         } else {
@@ -408,10 +409,7 @@ __device__ __forceinline__ int parent_of(const PagesArgs &p, int r)
 __global__ __launch_bounds__(256) void pages_fork_kernel(const PagesArgs p)
 {
     const int pieces = (p.max_pages + ROW_PIECE - 1) / ROW_PIECE, r = blockIdx.x / pieces, i0 = (blockIdx.x - r * pieces) * ROW_PIECE;
-    if (i0 == 0 && threadIdx.x == 0) {
-        if (p.want[r] >= p.n_req) atomicAdd(p.failed, 1);
-        p.grown[r] = -1;                                    // last pages may be shared from now on
-    }
+    if (p.want[r] >= p.n_req && i0 == 0 && threadIdx.x == 0) atomicAdd(p.failed, 1);
     const int of = parent_of(p, r);
     if (of < 0) return;
     const int tokens = p.lens[of], had = pages_of(p.lens[r], p.page_shift, p.max_pages), gets = pages_of(tokens, p.page_shift, p.max_pages);
@@ -443,7 +441,11 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(const PagesArgs p)
 __global__ __launch_bounds__(256) void pages_forked_kernel(const PagesArgs p)
 {
     const int pieces = (p.max_pages + ROW_PIECE - 1) / ROW_PIECE, r = blockIdx.x / pieces, i0 = (blockIdx.x - r * pieces) * ROW_PIECE;
-    if (parent_of(p, r) < 0) return;
+    const bool first = i0 == 0 && threadIdx.x == 0;
+    if (parent_of(p, r) < 0) {
+        if (first) p.grown[r] = -1;                         // last pages may be shared from now on
+        return;
+    }
     const int tokens = p.row_page[r];
     if (p.pieces[blockIdx.x]) {
         int32_t *mine = p.table + (size_t)r * p.max_pages;
@@ -462,7 +464,7 @@ __global__ __launch_bounds__(256) void pages_forked_kernel(const PagesArgs p)
         }
         drop_pages(p, old);
     }
-    if (i0 == 0 && threadIdx.x == 0) p.lens[r] = tokens;
+    if (first) { p.lens[r] = tokens; p.grown[r] = -1; }
 }
 
 int launch_pages_fork(const PagesArgs &a, hipStream_t s)
@@ -483,7 +485,7 @@ __global__ __launch_bounds__(ASSIGN_NT) void pages_moves_kernel(const PagesArgs 
     const int tid = threadIdx.x;
     const int words = (int)((p.n_pages + 63) >> 6);
     // a thread's word of the first round stays in registers
-    const unsigned long long m0 = tid < words ? load_word(p.managed, tid) : 0ull, f0 = tid < words ? m0 & load_word(p.free_pages, tid) : 0ull;
+    const unsigned long long m0 = tid < words ? load_word(p.managed, tid) : 0ull, f0 = tid < words ? load_word(p.free_pages, tid) : 0ull;
     unsigned used = (unsigned)__builtin_popcountll(m0 & ~f0);
     for (int w = tid + ASSIGN_NT; w < words; w += ASSIGN_NT) used += (unsigned)__builtin_popcountll(load_word(p.managed, w) & ~load_word(p.free_pages, w));
     if (tid == 0) border = (int)p.n_pages;
@@ -508,7 +510,7 @@ __global__ __launch_bounds__(ASSIGN_NT) void pages_moves_kernel(const PagesArgs 
     unsigned from = 0, to = 0;
     for (int w0 = 0; w0 < words; w0 += ASSIGN_NT) {
         const int w = w0 + tid;
-        const unsigned long long m = w0 == 0 ? m0 : w < words ? load_word(p.managed, w) : 0ull, f = w0 == 0 ? f0 : w < words ? m & load_word(p.free_pages, w) : 0ull;
+        const unsigned long long m = w0 == 0 ? m0 : w < words ? load_word(p.managed, w) : 0ull, f = w0 == 0 ? f0 : w < words ? load_word(p.free_pages, w) : 0ull;
         const unsigned long long below = B >= w * 64 + 64 ? ~0ull : B <= w * 64 ? 0ull : (1ull << (B - w * 64)) - 1;
         const unsigned long long holes = f & below, movers = m & ~f & ~below;
         s = block_scan({(unsigned)__builtin_popcountll(movers), (unsigned)__builtin_popcountll(holes)}, lds, total);

@@ -58,8 +58,7 @@ class KVPages:
     def give_back(self) -> int:
         """Gives the cache the pages behind the last one in use (all that are free, after ``compact``) and returns how many.
         Waits for the device."""
-        managed = self._managed.cpu().numpy().astype(bool)
-        free = managed & self._free.cpu().numpy().astype(bool)          # of other pages the byte says nothing
+        managed, free = self._managed.cpu().numpy().astype(bool), self._free.cpu().numpy().astype(bool)
         used = np.flatnonzero(managed & ~free)
         ids = np.flatnonzero(free)
         ids = ids[ids > (used[-1] if len(used) else -1)]

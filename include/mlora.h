@@ -539,7 +539,7 @@ int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const
  * ceil(lens[r] / page_tokens)), -1 behind them.  Pages outside the managed ones may stand in a table: they are counted and
  * copied from, but never handed out and never moved.
  *   mlora_pages_layout writes the offsets of the state's parts, in int32 words: at[0] free (a byte a page, padded with zeros to 64 of them: 1
- *     where no entry names it; that of a page that is not managed says nothing), [1] table, [2] lens, [3] refs [n_pages], [4] failed, [5] live, [6] the state's length; and [7] the scratch's
+ *     where it is managed and named by no entry), [1] table, [2] lens, [3] refs [n_pages], [4] failed, [5] live, [6] the state's length; and [7] the scratch's
  *     length, whose first words are the managed pages' bytes, likewise, and behind them, from word at[1] on, grown[n_req].  The rest of the scratch starts as zeros; both
  *     buffers belong to these calls, which must be ordered on one stream.
  *   mlora_pages_resize gives rows new lengths want[r] (device int32; negative: the row is left as it is).  First every shorter row's pages

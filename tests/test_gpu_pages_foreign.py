@@ -34,7 +34,7 @@ def test_pages_given_back(n_req, max_pages):
     say(f"foreign pages given back {n_req} x {max_pages}")
     _, p = tables([([0, 3, 9], 48), ([3, 1], 20)] + [([], 0)] * (n_req - 2), max_pages=max_pages)
     p.resize(ints([16, 0] + [-1] * (n_req - 2)))
-    assert p.refs.tolist() == [1] + [0] * 11 and (p._free & p._managed).nonzero().flatten().tolist() == [1, 2, 4, 5, 6, 7, 8, 10, 11]
+    assert p.refs.tolist() == [1] + [0] * 11 and p._free.nonzero().flatten().tolist() == [1, 2, 4, 5, 6, 7, 8, 10, 11]
     p.resize(ints([0, min(max_pages, 9) * 16] + [-1] * (n_req - 2)))
     assert p.table[1].tolist()[:9] == [1, 2, 4, 5, 6, 7, 8, 10, 11][:max_pages]
     p.resize(ints([0] * n_req))
@@ -46,7 +46,7 @@ def test_pages_dropped_by_a_fork():
     say("foreign pages dropped by a fork")
     _, p = tables([([0, 9], 30), ([1], 5), ([3, 2], 17)])
     p.fork(ints([1, -1, 1]))
-    assert p.refs.tolist() == [0, 3] + [0] * 10 and (p._free & p._managed).nonzero().flatten().tolist() == [2, 4, 5, 6, 7, 8, 10, 11]
+    assert p.refs.tolist() == [0, 3] + [0] * 10 and p._free.nonzero().flatten().tolist() == [2, 4, 5, 6, 7, 8, 10, 11]
     p.resize(ints([16, 5, 64]))
     assert p.failed.tolist() == [0] and not {0, 3, 9} & set(p.table.flatten().tolist())
 
