@@ -519,8 +519,11 @@ int mlora_prefix_attention(void *out, int64_t out_stride, const void *q, int64_t
  *   mlora_mx4_values: the values a packed operand stands for, rounded to the 16-bit type (exact for what was quantised from that type).
  *     In these three, packed may not overlap what it is made from or what is made from it.
  *   mlora_mx4_gemm_multi takes y (16-bit [T, hout]), x and w (packed), hin and hout as HOST arrays of n_proj entries; no y may overlap another y, an x
- *     or a w.  Products exact, sums in fp32, the result rounded once; a block with a NaN makes its results NaN, and where a sum leaves fp32's range
- *     the result is infinite or NaN.
+ *     or a w.  The result is rounded once, from fp32.  The sum of a block's products is exact; the matrix instruction then brings up to four blocks' sums and the
+ *     running sum to one exponent, that of the largest product or sum among them, and cuts each of them, and their sum, off below 2^-23 of that, so small
+ *     blocks beside large ones that cancel are lost.  All in all a result is off by less than (8 ceil(k / 128) + 8) 2^-23 of the sum of its products' magnitudes
+ *     (and y's), besides the rounding.  A block with a NaN makes its results NaN; where a product or a partial sum leaves fp32's range, the result is infinite, of
+ *     either sign, or NaN.
  *   mlora_mx4_form: the output columns (shape[0]) and tokens (shape[1]) of a workgroup of such a call.  Informational.
  * rows <= 2^20 where they are tokens (T), 2^24 otherwise; k <= 2^24.  The counterpart of the reference's quantised base GEMMs with quantised
  * activations (quantize_gemm_int8.py:18,109), in the format of the 4-bit matrix instructions.
