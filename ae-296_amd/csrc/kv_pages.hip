@@ -162,8 +162,9 @@ __device__ __forceinline__ void many_bits(Words &lds, unsigned long long word, u
 // Everything that depends on the order of the rows, in one workgroup, a thread a row at a time.  ONE: no more rows than threads, which then keep theirs
 // in registers.  RELEASE: pages are given back here as well, and there is no launch before this one.
 // Bound by chains of dependent loads, each a way to the last-level cache (the tables were written on other XCDs): lengths -> the row's last page -> its count, the free
-// pages beside them, and where pages are given back or shared the same again behind that.  256 rows, 18471 pages, every sixteenth row needs one: 5.4 us; as many in
-// groups of four that share their last pages, a twentieth of them ending: 12.8.
+// pages beside them, and where pages are given back or shared the same again behind that.  256 rows, 18471 pages, every sixteenth row needs one: 6.0 us; as many in
+// groups of four that share their last pages, a twentieth of them ending: 13.7.  Large caches: a thread reads the bytes of 64 pages in turn, twice where the lowest
+// free page lies far up (2 M pages: 45 us; behind 1.2 M in use 69).
 constexpr unsigned HELD_PICKS = 2048;
 template <bool ONE, bool RELEASE>
 __global__ __launch_bounds__(ASSIGN_NT) void pages_assign_kernel(const PagesArgs p)
@@ -383,8 +384,13 @@ static dim3 row_pieces(const PagesArgs &a) { return dim3((unsigned)a.n_req * (un
 
 int launch_pages_resize(const PagesArgs &a, hipStream_t s)
 {
-    // Pages are given back by the workgroup that hands them out, 4096 at a time, or by a launch of their own: 256 rows of 512 entries, a step in which nobody
-    // ends 8.4 and 9.8 us, one row 10.9 and 11.0, a tenth of them 21.1 and 11.0, all 115 and 10.7
+    // Pages are given back by the workgroup that hands them out, 4096 at a time, up to so many entries, else by a launch of their own.  us a call (and of the
+    // tables put back), the former / the latter, where nobody ends, one row, a tenth of the rows, all rows:
+    //     256 rows of  16 entries    9.1 / 10.1   11.2 / 11.2   11.2 / 11.7    13.6 / 11.0
+    //     256 rows of  64            9.4 / 10.6   11.6 / 11.3   12.7 / 11.8    25.7 / 11.2
+    //     256 rows of 256            9.8 / 11.0   12.5 / 11.7   18.1 / 12.2    72.4 / 11.8
+    //     256 rows of 512           11.1 / 12.2   13.7 / 13.7   25.8 / 13.9   134.6 / 13.5
+    // The line is where a step without an end, which saves the launch at any size, is bought by no more than 60 us of one in which everything ends.
     const bool release = (long long)a.n_req * a.max_pages <= RELEASE_ENTRIES, one = a.n_req <= ASSIGN_NT;
     if (!release) hipLaunchKernelGGL(pages_release_kernel, row_pieces(a), dim3(256), 0, s, a);
     if (one && release) hipLaunchKernelGGL((pages_assign_kernel<true, true>), dim3(1), dim3(ASSIGN_NT), 0, s, a);

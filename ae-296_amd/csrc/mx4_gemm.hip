@@ -398,10 +398,15 @@ __global__ __launch_bounds__(MX_NT * KS) void mx4_tile_kernel(const Mx4Args p)
 // Tiles of 256 x 256, the first `whole` of them whole, and the others, which would be half a round of workgroups or less, as halves of 128 tokens (8000 tokens,
 // 13824 -> 5120, 2.5 rounds: 264 -> 240 us; 5120 -> 2 x 13824, 13.5 rounds: 552 -> 530).
 //
-// What bounds it: power.  A step of a whole tile is 128 matrix instructions, 1024 cycles of each pipe.  On one unit alone it takes 500 ns, 0.86 of the pipes' rate
-// at 2.4 GHz (a barrier a step and one wavefront a pipe); with all units at work 795 ns, where the instructions alone, from registers and on
-// random numbers, take 700 (5.9 to 6.4 PFLOP/s; on ones up to 9.4): the card lowers its clock to 1.7 GHz.  64 rows of either operand in LDS for every 32 read
+// What bounds it: its steps, and the time between tiles.  A step of a whole tile is 128 matrix instructions, 1024 cycles of each pipe.  On one unit alone it takes
+// 500 ns, 0.86 of the pipes' rate at 2.4 GHz (a barrier a step and one wavefront a pipe); with all units at work 795 to 850, where the instructions alone,
+// from registers and on random numbers, take 700 (5.9 to 6.4 PFLOP/s; on ones up to 9.4): the card lowers its clock to 1.7 GHz.  Besides the steps a
+// round of tiles takes 7 to 10 us in which the pipes have nothing (the ring's filling, the results' way out; one workgroup a unit, so nothing runs beside it): of
+// 1225 us for a Llama-13B layer at 8000 tokens, 26 rounds, the steps are 962 and this is 263.  64 rows of either operand in LDS for every 32 read
 // feed the pipes at half of the LDS' rate; 128 x 128 tiles need all of it and run at 1.5 GHz.
+//
+// Accumulating, y is read eight bytes a lane between the writes to LDS: 8000 tokens, 4096 -> 2 x 11008 360 -> 479 us, 13824 -> 5120 246 -> 266; 64 tokens 13.0 -> 14.1
+// and 16.3 -> 16.7.
 template <int DT, bool ACC>
 __global__ __launch_bounds__(MX_NT) void mx4_halves_kernel(const Mx4Args p)
 {
@@ -459,13 +464,14 @@ static int launch_slim(Mx4Args &a, hipStream_t s)
 // ------------------------------------------------------------------ which form
 // A form's time: start + round * m + max(step, m * step_full) * K tiles, with m the workgroups of the busiest compute unit (a workgroup alone is bound by the
 // way of its operands from memory, several share the unit), but not less than the call's bytes take: where forms are alike then, the one for the fewest tokens
-// is taken.  The constants (us) are fitted to 2064 times of sixteen calls (one to three products of a whole, half or quarter layer of Llama-7B and 13B) at 1 to 8000
-// tokens, each form over the range in which it comes near the fastest; fitted and measured times differ by 5 % (few tokens) to 12 % (tiles) on average.  The
-// form with the least time is 0.5 % behind the fastest on average; the worst were 24 to 64 tokens, 5120 -> 2 x 13824 (64 columns x 64 tokens, 16 to 23 % behind
-// 128 columns) and then 1.5 rounds of 256 x 256 tiles (8 % behind 128 x 128).  Examples, with another one:
-//      1 token, 4096 -> 4096: 16 columns x 16 tokens 4.1 us, 32 columns 4.8;     64 tokens: 32 x 32 5.7, 32 columns x 64 tokens 6.9
-//      64 tokens, 4096 -> 2 x 11008: 128 columns x 64 tokens 13.1, 64 x 64 15.5;  512 tokens: 256 x 256 29.8, 128 x 128 32.4
-//      512 tokens, 11008 -> 4096: 128 columns x 64 tokens 23.7, 64 x 64 28.0;     1536 tokens: 256 x 256 in halves 41.4, 128 x 128 41.0
+// is taken.  The constants (us) are fitted to times of sixteen calls (one to three products of a whole, half or quarter layer of Llama-7B and 13B) at 1 to 8000
+// tokens, each form over the range in which it comes near the fastest; fitted and measured times differ by 6 % (few tokens) to 12 % (tiles) on average.  Measured
+// once more with the forms as they are, at 432 sizes, the form with the least time is 0.7 % behind the fastest on average, 8 % or more at
+// eight: 24 to 64 tokens, 5120 -> 2 x 13824 (64 columns x 64 tokens, 14 to 21 % behind 128 columns), 384 tokens, 4096 -> 2 x 5504 (256 x 256, 10 % behind 128 x 128), one
+// token, 4096 -> 2 x 11008 (32 columns, 10 % behind 16), 192 and 256 tokens, 2752 -> 4096 (64 x 64, 8 % behind 128 x 64).  Examples, with another one:
+//      1 token, 4096 -> 4096: 16 columns x 16 tokens 4.4 us, 32 columns 5.0;     64 tokens: 32 x 32 6.0, 32 columns x 64 tokens 7.2
+//      64 tokens, 4096 -> 2 x 11008: 128 columns x 64 tokens 12.8, 64 x 64 15.8;  512 tokens: 256 x 256 29.4, 128 x 128 32.6
+//      512 tokens, 11008 -> 4096: 128 columns x 64 tokens 23.3, 64 x 64 27.5;     1536 tokens: 256 x 256 in halves 44.5, 128 x 128 41.7
 namespace {
 struct Mx4Form {
     int columns, tokens;
