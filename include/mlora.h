@@ -553,7 +553,7 @@ int mlora_mx4_gemm_multi(int n_proj, void *const *y, const void *const *x, const
  *     nothing that it writes on; otherwise it keeps its length and pages, and is counted in `failed`, as is a row of more than max_pages pages.
  *     grown[r] is r where the call made row r longer and -1 for every other row.  Only tokens from a row's old length on, of a row that got longer, may
  *     be written: the last page of another may be shared, and a token appended to it would replace one of whoever shares it.  With one new token a row,
- *     grown serves as tok_req of the calls above as it is.
+ *     grown serves as tok_req of the calls above as it is (before the first resize it holds the scratch's zeros, which would name row 0).
  *   mlora_pages_fork: row r goes on from row parent[r]'s tokens (negative or r: from its own), all rows at once: it gives its own pages back
  *     and names the parent's.  A parent of n_req or more leaves the row as it is and is counted in `failed`.  grown is -1
  *     for all rows until the next resize.
